@@ -671,6 +671,73 @@ int vcb_zw_colsum(int32_t B, int32_t n, const int64_t* off, const int32_t* k,
 
 size_t vcb_zw_colsum_workspace(int64_t total_chunks, int32_t n);
 
+/* ---- Training step of the networks bounded above: linear layer, loss and
+ * optimiser (no reference counterpart).  Matrices are row-major with unit
+ * column stride and a row stride in elements (ld*); element types are vcb_dtype
+ * and all matrices of a call share one.  Accumulation is in fp32. ---- */
+enum vcb_dtype { VCB_F32 = 0, VCB_BF16 = 1, VCB_F16 = 2 };
+enum vcb_act { VCB_ACT_NONE = 0, VCB_ACT_RELU = 1, VCB_ACT_GELU = 2 /* erf */, VCB_ACT_SILU = 3 };
+
+/* Z = X W^T + bias, Y = act(Z) + residual for X (M x K) and W (N x K); bias
+ * (N), residual (M x N) and z (M x N, the pre-activation a backward pass
+ * needs) may be NULL.  workspace: vcb_linear_forward_workspace bytes, 16-byte
+ * aligned (NULL when that is 0). */
+int vcb_linear_forward(int32_t M, int32_t N, int32_t K, int32_t type, const void* x,
+                       int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                       int32_t act, const void* residual, int64_t ldr, void* y,
+                       int64_t ldy, void* z, int64_t ldz, void* workspace,
+                       size_t workspace_bytes, void* stream);
+size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type);
+
+/* Gradients of vcb_linear_forward: with dZ = dY * act'(z), dX = dZ W (M x K),
+ * dW = dZ^T X (N x K), db = sum of dZ over the rows (N); each may be NULL.
+ * z may be NULL when act is VCB_ACT_NONE.  (The residual's gradient is dY.) */
+int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type, const void* dy,
+                        int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const void* z, int64_t ldz, int32_t act, void* dx, int64_t lddx,
+                        void* dw, int64_t lddw, void* db, void* workspace,
+                        size_t workspace_bytes, void* stream);
+size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type);
+
+/* Softmax cross-entropy of logits (R x C) with int64 labels (R), and its
+ * gradient (R x C): loss[0] = mean over the rows whose label is not
+ * ignore_index of logsumexp(x_r) - x_r,label, 0 when there is none; ignored
+ * rows get gradient 0.  A row whose logits are all -inf has loss +inf and
+ * gradient 0; a row whose label is outside [0, C) becomes NaN, and so does the
+ * loss.  workspace: vcb_cross_entropy_workspace(R) bytes, 16-byte aligned. */
+int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
+                      const int64_t* labels, int64_t ignore_index, float* loss, void* grad,
+                      int64_t ldg, void* workspace, size_t workspace_bytes, void* stream);
+size_t vcb_cross_entropy_workspace(int32_t R);
+
+/* One AdamW step over `count` tensors.  Tensor i's moments are the elements
+ * [off, off + n) of the state, off a multiple of 256.  state_bits 32: m and v
+ * are fp32 and the scales unused; 8: m int8 and v uint8 codes with one fp32
+ * scale per 256 elements,
+ *   m = m_scale sgn(c) (c / 127)^2,   v = v_scale (c / 255)^4.
+ * Constants of step t: b1, c1 = 1 - b1, b2, c2 = 1 - b2, eps, size = lr / (1 -
+ * b1^t), root = (1 - b2^t)^-1/2, keep = 1 - lr * weight_decay, and the key of
+ * the 8-bit codes' rounding noise.  Gradients have the weights' type or fp32.
+ * `tensors` is read before the call returns. */
+typedef struct {
+  void* p;
+  const void* g;
+  int64_t n, off;
+} vcb_adamw_tensor;
+
+typedef struct {
+  float b1, c1, b2, c2, eps, size, root, keep;
+  uint32_t key;
+} vcb_adamw_opts;
+
+int vcb_adamw(int32_t count, const vcb_adamw_tensor* tensors, int32_t p_type, int32_t g_type,
+              int32_t state_bits, void* m, void* v, float* m_scale, float* v_scale,
+              const vcb_adamw_opts* opts, void* stream);
+
+/* The values that n (a multiple of 256) elements of an 8-bit state stand for. */
+int vcb_adamw_values(int64_t n, const void* m, const void* v, const float* m_scale,
+                     const float* v_scale, float* m_out, float* v_out, void* stream);
+
 /* Diagnostic: FP32 FFMA throughput probe (no reference counterpart).  Runs
  * `blocks` CTAs of 256 threads, each thread `iters` x 64 dependent-chain FMAs
  * (8 independent chains); FLOPs = blocks * 256 * iters * 128.  `out` must

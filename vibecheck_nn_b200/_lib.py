@@ -41,8 +41,14 @@ class VcbBabOpts(ctypes.Structure):
                 ('boost', ctypes.c_void_p)]
 
 
+class VcbAdamwOpts(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_float) for k in ('b1', 'c1', 'b2', 'c2', 'eps', 'size', 'root',
+                                              'keep')] + [('key', ctypes.c_uint32)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 
 # name -> argtypes; every function returns int (status) unless listed below.
 SIGNATURES = {
@@ -127,6 +133,16 @@ SIGNATURES = {
     'vcb_conv_bias_dot': [_I, _I, _I, _P, _P, _P, _P],
     'vcb_ibp_relu': [_I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P],
     'vcb_relu_back': [_I, _I, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P],
+    'vcb_linear_forward': [_I, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _P, _L, _P,
+                           ctypes.c_size_t, _P],
+    'vcb_linear_forward_workspace': [_I, _I, _I, _I],
+    'vcb_linear_backward': [_I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _L,
+                            _P, _P, ctypes.c_size_t, _P],
+    'vcb_linear_backward_workspace': [_I, _I, _I, _I],
+    'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
+    'vcb_cross_entropy_workspace': [_I],
+    'vcb_adamw': [_I, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts), _P],
+    'vcb_adamw_values': [_L, _P, _P, _P, _P, _P, _P, _P],
     'vcb_bab_step': [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P,
                      _P, _P, _P, _P, _P],
 }
@@ -136,7 +152,10 @@ RESTYPES = {'vcb_last_error': ctypes.c_char_p,
             'vcb_conv_back_workspace': ctypes.c_size_t,
             'vcb_bab_step_wide_workspace': ctypes.c_size_t,
             'vcb_zw_colsum_workspace': ctypes.c_size_t,
-            'vcb_multisub_emit_workspace': ctypes.c_int64}
+            'vcb_multisub_emit_workspace': ctypes.c_int64,
+            'vcb_linear_forward_workspace': ctypes.c_size_t,
+            'vcb_linear_backward_workspace': ctypes.c_size_t,
+            'vcb_cross_entropy_workspace': ctypes.c_size_t}
 
 _lib = None
 
@@ -224,6 +243,31 @@ def workspace(nbytes, device):
 
 def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class _Here:
+    """Context manager that does nothing (the tensor's device is current)."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """Makes ``device`` current for a launch on its stream."""
+    if device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def raw_stream(device):
+    """The current stream of ``device`` as an integer handle."""
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def require_cuda(t, name='tensor'):

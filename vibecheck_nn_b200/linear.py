@@ -1,0 +1,177 @@
+"""Linear layer with its epilogue, and its gradients: the layers of a network
+that is trained here and bounded by the rest of the package.
+
+* ``linear_forward`` -- ``y = act(x W^T + b) + r`` in one product; with
+  ``keep`` also the pre-activation ``z = x W^T + b`` for the backward pass;
+* ``linear_backward`` -- ``dz = dy * act'(z)``, ``dx = dz W``, ``dW = dz^T x``
+  and ``db``;
+* ``linear`` -- the same as a differentiable function.
+
+``x`` is (..., K), ``weight`` (N, K) as in a ``gg`` dict's fc layer.  float32,
+bfloat16 and float16, one type per call; sums are held in float32 and each
+output is rounded once.  In float32 a product keeps float32 accuracy (operands
+are split, not rounded, for the tensor cores).  ``act`` is one of 'none',
+'relu', 'gelu' (with erf) and 'silu'; a ReLU's slope at 0 is 0.  Work runs on
+the current stream of ``x``'s device; like the tensor-core bounds, a caller
+can ask ``_lib.fault_check`` whether a bounded device wait ran out.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTS = {'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3}
+
+
+def type_of(t, name):
+    """vcb_dtype of a CUDA tensor; refuses what the kernels do not take."""
+    _lib.require_cuda(t, name)
+    code = TYPES.get(t.dtype)
+    if code is None:
+        raise _lib.UnsupportedInput(f'vibecheck_nn_b200: {name} must be float32, bfloat16 or '
+                                    f'float16 (got {t.dtype})')
+    return code
+
+
+def rows_of(t, cols, like, name):
+    """``t`` (..., cols) as rows with unit column stride -> (tensor, row
+    stride); copies only what no row stride describes."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f'{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}')
+    if t.dim() < 1 or t.shape[-1] != cols:
+        raise ValueError(f'{name}: shape {tuple(t.shape)}, expected (..., {cols})')
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.new_empty((t.shape[:-1].numel(), 0))
+    rows = t.shape[0]
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        t = t.contiguous()
+        ld = cols
+    return t, ld
+
+
+def _act(act):
+    code = ACTS.get(act)
+    if code is None:
+        raise ValueError(f'act {act!r}: one of {sorted(ACTS)}')
+    return code
+
+
+def _weight(x, weight):
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError('weight must be (N, K)')
+    N, K = weight.shape
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f'weight: {weight.dtype} on {weight.device}, expected {x.dtype} on '
+                         f'{x.device}')
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f'x: shape {tuple(x.shape)}, expected (..., {K})')
+    return N, K
+
+
+def linear_forward(x, weight, bias=None, act='none', residual=None, keep=False):
+    """``act(x W^T + bias) + residual``, shape (..., N); with ``keep`` the pair
+    (y, z)."""
+    ty = type_of(x, 'x')
+    code = _act(act)
+    N, K = _weight(x, weight)
+    lead = x.shape[:-1]
+    x2, ldx = rows_of(x, K, x, 'x')
+    w2, ldw = rows_of(weight, K, x, 'weight')
+    M = x2.shape[0]
+    if bias is not None:
+        bias = _vector(bias, N, x, 'bias')
+    r2, ldr = None, 0
+    if residual is not None:
+        if residual.shape != (*lead, N):
+            raise ValueError(f'residual: shape {tuple(residual.shape)}, expected {(*lead, N)}')
+        r2, ldr = rows_of(residual, N, x, 'residual')
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if keep else None
+    with _lib.on_device(x.device):
+        L = _lib.lib()
+        nbytes = L.vcb_linear_forward_workspace(M, N, K, ty)
+        ws = _lib.workspace(nbytes, x.device)
+        rc = L.vcb_linear_forward(M, N, K, ty, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
+                                  _p(bias), code, _p(r2), ldr, y.data_ptr(), N, _p(z), N,
+                                  _p(ws), nbytes, _lib.raw_stream(x.device))
+    _lib.check(rc, 'vcb_linear_forward')
+    if x.dim() != 2:
+        y = y.view(*lead, N)
+        z = z.view(*lead, N) if keep else None
+    return (y, z) if keep else y
+
+
+def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, True)):
+    """Gradients (dx, dW, db) of ``linear_forward`` for the upstream ``dy``
+    (..., N); ``z`` is the pre-activation (not needed for act 'none').  db is
+    None unless ``bias``; ``need`` switches dx and dW off.  The residual's
+    gradient is ``dy`` itself."""
+    ty = type_of(x, 'x')
+    code = _act(act)
+    N, K = _weight(x, weight)
+    if dy.shape != (*x.shape[:-1], N):
+        raise ValueError(f'dy: shape {tuple(dy.shape)}, expected {(*x.shape[:-1], N)}')
+    g2, ldg = rows_of(dy, N, x, 'dy')
+    x2, ldx = rows_of(x, K, x, 'x')
+    w2, ldw = rows_of(weight, K, x, 'weight')
+    z2, ldz = None, 0
+    if code:
+        if z is None or z.shape != dy.shape:
+            raise ValueError(f'act {act!r} needs z of shape {tuple(dy.shape)}')
+        z2, ldz = rows_of(z, N, x, 'z')
+    M = x2.shape[0]
+    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)  # noqa: E731
+    dx = new(M, K) if need[0] else None
+    dw = new(N, K) if need[1] else None
+    db = new(N) if bias else None
+    with _lib.on_device(x.device):
+        L = _lib.lib()
+        nbytes = L.vcb_linear_backward_workspace(M, N, K, ty)
+        ws = _lib.workspace(nbytes, x.device)
+        rc = L.vcb_linear_backward(M, N, K, ty, g2.data_ptr(), ldg, x2.data_ptr(), ldx,
+                                   w2.data_ptr(), ldw, _p(z2), ldz, code, _p(dx), K, _p(dw), K,
+                                   _p(db), _p(ws), nbytes, _lib.raw_stream(x.device))
+    _lib.check(rc, 'vcb_linear_backward')
+    if dx is not None and x.dim() != 2:
+        dx = dx.view(x.shape)
+    return dx, dw, db
+
+
+def _vector(t, n, like, name):
+    if t.dtype != like.dtype or t.device != like.device or t.shape != (n,):
+        raise ValueError(f'{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected '
+                         f'{like.dtype} ({n},) on {like.device}')
+    return t.contiguous()
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        keep = act != 'none' and any(ctx.needs_input_grad[:3])
+        out = linear_forward(x, weight, bias, act, residual, keep)
+        y, z = out if keep else (out, None)
+        ctx.act = act
+        ctx.save_for_backward(x, weight, z)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        gx, gw, gb = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if gx or gw or gb:
+            dx, dw, db = linear_backward(dy, x, weight, z, ctx.act, gb, (gx, gw))
+        return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None
+
+
+def linear(x, weight, bias=None, act='none', residual=None):
+    """Differentiable ``linear_forward`` (gradients of x, weight, bias and
+    residual)."""
+    return _Linear.apply(x, weight, bias, act, residual)

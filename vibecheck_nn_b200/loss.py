@@ -1,0 +1,61 @@
+"""Softmax cross-entropy with its gradient in one pass over the logits.
+
+* ``cross_entropy_grad`` -- (loss, dlogits) of the mean over labelled rows;
+* ``cross_entropy`` -- the same loss as a differentiable function.
+
+Logits (..., C) in float32, bfloat16 or float16, int64 labels (...).  Rows
+labelled ``ignore_index`` count for nothing and get gradient 0; with no
+labelled row the loss is 0.  A row whose logits are all ``-inf`` has loss
+``inf`` and gradient 0.  Labels are not read back to the host: one outside
+[0, C) makes its row's gradient and the loss NaN.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .linear import rows_of, type_of
+
+
+def cross_entropy_grad(logits, labels, ignore_index=-100):
+    """(loss, d loss / d logits): loss a float32 scalar on the device, the
+    gradient in the logits' type and shape."""
+    ty = type_of(logits, 'logits')
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f'logits: shape {tuple(logits.shape)}, expected (..., C) with C > 0')
+    if not isinstance(labels, torch.Tensor) or labels.dtype != torch.int64 \
+            or labels.device != logits.device or labels.shape != logits.shape[:-1]:
+        raise ValueError(f'labels must be int64 {tuple(logits.shape[:-1])} on {logits.device}')
+    C = logits.shape[-1]
+    x2, ld = rows_of(logits, C, logits, 'logits')
+    labels = labels.contiguous()
+    R = x2.shape[0]
+    grad = torch.empty((R, C), dtype=logits.dtype, device=logits.device)
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    with _lib.on_device(logits.device):
+        L = _lib.lib()
+        nbytes = L.vcb_cross_entropy_workspace(R)
+        ws = _lib.workspace(nbytes, logits.device)
+        rc = L.vcb_cross_entropy(R, C, ty, x2.data_ptr(), ld, labels.data_ptr(), int(ignore_index),
+                                 loss.data_ptr(), grad.data_ptr(), C, ws.data_ptr(), nbytes,
+                                 _lib.raw_stream(logits.device))
+    _lib.check(rc, 'vcb_cross_entropy')
+    return loss, grad if logits.dim() == 2 else grad.view(logits.shape)
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ignore_index):
+        loss, grad = cross_entropy_grad(logits, labels, ignore_index)
+        ctx.save_for_backward(grad)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        grad, = ctx.saved_tensors
+        return (grad * g).to(grad.dtype), None, None
+
+
+def cross_entropy(logits, labels, ignore_index=-100):
+    """Differentiable mean cross-entropy over the labelled rows."""
+    return _CrossEntropy.apply(logits, labels, ignore_index)

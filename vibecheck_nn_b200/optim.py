@@ -1,0 +1,149 @@
+"""AdamW over all tensors of a network in one launch, moments in 32 or 8 bits.
+
+    m = b1 m + (1 - b1) g            v = b2 v + (1 - b2) g^2
+    p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+
+The moments of all tensors lie in one flat buffer; tensor i starts at
+``offsets[i]``, a multiple of 256.  ``state_bits=8`` keeps codes with one
+float32 scale per 256 elements (``m = s sgn(c) (c/127)^2``, ``v = s
+(c/255)^4``): 2 bytes per weight instead of 8.  Codes are rounded up or down
+with the probability that keeps a moment's mean, from a hash of the element's
+place, the step and ``seed``, so a run is repeatable.  A gradient that is not
+finite makes its block of 256 moments NaN.
+
+Weights are updated in place, in float32 arithmetic, rounded once to their own
+type (float32, bfloat16, float16: in 16 bits a step below half a unit in the
+last place is lost); gradients have the weights' type or float32.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _lib
+from .linear import type_of
+
+BLOCK = 256
+_MASK32 = 0xFFFFFFFF
+_TABLE = np.dtype([('p', 'u8'), ('g', 'u8'), ('n', 'i8'), ('off', 'i8')])
+
+
+class AdamW:
+    """Optimiser of the CUDA tensors ``params`` (contiguous, one device)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+                 state_bits=32, seed=0):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError('no parameters')
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits {state_bits}: 8 or 32')
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and lr >= 0):
+            raise ValueError(f'lr {lr}, betas {betas}, eps {eps}')
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.state_bits, self.seed, self.t = state_bits, int(seed), 0
+        self.device = self.params[0].device
+        self._types = [type_of(p, f'parameter {i}') for i, p in enumerate(self.params)]
+        self._shapes = [p.shape for p in self.params]
+        self._table = np.zeros(len(self.params), _TABLE)
+        self.offsets, total = [], 0
+        for i, p in enumerate(self.params):
+            if p.device != self.device or not p.is_contiguous():
+                raise ValueError(f'parameter {i}: must be contiguous on {self.device}')
+            self.offsets.append(total)
+            self._table[i] = (0, 0, p.numel(), total)
+            total += -(-p.numel() // BLOCK) * BLOCK
+        new = lambda n, dt: torch.zeros(n, dtype=dt, device=self.device)  # noqa: E731
+        if state_bits == 32:
+            self.m, self.v = new(total, torch.float32), new(total, torch.float32)
+            self.m_scale = self.v_scale = None
+        else:
+            self.m, self.v = new(total, torch.int8), new(total, torch.uint8)
+            self.m_scale = new(total // BLOCK, torch.float32)
+            self.v_scale = new(total // BLOCK, torch.float32)
+
+    def _opts(self):
+        b1, b2 = self.betas
+        t = self.t
+        return _lib.VcbAdamwOpts(b1, 1 - b1, b2, 1 - b2, self.eps, self.lr / (1 - b1 ** t),
+                                 (1 - b2 ** t) ** -0.5, 1 - self.lr * self.weight_decay,
+                                 (self.seed * 0xBB67AE85 + t * 0x6A09E667) & _MASK32)
+
+    def step(self, grads=None):
+        """One step with ``grads`` (by default every parameter's ``.grad``); a
+        parameter whose gradient is None stays as it is."""
+        ps = self.params
+        grads = [p.grad for p in ps] if grads is None else list(grads)
+        if len(grads) != len(ps):
+            raise ValueError(f'{len(grads)} gradients for {len(ps)} parameters')
+        kinds = {}
+        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
+            if g is None:
+                continue
+            if g.shape != shape or g.device != self.device:
+                raise ValueError(f'gradient {i}: {tuple(g.shape)} on {g.device}, expected '
+                                 f'{tuple(shape)} on {self.device}')
+            if not g.is_contiguous():
+                grads[i] = g = g.contiguous()
+            kinds.setdefault((self._types[i], g.dtype), []).append(i)
+        for pt, dtype in kinds:
+            if dtype != torch.float32 and dtype != ps[kinds[pt, dtype][0]].dtype:
+                raise _lib.UnsupportedInput(
+                    f'vibecheck_nn_b200: gradient of type {dtype}; the weights\' or float32')
+        self.t += 1
+        opts = self._opts()
+        with _lib.on_device(self.device):
+            L, st = _lib.lib(), _lib.raw_stream(self.device)
+            for (pt, dtype), idx in kinds.items():
+                tab = self._table if len(idx) == len(ps) else self._table[idx]
+                tab['p'] = [ps[i].data_ptr() for i in idx]
+                tab['g'] = [grads[i].data_ptr() for i in idx]
+                gt = 0 if dtype == torch.float32 else pt
+                rc = L.vcb_adamw(len(idx), tab.ctypes.data, pt, gt, self.state_bits,
+                                 self.m.data_ptr(), self.v.data_ptr(), _p(self.m_scale),
+                                 _p(self.v_scale), ctypes.byref(opts), st)
+                _lib.check(rc, 'vcb_adamw')
+        torch.autograd.graph.increment_version(ps)
+
+    def moments(self):
+        """(m, v) of all tensors as flat float32 buffers (the state itself
+        with 32-bit states, the values the codes stand for with 8-bit ones)."""
+        if self.state_bits == 32:
+            return self.m, self.v
+        n = self.m.numel()
+        m = torch.empty(n, dtype=torch.float32, device=self.device)
+        v = torch.empty(n, dtype=torch.float32, device=self.device)
+        with _lib.on_device(self.device):
+            rc = _lib.lib().vcb_adamw_values(n, self.m.data_ptr(), self.v.data_ptr(),
+                                             self.m_scale.data_ptr(), self.v_scale.data_ptr(),
+                                             m.data_ptr(), v.data_ptr(),
+                                             _lib.raw_stream(self.device))
+        _lib.check(rc, 'vcb_adamw_values')
+        return m, v
+
+    def _buffers(self):
+        names = ('m', 'v') if self.state_bits == 32 else ('m', 'v', 'm_scale', 'v_scale')
+        return {k: getattr(self, k) for k in names}
+
+    def state_dict(self):
+        """The step count, the seed and copies of the state's buffers."""
+        return {'step': self.t, 'seed': self.seed,
+                **{k: t.clone() for k, t in self._buffers().items()}}
+
+    def load_state_dict(self, state):
+        """Takes over a state of the same tensors and ``state_bits``."""
+        for k, t in self._buffers().items():
+            s = state[k]
+            if s.shape != t.shape or s.dtype != t.dtype:
+                raise ValueError(f'state {k}: {s.dtype} {tuple(s.shape)}, expected {t.dtype} '
+                                 f'{tuple(t.shape)}')
+        for k, t in self._buffers().items():
+            t.copy_(state[k])
+        self.t = int(state['step'])
+        self.seed = int(state.get('seed', self.seed))
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
