@@ -41,6 +41,111 @@ __device__ __forceinline__ float act_grad(float dy, float z, int act) {
   return dy * act_slope(z, act);
 }
 
+// Where a product's rows go and what is done to them on the way.
+struct Epilogue {
+  void *out, *z;
+  const void *bias, *res;
+  long long ldo, ldz, ldr;
+  int act;
+  int vec;  // out, z and res take 4-element vectors
+};
+
+inline bool vector_rows(const Epilogue& e, int elem) {
+  const auto ok = [&](const void* p, long long ld) {
+    return !p || (reinterpret_cast<uintptr_t>(p) % (4 * elem) == 0 && ld % 4 == 0);
+  };
+  return ok(e.out, e.ldo) && ok(e.z, e.ldz) && ok(e.res, e.ldr);
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void act_all(float (&v)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) v[c] = act_value(v[c], ACT);
+}
+
+// Bias of the columns j .. j + 3.
+template <typename T>
+__device__ __forceinline__ void bias_at(const Epilogue& e, int J, int j, float (&b)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    b[k] = e.bias && j + k < J ? to_f32(static_cast<const T*>(e.bias)[j + k]) : 0.f;
+}
+
+// v[c] of lane l: column c of row l.  Afterwards v[4 q + k] is column 4 q + l % 4
+// of row (l - l % 4) + k: four lanes have traded 4 x 4 blocks.
+__device__ __forceinline__ void transpose16(float (&v)[16], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+  for (int q = 0; q < 16; q += 4) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[q + k] : v[q + k + 1], 1);
+      if (odd) v[q + k] = got; else v[q + k + 1] = got;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float got = __shfl_xor_sync(0xffffffffu, high ? v[q + k] : v[q + k + 2], 2);
+      if (high) v[q + k] = got; else v[q + k + 2] = got;
+    }
+  }
+}
+
+// Rows i, i + 4, .. (N of them), columns j .. j + 3 of the output: bias,
+// pre-activation, act, residual, one rounding.
+template <typename T, int N>
+__device__ __forceinline__ void emit(const Epilogue& e, int I, int J, int i, int j,
+                                     const float (&bias)[4], float (&v)[4 * N]) {
+  if (j >= J) return;
+  const bool vec = e.vec && j + 4 <= J;
+  float r[4 * N];
+  if (e.res) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const T* at = static_cast<const T*>(e.res) + (i + 4 * q) * e.ldr + j;
+      float t[4] = {};
+      if (i + 4 * q < I) {
+        if (vec) {
+          load4(at, t);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (j + k < J) t[k] = to_f32(at[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[4 * q + k] = t[k];
+    }
+  }
+  const auto put = [&](void* base, long long ld) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      if (i + 4 * q >= I) break;
+      T* at = static_cast<T*>(base) + (i + 4 * q) * ld + j;
+      if (vec) {
+        store4(at, {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (j + k < J) at[k] = from_f32<T>(v[4 * q + k]);
+      }
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < 4 * N; ++c) v[c] += bias[c & 3];
+  if (e.z) put(e.z, e.ldz);
+  switch (e.act) {
+    case VCB_ACT_RELU: act_all<VCB_ACT_RELU>(v); break;
+    case VCB_ACT_GELU: act_all<VCB_ACT_GELU>(v); break;
+    case VCB_ACT_SILU: act_all<VCB_ACT_SILU>(v); break;
+    default: break;
+  }
+  if (e.res) {
+#pragma unroll
+    for (int c = 0; c < 4 * N; ++c) v[c] += r[c];
+  }
+  put(e.out, e.ldo);
+}
+
 struct Fwd {
   int M, N, K, type, act;
   long long ldx, ldw, ldr, ldy, ldz;
@@ -54,6 +159,19 @@ struct Bwd {
   const void *dy, *x, *w, *z;
   void *dx, *dw, *db;
 };
+
+// Tensor-core paths (vcb_linear_tc.cu: 16-bit types).  `bytes`: what they need
+// of the workspace; the launch functions take one that large, 16-byte aligned.
+bool tc_forward_fits(const Fwd& f);
+size_t tc_forward_bytes(int M, int N, int K);
+int tc_forward(const Fwd& f, void* ws, cudaStream_t st);
+bool tc_backward_fits(const Bwd& b);
+size_t tc_backward_bytes(int M, int N, int K);
+int tc_backward(const Bwd& b, void* ws, cudaStream_t st);
+
+// Reads and clears the fault word of the tensor-core kernels after
+// synchronising st; *was_set = 1 when a bounded wait had run out.
+int linear_fault_take(cudaStream_t st, int* was_set);
 
 }  // namespace lin
 }  // namespace vcb

@@ -1,0 +1,981 @@
+// The linear layer's products in 16-bit types on the tensor cores
+// (tcgen05.mma kind::f16, fp32 accumulators in tensor memory).
+//
+// Every product of the layer is  out(i, j) = sum_t B(i, t) A(j, t)  with j the
+// contiguous index of the output:
+//   forward  Y  (i = m, j = n, t = k):  A = W    B = X
+//   dX          (i = m, j = k, t = n):  A = W^T  B = dZ
+//   dW          (i = n, j = k, t = m):  A = X^T  B = dZ^T
+// The MMA's M rows (tensor memory lanes) are the j's: neighbouring lanes then
+// store neighbouring elements of a row of the output, so the epilogue needs no
+// staging, a bias is one register per lane, and few rows i cost only a narrow
+// MMA (N = 16 for up to 16 tokens).  Transposed operands are read as they lie:
+// a 16-bit operand of tcgen05.mma may be contiguous along its row index
+// ("MN-major") as well as along t ("K-major"); TMA brings 64 x 64 boxes with
+// 128-byte swizzle for the former.
+//
+// Two kernels:
+//  * pair_kernel, large products: two CTAs per 256 x 256 tile
+//    (cta_group::2), persistent, six 32 KB stages per CTA, two accumulators in
+//    tensor memory so that a tile's epilogue overlaps the next tile's MMAs.  A
+//    single CTA's 128 x 256 tile would need 96 B per cycle and SM from L2 at
+//    full MMA rate, the pair needs 64.
+//  * split_kernel, everything else: a 128 x bn tile, its contraction cut over
+//    the up to 8 CTAs of a cluster when there are few tiles (few tokens: the
+//    weight is what is read, and every SM takes part in reading it).  The
+//    partial sums are joined over distributed shared memory in the order of
+//    the ranks: no atomics, no second launch, the same bits every time.
+// Every mbarrier wait is bounded: when one runs out the CTA raises the fault
+// word (vcb_fault_check), writes NaN to the tiles it has not finished, waits
+// for its copies and MMAs in flight, frees its tensor memory and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "vcb_linear.cuh"
+#include "vcb_tcgen05.cuh"
+
+namespace vcb {
+namespace lin {
+namespace {
+
+using namespace tc5;
+
+__device__ int g_linear_fault;
+std::atomic<bool> g_launched{false};
+
+constexpr int kBK = 64;                      // contraction per stage: 128 bytes
+constexpr int kTileJ = 128;                  // MMA rows of one CTA
+constexpr int kBytesA = kTileJ * kBK * 2;    // 16 KB
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kMostStages = 12;
+constexpr unsigned kSpinLimit = 1u << 20;    // pipeline waits (a stage is microseconds)
+constexpr unsigned kDoneLimit = 1u << 24;    // waits for a whole mainloop
+
+struct alignas(64) Prod {
+  CUtensorMap a, b;
+  int J, I, T;
+  int a_mn, b_mn;
+  int bn;                // columns of the tile (rows i), a multiple of 16
+  int tiles_j, tiles_i;
+  int nk;                // stages of a full contraction
+  uint32_t idesc;
+  Epilogue epi;
+};
+
+struct Launch {
+  Prod p[2];
+  int units0, units;  // tiles of the first product, of both
+  int split;          // split_kernel: CTAs per tile of the first product (cluster size)
+  int stages;
+};
+
+// One lane of a converged warp.  The producer's and the issuer's loops are run
+// by all 32 lanes and only the instruction itself by the elected one: what it
+// takes (descriptors, addresses, the instruction word) is then uniform over the
+// warp and stays in uniform registers.  Run by lane 0 alone, every operand went
+// through a vector register first: 620 cycles per stage instead of the MMAs'.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ uint32_t ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+          : "memory");
+}
+
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, unsigned parity, unsigned limit,
+                                                  const volatile int* abort) {
+  const uint32_t a = smem_u32(bar);
+  for (unsigned i = 0; i < limit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255) == 255 && *abort) return false;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                       int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// As tma_2d for a CTA pair: `bar` may lie in the other CTA of the pair.
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// One operand's rows [row, row + rows) x contraction [t, t + 64).  K-major: one
+// box of `rows` rows; MN-major: boxes of 64 (rows) x 64 (t), 8 KB each.
+template <bool PAIR>
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                             int mn, int row, int rows, int t) {
+  if (!mn) {
+    if (PAIR) tma_2d_pair(dst, map, bar, t, row); else tma_2d(dst, map, bar, t, row);
+  } else {
+    for (int q = 0; q < rows; q += 64) {
+      if (PAIR) tma_2d_pair(dst + q * 128, map, bar, row + q, t);
+      else tma_2d(dst + q * 128, map, bar, row + q, t);
+    }
+  }
+}
+
+// Shared-memory operand, 128-byte swizzle.  K-major: 8-row groups 1,024 B
+// apart.  MN-major: 64 rows contiguous per t, 8-t groups 1,024 B apart (stride
+// offset), 64-row boxes 8,192 B apart (leading offset).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int mn) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(mn ? 8192 >> 4 : 1) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// Instruction descriptor: D f32, A and B both f16 (0) or bf16 (1).
+uint32_t idesc_16(int type, int M, int N, int a_mn, int b_mn) {
+  const uint32_t f = type == VCB_BF16 ? 1 : 0;
+  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+// One operand's descriptors: of the first stage, and their steps (in the
+// descriptor's 16-byte units) per 16 of the contraction and per stage.  The
+// address field of a descriptor has room for every stage, so adding to the low
+// word suffices.
+struct Desc {
+  uint64_t base;
+  uint32_t k, stage;
+};
+
+__device__ __forceinline__ Desc operand(uint32_t saddr, int mn, uint32_t stage_bytes) {
+  return {operand_desc(saddr, mn), (mn ? 2048u : 32u) >> 4, stage_bytes >> 4};
+}
+
+// The four MMAs of stage s.
+template <bool PAIR>
+__device__ __forceinline__ void mma_stage(uint32_t d, const Desc& a, const Desc& b, uint32_t s,
+                                          uint32_t idesc, bool first) {
+  const uint64_t da = a.base + s * a.stage, db = b.base + s * b.stage;
+#pragma unroll
+  for (int k = 0; k < kBK / 16; ++k)
+    mma_f16<PAIR>(d, da + k * a.k, db + k * b.k, idesc, first && k == 0 ? 0u : 1u);
+}
+
+// A position in a ring of stages and the parity of its use.
+struct Ring {
+  int s = 0;
+  unsigned parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) s = 0, parity ^= 1;
+  }
+};
+
+// Arrive on `bar` of both CTAs of the pair when the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Epilogue of one warp: lanes 32 (warp % 4).. of the accumulator at `acc`,
+// every other chunk of 16 columns (warp / 4).  `ok` false: NaN instead.
+template <typename T>
+__device__ __forceinline__ void tile_epilogue(const Prod& p, uint32_t acc, int warp, int lane,
+                                              int j0, int i0, bool ok) {
+  const Epilogue e = p.epi;
+  const int I = p.I, J = p.J, bn = p.bn;
+  const int j = j0 + (warp & 3) * 32 + (lane & ~3);
+  float bias[4];
+  bias_at<T>(e, J, j, bias);
+  const uint32_t base = acc + ((uint32_t)((warp & 3) * 32) << 16);
+  for (int c = (warp >> 2) * 16; c < bn; c += 32) {
+    if (i0 + c >= I) break;  // warp-uniform
+    uint32_t r[16];
+    if (ok) {
+      tmem_ld16(base + c, r);
+      tmem_wait_ld(r);
+    }
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(r[k]) : NAN;
+    transpose16(v, lane);
+    emit<T, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v);
+  }
+}
+
+// Tile u of a product: eight tile rows i share the tiles j that run beside
+// them, so that concurrent CTAs read few distinct operand rows.
+__device__ __forceinline__ void tile_at(const Prod& p, int u, int& ti, int& tj) {
+  constexpr int G = 8;
+  const int per = G * p.tiles_j, g = u / per, in = u - g * per;
+  const int rows = min(G, p.tiles_i - g * G);
+  ti = g * G + in % rows;
+  tj = in / rows;
+}
+
+constexpr int kPairStages = 6;
+constexpr int kPairStage = 2 * kBytesA;  // per CTA: 128 rows of A and 128 of B
+constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    pair_kernel(const __grid_constant__ Launch L) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages];
+  __shared__ __align__(8) uint64_t acc_full[2], acc_free[2], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const volatile int* vfailed = &failed;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = ctarank();
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&acc_full[q], 1);
+      mbar_init(&acc_free[q], 2 * kEpiWarps);
+    }
+    mbar_init(&done, 1);
+    failed = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // barriers of both CTAs are ready
+  fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+
+  if (warp == kEpiWarps) {
+    {  // TMA producer: this CTA's halves of A and B, counted by the leader
+      const bool one = elect_one();
+      unsigned g = 0;
+      Ring ring;
+      bool ok = true;
+      const uint32_t full0 = map_rank(smem_u32(full), 0);
+      for (int u = first; ok && u < L.units; u += step) {
+        const Prod& p = L.p[u >= L.units0];
+        int ti, tj;
+        tile_at(p, u >= L.units0 ? u - L.units0 : u, ti, tj);
+        const int ja = (tj * 2 + rank) * kTileJ, ib = (ti * 2 + rank) * kTileJ;
+        const int nk = p.nk, a_mn = p.a_mn, b_mn = p.b_mn;
+        for (int kb = 0; kb < nk; ++kb, ++g, ring.next(kPairStages)) {
+          const int s = ring.s;
+          if (g >= kPairStages && !mbar_wait(&empty[s], ring.parity ^ 1, kSpinLimit, vfailed)) {
+            ok = false;
+            break;
+          }
+          if (one) {
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairStage);
+            const uint32_t bar = full0 + s * 8, st = smem + s * kPairStage;
+            load_operand<true>(st, &p.a, bar, a_mn, ja, kTileJ, kb * kBK);
+            load_operand<true>(st + kBytesA, &p.b, bar, b_mn, ib, kTileJ, kb * kBK);
+          }
+        }
+      }
+      if (!ok) failed = 1;
+      if (rank == 0)  // the copies in flight land before the pair leaves
+        for (unsigned k = g > kPairStages ? g - kPairStages : 0; k < g; ++k)
+          if (!mbar_wait(&full[k % kPairStages], (k / kPairStages) & 1, kSpinLimit)) failed = 1;
+    }
+  } else if (warp == kEpiWarps + 1) {
+    if (rank == 0) {  // MMA issuer of the pair
+      const bool one = elect_one();
+      unsigned t = 0;
+      Ring ring;
+      bool ok = true;
+      for (int u = first; ok && u < L.units; u += step, ++t) {
+        const Prod& p = L.p[u >= L.units0];
+        const int q = t & 1, nk = p.nk;
+        const Desc da = operand(smem, p.a_mn, kPairStage);
+        const Desc db = operand(smem + kBytesA, p.b_mn, kPairStage);
+        const uint32_t idesc = p.idesc;
+        if (t >= 2 && !mbar_wait_cluster(&acc_free[q], ((t >> 1) - 1) & 1, kDoneLimit, vfailed)) {
+          ok = false;
+          break;
+        }
+        for (int kb = 0; kb < nk; ++kb, ring.next(kPairStages)) {
+          const int s = ring.s;
+          if (!mbar_wait_cluster(&full[s], ring.parity, kSpinLimit, vfailed)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          if (one) {
+            mma_stage<true>(tmem + q * 256, da, db, s, idesc, kb == 0);
+            commit_pair(&empty[s]);
+          }
+        }
+        if (ok && one) commit_pair(&acc_full[q]);
+      }
+      if (!ok) failed = 1;
+      if (one) commit_pair(&done);  // every MMA has finished before tensor memory is freed
+    }
+    if (!mbar_wait(&done, 0, kDoneLimit)) failed = 1;
+  } else {
+    unsigned t = 0;
+    bool ok = true;
+    for (int u = first; u < L.units; u += step, ++t) {
+      const Prod& p = L.p[u >= L.units0];
+      int ti, tj;
+      tile_at(p, u >= L.units0 ? u - L.units0 : u, ti, tj);
+      const int q = t & 1;
+      ok = ok && mbar_wait(&acc_full[q], (t >> 1) & 1, kDoneLimit, vfailed);
+      ok = __all_sync(0xffffffffu, ok);
+      fence_after_sync();
+      tile_epilogue<T>(p, tmem + q * 256, warp, lane, (tj * 2 + rank) * kTileJ, ti * 2 * kTileJ,
+                       ok);
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                         map_rank(smem_u32(&acc_free[q]), 0))
+                     : "memory");
+    }
+    if (!ok) failed = 1;
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (threadIdx.x == 0 && failed) atomicExch(&g_linear_fault, 1);
+}
+
+__device__ __forceinline__ float peer_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float4 peer_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// One tile per CTA; the tiles of the first product are shared by the
+// L.split CTAs of a cluster, each taking a part of the contraction.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    split_kernel(const __grid_constant__ Launch L) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  __shared__ __align__(8) uint64_t full[kMostStages], empty[kMostStages], acc_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const volatile int* vfailed = &failed;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int size = L.split, rank = blockIdx.x % size, cluster = blockIdx.x / size;
+  // this CTA's tile and part of the contraction
+  const bool second = cluster >= L.units0;
+  const Prod& p = L.p[second];
+  const int u = second ? (cluster - L.units0) * size + rank : cluster;
+  const bool idle = second && u >= p.tiles_i * p.tiles_j;
+  int ti = 0, tj = 0;
+  if (!idle) tile_at(p, u, ti, tj);
+  const int parts = second ? 1 : size, part = second ? 0 : rank;
+  const int k0 = idle ? 0 : static_cast<int>((long long)p.nk * part / parts);
+  const int k1 = idle ? 0 : static_cast<int>((long long)p.nk * (part + 1) / parts);
+  const int stages = L.stages, stage_bytes = kBytesA + p.bn * kBK * 2;
+  const uint32_t columns = max(32, p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&acc_full, 1);
+    failed = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(columns));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  const int j0 = tj * kTileJ, i0 = ti * p.bn;
+  bool ok = true;
+
+  if (warp == kEpiWarps) {
+    {  // TMA producer
+      const bool one = elect_one();
+      int g = 0;
+      Ring ring;
+      const int a_mn = p.a_mn, b_mn = p.b_mn, bn = p.bn;
+      for (int kb = k0; kb < k1; ++kb, ++g, ring.next(stages)) {
+        const int s = ring.s;
+        if (g >= stages && !mbar_wait(&empty[s], ring.parity ^ 1, kSpinLimit, vfailed)) {
+          ok = false;
+          break;
+        }
+        if (one) {
+          mbar_expect_tx(&full[s], stage_bytes);
+          const uint32_t st = smem + s * stage_bytes, bar = smem_u32(&full[s]);
+          load_operand<false>(st, &p.a, bar, a_mn, j0, kTileJ, kb * kBK);
+          load_operand<false>(st + kBytesA, &p.b, bar, b_mn, i0, bn, kb * kBK);
+        }
+      }
+      if (!ok) failed = 1;
+      for (int k = g > stages ? g - stages : 0; k < g; ++k)
+        if (!mbar_wait(&full[k % stages], (k / stages) & 1, kSpinLimit)) failed = 1;
+    }
+  } else if (warp == kEpiWarps + 1) {
+    {  // MMA issuer
+      const bool one = elect_one();
+      Ring ring;
+      const Desc da = operand(smem, p.a_mn, stage_bytes);
+      const Desc db = operand(smem + kBytesA, p.b_mn, stage_bytes);
+      const uint32_t idesc = p.idesc;
+      for (int kb = k0; kb < k1; ++kb, ring.next(stages)) {
+        const int s = ring.s;
+        if (!mbar_wait(&full[s], ring.parity, kSpinLimit, vfailed)) {
+          ok = false;
+          break;
+        }
+        fence_after_sync();
+        if (one) {
+          mma_stage<false>(tmem, da, db, s, idesc, kb == k0);
+          mma_commit(&empty[s]);
+        }
+      }
+      if (!ok) failed = 1;
+      if (one) mma_commit(&acc_full);
+      if (!mbar_wait(&acc_full, 0, kDoneLimit)) failed = 1;
+    }
+  } else {
+    ok = mbar_wait(&acc_full, 0, kDoneLimit) && !*vfailed;
+    ok = __all_sync(0xffffffffu, ok);
+    fence_after_sync();
+    if (parts == 1) {
+      if (!idle) tile_epilogue<T>(p, tmem, warp, lane, j0, i0, ok);
+    } else {
+      // partial sums where the stages were, a column's 128 rows together
+      const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      for (int c = (warp >> 2) * 16; c < p.bn && i0 + c < p.I; c += 32) {
+        uint32_t r[16];
+        tmem_ld16(base + c, r);
+        tmem_wait_ld(r);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(
+                           smem + ((c + k) * kTileJ + (warp & 3) * 32 + lane) * 4),
+                       "f"(ok ? __uint_as_float(r[k]) : NAN)
+                       : "memory");
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(columns));
+  if (threadIdx.x == 0 && failed) atomicExch(&g_linear_fault, 1);
+  if (size == 1) return;
+  cluster_sync();
+  if (parts > 1 && warp < kEpiWarps) {
+    // columns are dealt over the ranks and their warps; 4 rows per lane
+    const Epilogue e = p.epi;
+    const int columns = min(p.bn, p.I - i0), j = j0 + lane * 4;
+    float bias[4];
+    bias_at<T>(e, p.J, j, bias);
+    for (int c = rank * kEpiWarps + warp; c < columns; c += size * kEpiWarps) {
+      const uint32_t at = smem + (c * kTileJ + lane * 4) * 4;
+      float v[4] = {};
+      for (int k = 0; k < size; ++k) {
+        const float4 t = peer_f32x4(map_rank(at, k));
+        v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+      }
+      emit<T, 1>(e, p.I, p.J, i0 + c, j, bias, v);
+    }
+  }
+  cluster_sync();  // no CTA leaves while its partial sums are read
+}
+
+// What a backward pass needs first: dz = dy act'(z) in rows that TMA can read,
+// db, and copies of operands whose rows TMA cannot read (not 16-byte aligned).
+struct Copy {
+  const void* src;
+  void* dst;
+  long long lds, ldd, rows;
+  int cols;
+};
+
+struct Prep {
+  int M, N, act, strips;  // strips of 128 columns of dy, 0 for none
+  const void *dy, *z;
+  void *dz, *db;          // either may be NULL
+  long long lddy, ldz, lddz;
+  Copy copy[2];
+  int copies;
+};
+
+constexpr int kPrepCluster = 8, kPrepThreads = 256;
+
+// A cluster of 8 CTAs per strip: each sums its eighth of the rows (a warp per
+// row, 4 columns per lane), rank 0 adds the eight sums in order.  Bound by HBM:
+// dy and z are read and dz is written once.  The remaining CTAs copy.
+template <typename T>
+__global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThreads)
+    prep_kernel(const __grid_constant__ Prep a) {
+  __shared__ float part[kPrepThreads / 32][128];
+  __shared__ float mine[128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int strip = blockIdx.x / kPrepCluster;
+  if (strip < a.strips) {
+    const int rank = blockIdx.x % kPrepCluster, c = strip * 128 + lane * 4;
+    const long long r0 = static_cast<long long>(a.M) * rank / kPrepCluster;
+    const long long r1 = static_cast<long long>(a.M) * (rank + 1) / kPrepCluster;
+    const T *dy = static_cast<const T*>(a.dy), *z = static_cast<const T*>(a.z);
+    const bool vy = reinterpret_cast<uintptr_t>(dy) % 8 == 0 && a.lddy % 4 == 0 && c + 4 <= a.N;
+    const bool vz = reinterpret_cast<uintptr_t>(z) % 8 == 0 && a.ldz % 4 == 0 && c + 4 <= a.N;
+    float sum[4] = {};
+    constexpr int U = 4, W = kPrepThreads / 32;
+    for (long long r = r0 + warp; r < r1; r += U * W) {
+      float g[U][4], t[U][4];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const long long row = r + k * W;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[k][i] = t[k][i] = 0.f;
+        if (row >= r1) continue;
+        if (vy) {
+          load4(dy + row * a.lddy + c, g[k]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < a.N) g[k][i] = to_f32(dy[row * a.lddy + c + i]);
+        }
+        if (a.act == VCB_ACT_NONE) continue;
+        if (vz) {
+          load4(z + row * a.ldz + c, t[k]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < a.N) t[k][i] = to_f32(z[row * a.ldz + c + i]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const long long row = r + k * W;
+        if (row >= r1) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          g[k][i] = act_grad(g[k][i], t[k][i], a.act);
+          sum[i] += g[k][i];
+        }
+        // lddz is a multiple of 8, so a vector that crosses N stays in its row
+        if (a.dz && c < a.N) store4(static_cast<T*>(a.dz) + row * a.lddz + c, g[k]);
+      }
+    }
+    if (a.db) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[warp][lane * 4 + i] = sum[i];
+      __syncthreads();
+      if (threadIdx.x < 128) {
+        float v = 0.f;
+        for (int w = 0; w < kPrepThreads / 32; ++w) v += part[w][threadIdx.x];
+        mine[threadIdx.x] = v;
+      }
+    }
+    cluster_sync();
+    if (a.db && rank == 0 && threadIdx.x < 128) {
+      const int col = strip * 128 + threadIdx.x;
+      float v = 0.f;
+      for (int k = 0; k < kPrepCluster; ++k) v += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
+      if (col < a.N) static_cast<T*>(a.db)[col] = from_f32<T>(v);
+    }
+    cluster_sync();  // no CTA leaves while its sums are read
+    return;
+  }
+  // copies: eight elements per thread, written as one 16-byte vector
+  const long long t0 = (blockIdx.x - a.strips * kPrepCluster) * (long long)kPrepThreads + threadIdx.x;
+  const long long nt = (gridDim.x - a.strips * kPrepCluster) * (long long)kPrepThreads;
+  for (int k = 0; k < a.copies; ++k) {
+    const Copy& q = a.copy[k];
+    const long long vecs = (q.cols + 7) / 8, all = q.rows * vecs;
+    for (long long v = t0; v < all; v += nt) {
+      const long long row = v / vecs;
+      const int c = static_cast<int>(v - row * vecs) * 8;
+      const uint16_t* src = static_cast<const uint16_t*>(q.src) + row * q.lds + c;
+      __align__(16) uint16_t e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(q.dst) + row * q.ldd + c) =
+          *reinterpret_cast<const uint4*>(e);
+    }
+  }
+}
+
+// ---- host ----
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// Row-major (rows x cols) 16-bit matrix in boxes of box_rows x 64 columns.
+int make_map(CUtensorMap* map, const void* p, int rows, int cols, long long ld, int box_rows,
+             const char* who) {
+  const auto fn = encode_fn();
+  if (!fn) return fail(VCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(p), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VCB_ERR_CUDA, "%s: tensor map encode failed (%d)", who, (int)r);
+  return VCB_OK;
+}
+
+}  // namespace
+
+// How a launch cuts its work: pairs, or bn columns and `split` CTAs per tile.
+struct Plan {
+  bool pair;
+  int bn, split;
+};
+
+// Cycles of a launch: rounds of tiles over the SMs times the longer of the MMAs
+// (128 rows take 64 cycles per 16 of the contraction up to 128 columns, then
+// half a cycle a column; a pair's 256 x 256 takes 128) and the operands'
+// way from L2 (about 60 B per cycle and SM), plus a start and an epilogue.
+Plan plan_of(int I, int J, int T, bool pair_possible, bool by64) {
+  const int sms = sm_count();
+  const int nk = std::max(1, (T + kBK - 1) / kBK);
+  const auto ceil = [](long long a, long long b) { return (a + b - 1) / b; };
+  Plan best{false, 16, 1};
+  double least = 1e300;
+  for (int bn : {16, 32, 48, 64, 96, 128, 192, 256}) {
+    if (by64 && bn % 64) continue;  // an MN-major operand comes in boxes of 64
+    const long long tiles = ceil(I, bn) * ceil(J, kTileJ);
+    for (int split : {1, 2, 4, 8}) {
+      if (split > nk) break;
+      const double stage = std::max(4.0 * std::max(64, bn / 2), (kTileJ + bn) * 128 / 60.0);
+      const double rounds = static_cast<double>(ceil(tiles * split, sms));
+      const double t = rounds * (ceil(nk, split) * stage + 2500 + 12.0 * bn) +
+                       (split > 1 ? 1500 + 6.0 * bn : 0);
+      if (t < least) least = t, best = {false, bn, split};
+    }
+  }
+  if (pair_possible) {
+    const long long tiles = ceil(I, 256) * ceil(J, 256);
+    const double t = static_cast<double>(ceil(tiles, sms / 2)) * nk * 540 + 8000;
+    if (t < least) best = {true, 256, 1};
+  }
+  return best;
+}
+
+struct Operand {
+  const void* p;
+  long long ld;
+  bool mn;  // contiguous along its row index, not along the contraction
+};
+
+int set_prod(Prod& r, int type, int I, int J, int T, const Operand& a, const Operand& b, int bn,
+             bool pair, const char* who) {
+  r.I = I, r.J = J, r.T = T;
+  r.a_mn = a.mn, r.b_mn = b.mn;
+  r.bn = bn;
+  const int tj = pair ? 256 : kTileJ;
+  r.tiles_j = (J + tj - 1) / tj;
+  r.tiles_i = (I + bn - 1) / bn;
+  r.nk = std::max(1, (T + kBK - 1) / kBK);
+  r.idesc = idesc_16(type, tj, bn, a.mn, b.mn);
+  const int rows_a = kTileJ, rows_b = pair ? kTileJ : bn;
+  int rc = a.mn ? make_map(&r.a, a.p, T, J, a.ld, kBK, who) : make_map(&r.a, a.p, J, T, a.ld, rows_a, who);
+  if (!rc)
+    rc = b.mn ? make_map(&r.b, b.p, T, I, b.ld, kBK, who) : make_map(&r.b, b.p, I, T, b.ld, rows_b, who);
+  return rc;
+}
+
+template <typename T>
+int launch_tc(Launch& L, const Plan& plan, cudaStream_t st, const char* who) {
+  g_launched = true;
+  if (plan.pair) {
+    const auto kernel = pair_kernel<T>;
+    const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), kPairSmem);
+    if (rc) return rc;
+    const int grid = 2 * std::min(L.units, sm_count() / 2);
+    kernel<<<grid, kThreads, kPairSmem, st>>>(L);
+    return check_launch(who);
+  }
+  const auto kernel = split_kernel<T>;
+  const int bn = std::max(L.units0 ? L.p[0].bn : 0, L.units > L.units0 ? L.p[1].bn : 0);
+  const int nk = std::max(L.units0 ? (L.p[0].nk + plan.split - 1) / plan.split : 0,
+                          L.units > L.units0 ? L.p[1].nk : 0);
+  const int stage = kBytesA + bn * kBK * 2;
+  const long long clusters =
+      L.units0 + (L.units - L.units0 + plan.split - 1LL) / plan.split;
+  // two CTAs per SM overlap one's epilogue with the other's loads
+  const int room = clusters * plan.split > sm_count() ? 100 << 10 : 200 << 10;
+  L.stages = std::max(2, std::min({kMostStages, nk, room / stage}));
+  L.split = plan.split;
+  const int smem = std::max(L.stages * stage, plan.split > 1 ? bn * kTileJ * 4 : 0) + 1024;
+  const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - 1024);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * plan.split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = plan.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return check_launch(who);
+}
+
+int launch_type(Launch& L, const Plan& plan, int type, cudaStream_t st, const char* who) {
+  return type == VCB_BF16 ? launch_tc<__nv_bfloat16>(L, plan, st, who)
+                          : launch_tc<__half>(L, plan, st, who);
+}
+
+namespace {
+
+constexpr long long kTcLeast = 1LL << 24;  // M N K from which the tensor cores are used
+
+long long pad8(long long n) { return (n + 7) / 8 * 8; }
+size_t matrix_bytes(long long rows, long long cols) {
+  return static_cast<size_t>(rows) * pad8(cols) * 2 + 256;
+}
+
+bool tma_rows(const void* p, long long ld) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0;
+}
+
+// Sizes that 32-bit tile and TMA coordinates describe.
+bool fits(long long M, long long N, long long K) {
+  const long long most = 1LL << 30;
+  return M * N * K >= kTcLeast && M < most && N < most && K < most &&
+         ((M + 15) / 16) * ((N + 127) / 128) < most && ((N + 15) / 16) * ((K + 127) / 128) < most &&
+         ((M + 15) / 16) * ((K + 127) / 128) < most;
+}
+
+// Workspace in 256-byte pieces.
+struct Arena {
+  uint8_t* at;
+  void* take(size_t n) {
+    at = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(at) + 255) & ~uintptr_t{255});
+    void* p = at;
+    at += n;
+    return p;
+  }
+};
+
+// An operand as TMA can read it: itself, or a copy that `prep` makes.
+Operand readable(const void* p, long long ld, int rows, int cols, bool mn, Prep& prep, Arena& ws) {
+  if (tma_rows(p, ld)) return {p, ld, mn};
+  Copy& c = prep.copy[prep.copies++];
+  c = {p, ws.take(matrix_bytes(rows, cols)), ld, pad8(cols), rows, cols};
+  return {c.dst, c.ldd, mn};
+}
+
+int launch_prep(const Prep& a, int type, cudaStream_t st, const char* who) {
+  long long vecs = 0;
+  for (int k = 0; k < a.copies; ++k) vecs += a.copy[k].rows * ((a.copy[k].cols + 7) / 8);
+  const long long ctas = std::min<long long>((vecs + kPrepThreads - 1) / kPrepThreads,
+                                             4LL * sm_count());
+  const long long grid =
+      (a.strips + (ctas + kPrepCluster - 1) / kPrepCluster) * (long long)kPrepCluster;
+  if (grid == 0) return VCB_OK;
+  if (type == VCB_BF16)
+    prep_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), kPrepThreads, 0, st>>>(a);
+  else
+    prep_kernel<__half><<<static_cast<unsigned>(grid), kPrepThreads, 0, st>>>(a);
+  return check_launch(who);
+}
+
+}  // namespace
+
+bool tc_forward_fits(const Fwd& f) { return f.type != VCB_F32 && fits(f.M, f.N, f.K); }
+
+size_t tc_forward_bytes(int M, int N, int K) {
+  return fits(M, N, K) ? matrix_bytes(M, K) + matrix_bytes(N, K) + 256 : 0;
+}
+
+int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
+  const char* who = "vcb_linear_forward";
+  Prep prep{};
+  Arena arena{static_cast<uint8_t*>(ws)};
+  const Operand a = readable(f.w, f.ldw, f.N, f.K, false, prep, arena);
+  const Operand b = readable(f.x, f.ldx, f.M, f.K, false, prep, arena);
+  int rc = launch_prep(prep, f.type, st, who);
+  if (rc) return rc;
+  const Plan plan = plan_of(f.M, f.N, f.K, true, false);
+  Launch L{};
+  Prod& p = L.p[0];
+  rc = set_prod(p, f.type, f.M, f.N, f.K, a, b, plan.bn, plan.pair, who);
+  if (rc) return rc;
+  p.epi = {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
+  p.epi.vec = vector_rows(p.epi, 2);
+  L.units0 = L.units = p.tiles_i * p.tiles_j;
+  return launch_type(L, plan, f.type, st, who);
+}
+
+bool tc_backward_fits(const Bwd& b) {
+  return b.type != VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K);
+}
+
+size_t tc_backward_bytes(int M, int N, int K) {
+  return fits(M, N, K)
+             ? matrix_bytes(M, N) + matrix_bytes(N, K) + matrix_bytes(M, K) + 256
+             : 0;
+}
+
+int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
+  const char* who = "vcb_linear_backward";
+  Prep prep{};
+  Arena arena{static_cast<uint8_t*>(ws)};
+  prep.M = b.M, prep.N = b.N, prep.act = b.act;
+  prep.dy = b.dy, prep.lddy = b.lddy, prep.z = b.z, prep.ldz = b.ldz, prep.db = b.db;
+  Operand dz{b.dy, b.lddy, false};
+  if (b.act != VCB_ACT_NONE || !tma_rows(b.dy, b.lddy)) {
+    prep.lddz = pad8(b.N);
+    prep.dz = arena.take(matrix_bytes(b.M, b.N));
+    dz = {prep.dz, prep.lddz, false};
+  }
+  if (prep.dz || prep.db) prep.strips = (b.N + 127) / 128;
+  Operand w{}, x{};
+  if (b.dx) w = readable(b.w, b.ldw, b.N, b.K, true, prep, arena);
+  if (b.dw) x = readable(b.x, b.ldx, b.M, b.K, true, prep, arena);
+  int rc = launch_prep(prep, b.type, st, who);
+  if (rc) return rc;
+  // dX and dW share a launch when both are pairs; otherwise each is cut its own way
+  const Plan px = plan_of(b.M, b.K, b.N, true, false), pw = plan_of(b.N, b.K, b.M, true, true);
+  Launch L{};
+  Operand dzt = dz;
+  dzt.mn = true;
+  if (b.dx) {
+    rc = set_prod(L.p[0], b.type, b.M, b.K, b.N, w, dz, px.bn, px.pair, who);
+    if (rc) return rc;
+    L.p[0].epi = {b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
+    L.p[0].epi.vec = vector_rows(L.p[0].epi, 2);
+    L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
+  }
+  const bool together = b.dx && b.dw && px.pair == pw.pair;
+  if (b.dx && !together) {
+    rc = launch_type(L, px, b.type, st, who);
+    if (rc) return rc;
+    L.units0 = L.units = 0;
+  }
+  if (b.dw) {
+    Prod& p = L.p[1];
+    rc = set_prod(p, b.type, b.N, b.K, b.M, x, dzt, pw.bn, pw.pair, who);
+    if (rc) return rc;
+    p.epi = {b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+    p.epi.vec = vector_rows(p.epi, 2);
+    L.units += p.tiles_i * p.tiles_j;
+    Plan plan = pw;
+    if (together) plan.split = px.split;
+    if (!together) {  // the only product of its launch
+      L.p[0] = L.p[1];
+      L.units0 = L.units;
+    }
+    rc = launch_type(L, plan, b.type, st, who);
+  }
+  return rc;
+}
+
+int linear_fault_take(cudaStream_t st, int* was_set) {
+  *was_set = 0;
+  if (!g_launched) return VCB_OK;
+  int h = 0;
+  cudaError_t e =
+      cudaMemcpyFromSymbolAsync(&h, g_linear_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && h) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_linear_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  *was_set = h;
+  return cuda_fail(e, "vcb_fault_check");
+}
+
+}  // namespace lin
+}  // namespace vcb
