@@ -681,23 +681,27 @@ enum vcb_act { VCB_ACT_NONE = 0, VCB_ACT_RELU = 1, VCB_ACT_GELU = 2 /* erf */, V
 /* Z = X W^T + bias, Y = act(Z) + residual for X (M x K) and W (N x K); bias
  * (N), residual (M x N) and z (M x N, the pre-activation a backward pass
  * needs) may be NULL.  workspace: vcb_linear_forward_workspace bytes, 16-byte
- * aligned (NULL when that is 0). */
+ * aligned (NULL when that is 0); rows16 = 1 when the rows of x and w all start
+ * on 16-byte boundaries. */
 int vcb_linear_forward(int32_t M, int32_t N, int32_t K, int32_t type, const void* x,
                        int64_t ldx, const void* w, int64_t ldw, const void* bias,
                        int32_t act, const void* residual, int64_t ldr, void* y,
                        int64_t ldy, void* z, int64_t ldz, void* workspace,
                        size_t workspace_bytes, void* stream);
-size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type);
+size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
+                                    int32_t rows16);
 
 /* Gradients of vcb_linear_forward: with dZ = dY * act'(z), dX = dZ W (M x K),
  * dW = dZ^T X (N x K), db = sum of dZ over the rows (N); each may be NULL.
- * z may be NULL when act is VCB_ACT_NONE.  (The residual's gradient is dY.) */
+ * z may be NULL when act is VCB_ACT_NONE.  (The residual's gradient is dY.)
+ * Workspace as above; rows16 speaks of dy, x and w. */
 int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type, const void* dy,
                         int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
                         const void* z, int64_t ldz, int32_t act, void* dx, int64_t lddx,
                         void* dw, int64_t lddw, void* db, void* workspace,
                         size_t workspace_bytes, void* stream);
-size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type);
+size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
+                                     int32_t act, int32_t rows16);
 
 /* Softmax cross-entropy of logits (R x C) with int64 labels (R), and its
  * gradient (R x C): loss[0] = mean over the rows whose label is not

@@ -135,10 +135,10 @@ SIGNATURES = {
     'vcb_relu_back': [_I, _I, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P],
     'vcb_linear_forward': [_I, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _P, _L, _P,
                            ctypes.c_size_t, _P],
-    'vcb_linear_forward_workspace': [_I, _I, _I, _I],
+    'vcb_linear_forward_workspace': [_I, _I, _I, _I, _I],
     'vcb_linear_backward': [_I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _L,
                             _P, _P, ctypes.c_size_t, _P],
-    'vcb_linear_backward_workspace': [_I, _I, _I, _I],
+    'vcb_linear_backward_workspace': [_I, _I, _I, _I, _I, _I],
     'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
     'vcb_cross_entropy_workspace': [_I],
     'vcb_adamw': [_I, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts), _P],
@@ -267,7 +267,7 @@ def on_device(device):
 
 def raw_stream(device):
     """The current stream of ``device`` as an integer handle."""
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def require_cuda(t, name='tensor'):

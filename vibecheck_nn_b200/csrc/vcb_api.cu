@@ -79,12 +79,14 @@ extern "C" int vcb_fault_check(void* stream) {
     return vcb::fail(VCB_ERR_TIMEOUT,
                      "crown_tc_kernel: a bounded device-side wait expired; the bounds of the "
                      "boxes it had not finished are NaN");
-  const int rc2 = vcb::lin::linear_fault_take(static_cast<cudaStream_t>(stream), &set);
-  if (rc2) return rc2;
-  if (set)
-    return vcb::fail(VCB_ERR_TIMEOUT,
-                     "linear layer: a bounded device-side wait expired; the outputs it had not "
-                     "finished are NaN");
+  for (const auto take : {vcb::lin::tc_fault_take, vcb::lin::f32_fault_take}) {
+    const int status = take(static_cast<cudaStream_t>(stream), &set);
+    if (status) return status;
+    if (set)
+      return vcb::fail(VCB_ERR_TIMEOUT,
+                       "linear layer: a bounded device-side wait expired; the outputs it had not "
+                       "finished are NaN");
+  }
   return VCB_OK;
 }
 

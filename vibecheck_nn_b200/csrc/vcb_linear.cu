@@ -224,19 +224,27 @@ bool misaligned(const void* p, int type) {
 
 using namespace vcb;
 
-extern "C" size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type) {
-  if (M <= 0 || N <= 0 || K <= 0 || type == VCB_F32) return 0;
-  return lin::tc_forward_bytes(M, N, K);
+extern "C" size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
+                                               int32_t rows16) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (type == VCB_F32) return lin::f32_forward_bytes(M, N, K);
+  return rows16 ? 0 : lin::tc_forward_bytes(M, N, K);
 }
 
-extern "C" size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type) {
-  if (M <= 0 || N <= 0 || K <= 0 || type == VCB_F32) return 0;
-  return lin::tc_backward_bytes(M, N, K);
+extern "C" size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
+                                                int32_t act, int32_t rows16) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (type == VCB_F32) return lin::f32_backward_bytes(M, N, K);
+  return lin::tc_backward_bytes(M, N, K, act, rows16);
 }
 
 static int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
   if (need == 0 || (ws && have >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0)) return VCB_OK;
   return fail(VCB_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", who, have, need);
+}
+
+static bool rows16(const void* p, int64_t ld, int type) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * dtype_bytes(type) % 16 == 0;
 }
 
 extern "C" int vcb_linear_forward(int32_t M, int32_t N, int32_t K, int32_t type, const void* x,
@@ -254,10 +262,14 @@ extern "C" int vcb_linear_forward(int32_t M, int32_t N, int32_t K, int32_t type,
       misaligned(z, type))
     return fail(VCB_ERR_INVALID, "vcb_linear_forward: NULL or misaligned pointer");
   const lin::Fwd f{M, N, K, type, act, ldx, ldw, ldr, ldy, ldz, x, w, bias, residual, y, z};
-  if (!lin::tc_forward_fits(f)) return lin::small_forward(f, static_cast<cudaStream_t>(stream));
+  const bool f32 = lin::f32_forward_fits(f);
+  if (!f32 && !lin::tc_forward_fits(f)) return lin::small_forward(f, static_cast<cudaStream_t>(stream));
   const int rc = check_workspace(workspace, workspace_bytes,
-                                 vcb_linear_forward_workspace(M, N, K, type), "vcb_linear_forward");
-  return rc ? rc : lin::tc_forward(f, workspace, static_cast<cudaStream_t>(stream));
+                                 vcb_linear_forward_workspace(
+                                     M, N, K, type, rows16(x, ldx, type) && rows16(w, ldw, type)),
+                                 "vcb_linear_forward");
+  if (rc) return rc;
+  return (f32 ? lin::f32_forward : lin::tc_forward)(f, workspace, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type, const void* dy,
@@ -276,8 +288,15 @@ extern "C" int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type
       misaligned(dx, type) || misaligned(dw, type) || misaligned(db, type))
     return fail(VCB_ERR_INVALID, "vcb_linear_backward: NULL or misaligned pointer");
   const lin::Bwd b{M, N, K, type, act, lddy, ldx, ldw, ldz, lddx, lddw, dy, x, w, z, dx, dw, db};
-  if (!lin::tc_backward_fits(b)) return lin::small_backward(b, static_cast<cudaStream_t>(stream));
+  const bool f32 = lin::f32_backward_fits(b);
+  if (!f32 && !lin::tc_backward_fits(b)) return lin::small_backward(b, static_cast<cudaStream_t>(stream));
   const int rc = check_workspace(workspace, workspace_bytes,
-                                 vcb_linear_backward_workspace(M, N, K, type), "vcb_linear_backward");
-  return rc ? rc : lin::tc_backward(b, workspace, static_cast<cudaStream_t>(stream));
+                                 vcb_linear_backward_workspace(
+                                     M, N, K, type, act,
+                                     rows16(dy, lddy, type) && rows16(x, ldx, type) &&
+                                         rows16(w, ldw, type)),
+                                 "vcb_linear_backward");
+  if (rc) return rc;
+  return (f32 ? lin::f32_backward : lin::tc_backward)(b, workspace,
+                                                      static_cast<cudaStream_t>(stream));
 }

@@ -160,18 +160,26 @@ struct Bwd {
   void *dx, *dw, *db;
 };
 
-// Tensor-core paths (vcb_linear_tc.cu: 16-bit types).  `bytes`: what they need
+// Tensor-core paths (vcb_linear_tc.cu: 16-bit types; vcb_linear_f32.cu).  `bytes`: what they need
 // of the workspace; the launch functions take one that large, 16-byte aligned.
 bool tc_forward_fits(const Fwd& f);
 size_t tc_forward_bytes(int M, int N, int K);
 int tc_forward(const Fwd& f, void* ws, cudaStream_t st);
 bool tc_backward_fits(const Bwd& b);
-size_t tc_backward_bytes(int M, int N, int K);
+size_t tc_backward_bytes(int M, int N, int K, int act, bool rows16);
 int tc_backward(const Bwd& b, void* ws, cudaStream_t st);
 
-// Reads and clears the fault word of the tensor-core kernels after
-// synchronising st; *was_set = 1 when a bounded wait had run out.
-int linear_fault_take(cudaStream_t st, int* was_set);
+bool f32_forward_fits(const Fwd& f);
+size_t f32_forward_bytes(int M, int N, int K);
+int f32_forward(const Fwd& f, void* ws, cudaStream_t st);
+bool f32_backward_fits(const Bwd& b);
+size_t f32_backward_bytes(int M, int N, int K);
+int f32_backward(const Bwd& b, void* ws, cudaStream_t st);
+
+// Reads and clears the fault word of the 16-bit / float32 tensor-core kernels
+// after synchronising st; *was_set = 1 when a bounded wait had run out.
+int tc_fault_take(cudaStream_t st, int* was_set);
+int f32_fault_take(cudaStream_t st, int* was_set);
 
 }  // namespace lin
 }  // namespace vcb

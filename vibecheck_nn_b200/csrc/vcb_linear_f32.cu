@@ -1,0 +1,862 @@
+// The linear layer's float32 products on the tensor cores.
+//
+// A float32 operand row is scaled by a power of two, so that its largest entry
+// lies in [2^14, 2^15), and split in two half-precision numbers,
+//   x 2^-e = h + l + d,  h = fp16(x 2^-e),  l = fp16(x 2^-e - h),
+// |d| <= 2^-22 |x| 2^-e (and 2^-40 of the row's largest where l is subnormal).
+// The tensor cores form  h h' + h l' + l h'  with exact products and fp32
+// accumulators; l l' is below 2^-22 of the product and left out.  That is the
+// precision of three TF32 products at twice their rate: fp16 multiplies twice as
+// fast as TF32 and has as many significant bits, and the row scales supply the
+// exponents that it lacks.  A scale belongs to a row along which nothing is
+// summed (a row of the output, or a column of it), so it leaves the product as a
+// factor 2^(e + e').  An infinite or NaN entry makes the outputs of its row
+// infinite or NaN.
+//
+// The tensor cores drop low-order bits in every accumulation.  So an accumulator
+// in tensor memory takes one 64-deep stage (12 MMAs) only, and the epilogue warps
+// add the stages' sums in registers, rounding to nearest, while the next stage
+// fills the other accumulator.
+//
+// Preparation is bound by HBM: forward, one launch reads each row once, finds its
+// scale and writes both halves.  Backward, dz needs row scales for dX and column
+// scales for dW, so a first launch finds all scales (and db, and never stores
+// dz), a second writes the halves.  Then products as in vcb_linear_tc.cu:
+// f32_kernel<256, true> in CTA pairs for large ones, f32_kernel<64 / 128, false>
+// with the contraction cut over a cluster for the rest.
+#include <algorithm>
+#include <atomic>
+
+#include "vcb_linear_tc.cuh"
+
+namespace vcb {
+namespace lin {
+namespace {
+
+__device__ int g_f32_fault;
+std::atomic<bool> g_launched{false};
+
+// Exponent e of the scale 2^-e for a row whose largest |entry| has these bits.
+__device__ __forceinline__ int scale_exp(uint32_t bits) {
+  const int b = static_cast<int>(bits >> 23);
+  if (bits == 0 || b >= 255) return 0;  // all zero, or not finite
+  return max(b - 127 - 14, -126);
+}
+
+__device__ __forceinline__ float exp2i(int k) { return __int_as_float((k + 127) << 23); }
+
+// v 2^e for the sum e of two scale_exp(): in two steps, each in range.
+__device__ __forceinline__ float scaled(float v, int e) {
+  const int h = e >> 1;
+  return v * exp2i(h) * exp2i(e - h);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) {
+  return __float_as_uint(x) & 0x7FFFFFFFu;
+}
+
+// Larger |entry| as bits, NaN left aside: it needs no scale.
+__device__ __forceinline__ uint32_t more(uint32_t m, float x) {
+  const uint32_t b = abs_bits(x);
+  return b > 0x7F800000u ? m : max(m, b);
+}
+
+__device__ __forceinline__ void halves(float x, float scale, __half& h, __half& l) {
+  const float t = x * scale;
+  h = __float2half_rn(t);
+  const float back = __half2float(h);
+  // an infinite h has no remainder
+  l = isinf(back) ? __float2half_rn(0.f) : __float2half_rn(t - back);
+}
+
+__device__ __forceinline__ void put_halves(__half* h, long long plane, const float (&v)[4],
+                                           float scale) {
+  __half a[4], b[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) halves(v[k], scale, a[k], b[k]);
+  *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(a);
+  *reinterpret_cast<uint2*>(h + plane) = *reinterpret_cast<const uint2*>(b);
+}
+
+// Four entries of a row from column c; 0 beyond the last.
+__device__ __forceinline__ void row4(const float* row, int c, int cols, bool vec, float (&v)[4]) {
+  if (vec && c + 4 <= cols) {
+    load4(row + c, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = c + k < cols ? row[c + k] : 0.f;
+  }
+}
+
+// ---- preparation, forward: halves of the rows of two matrices ----
+struct RowJob {
+  const float* src;
+  long long ld, rows;
+  int cols, vec;
+  __half* h;        // rows x ldh, the second halves `plane` elements further
+  long long ldh, plane;
+  uint32_t* most;   // bits of the largest |entry| of each row
+};
+
+struct RowJobs {
+  RowJob j[2];
+};
+
+template <int TPR>  // threads per row
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJobs a) {
+  constexpr int kKeep = 4;  // vectors of a row that stay in registers
+  __shared__ uint32_t warp_most[8];
+  long long r = static_cast<long long>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const bool second = r >= a.j[0].rows;
+  const RowJob& q = a.j[second];
+  if (second) r -= a.j[0].rows;
+  const bool row = r < q.rows;  // uniform over the threads of a row
+  const float* src = q.src + r * q.ld;
+  float v[kKeep][4];
+  uint32_t m = 0;
+  if (row) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      const int c = (k * TPR + t) * 4;
+      row4(src, c, q.cols, q.vec, v[k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = more(m, v[k][i]);
+    }
+    for (int c = (kKeep * TPR + t) * 4; c < q.cols; c += TPR * 4) {
+      float w[4];
+      row4(src, c, q.cols, q.vec, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = more(m, w[i]);
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, warp_most[w]);
+  }
+  if (!row) return;
+  if (t == 0) q.most[r] = m;
+  const float scale = exp2i(-scale_exp(m));
+  __half* h = q.h + r * q.ldh;
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k) {
+    const int c = (k * TPR + t) * 4;
+    if (c < q.cols) put_halves(h + c, q.plane, v[k], scale);
+  }
+  for (int c = (kKeep * TPR + t) * 4; c < q.cols; c += TPR * 4) {
+    float w[4];
+    row4(src, c, q.cols, q.vec, w);
+    put_halves(h + c, q.plane, w, scale);
+  }
+}
+
+// ---- preparation, backward ----
+// A matrix in strips of 128 columns (a warp per row, 4 columns per lane); with z
+// the entries are dz = dy act'(z).
+struct ColJob {
+  const float *src, *z;
+  long long ld, ldz, rows;
+  int cols, vec, act, strips;
+  uint32_t *col_most, *row_most;  // row_most may be NULL; zero on entry
+  float* sum;                     // column sums, or NULL
+  __half *by_col, *by_row;        // halves with column scales; with row scales, or NULL
+  long long ldh, plane;
+};
+
+struct ColJobs {
+  ColJob j[3];
+  int count;
+};
+
+constexpr int kStripCluster = 8, kStripThreads = 256, kStripWarps = kStripThreads / 32;
+
+__device__ __forceinline__ void job4(const ColJob& q, long long r, int c, float (&v)[4]) {
+  row4(q.src + r * q.ld, c, q.cols, q.vec, v);
+  if (q.act == VCB_ACT_NONE) return;
+  float t[4];
+  row4(q.z + r * q.ldz, c, q.cols, q.vec, t);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = act_grad(v[k], t[k], q.act);
+}
+
+// The job and strip of cluster s.
+__device__ __forceinline__ const ColJob& strip_of(const ColJobs& a, int& s) {
+  int k = 0;
+  while (k + 1 < a.count && s >= a.j[k].strips) s -= a.j[k++].strips;
+  return a.j[k];
+}
+
+// Largest entries of every column (a cluster of 8 CTAs per strip, an eighth of the
+// rows each) and of every row (atomic maxima: any order gives the same), column
+// sums in the order of the ranks.
+__global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripThreads)
+    scales_kernel(const __grid_constant__ ColJobs a) {
+  __shared__ float part[kStripWarps][128], sum_mine[128];
+  __shared__ uint32_t most_part[kStripWarps][128], most_mine[128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % kStripCluster;
+  int strip = blockIdx.x / kStripCluster;
+  const ColJob& q = strip_of(a, strip);
+  const int c = strip * 128 + lane * 4;
+  const long long r0 = q.rows * rank / kStripCluster, r1 = q.rows * (rank + 1) / kStripCluster;
+  float sum[4] = {};
+  uint32_t most[4] = {};
+  constexpr int U = 4;
+  for (long long r = r0 + warp; r < r1; r += U * kStripWarps) {
+    float v[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
+      if (r + u * kStripWarps < r1) job4(q, r + u * kStripWarps, c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        most[i] = more(most[i], v[u][i]);
+        sum[i] += v[u][i];
+        m = more(m, v[u][i]);
+      }
+      if (q.row_most) {
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0 && r + u * kStripWarps < r1) atomicMax(q.row_most + r + u * kStripWarps, m);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    part[warp][lane * 4 + i] = sum[i];
+    most_part[warp][lane * 4 + i] = most[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    float s = 0.f;
+    uint32_t m = 0;
+    for (int w = 0; w < kStripWarps; ++w) {
+      s += part[w][threadIdx.x];
+      m = max(m, most_part[w][threadIdx.x]);
+    }
+    sum_mine[threadIdx.x] = s;
+    most_mine[threadIdx.x] = m;
+  }
+  cluster_sync();
+  const int col = strip * 128 + threadIdx.x;
+  if (rank == 0 && threadIdx.x < 128 && col < q.cols) {
+    float s = 0.f;
+    uint32_t m = 0;
+    for (int k = 0; k < kStripCluster; ++k) {
+      s += peer_f32(map_rank(smem_u32(sum_mine + threadIdx.x), k));
+      m = max(m, __float_as_uint(peer_f32(map_rank(smem_u32(most_mine + threadIdx.x), k))));
+    }
+    if (q.sum) q.sum[col] = s;
+    q.col_most[col] = m;
+  }
+  cluster_sync();  // no CTA leaves while its figures are read
+}
+
+constexpr int kHalvesRows = 64;  // rows of a CTA
+
+__global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_constant__ ColJobs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int strip = blockIdx.x;
+  const ColJob& q = strip_of(a, strip);
+  const int c = strip * 128 + lane * 4;
+  if (c >= q.cols) return;
+  float scale[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) scale[i] = c + i < q.cols ? exp2i(-scale_exp(q.col_most[c + i])) : 0.f;
+  const long long end = min(q.rows, (blockIdx.y + 1LL) * kHalvesRows);
+#pragma unroll 2
+  for (long long r = static_cast<long long>(blockIdx.y) * kHalvesRows + warp; r < end;
+       r += kStripWarps) {
+    float v[4];
+    job4(q, r, c, v);
+    if (q.by_row) put_halves(q.by_row + r * q.ldh + c, q.plane, v, exp2i(-scale_exp(q.row_most[r])));
+    if (q.by_col) {
+      __half h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) halves(v[i], scale[i], h[i], l[i]);
+      __half* at = q.by_col + r * q.ldh + c;
+      *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(h);
+      *reinterpret_cast<uint2*>(at + q.plane) = *reinterpret_cast<const uint2*>(l);
+    }
+  }
+}
+
+// ---- products ----
+struct alignas(64) Prod32 {
+  CUtensorMap a, b;  // (64, rows, 2 halves) boxes
+  int J, I, a_mn, b_mn, tiles_j, tiles_i, nk;
+  uint32_t idesc;
+  const uint32_t *most_a, *most_b;  // scales of the rows of A (j) and of B (i)
+  Epilogue epi;
+};
+
+struct Launch32 {
+  Prod32 p[2];
+  int units0, units, split;
+};
+
+template <int BN, bool PAIR>
+struct Cfg {
+  static constexpr int kRowsB = PAIR ? BN / 2 : BN;
+  static constexpr int kBytesB = 2 * kRowsB * 128;
+  static constexpr int kStage = 2 * kBytesA + kBytesB;
+  static constexpr int kStages = 196608 / kStage;
+  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kBufs = BN == 256 ? 2 : 4;
+  static constexpr int kColumns = kBufs * BN;  // of tensor memory
+  static constexpr int kCols = BN / 2;         // of an epilogue thread
+  static constexpr int kArrivals = kEpiWarps * (PAIR ? 2 : 1);
+};
+
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                       int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
+      : "memory");
+}
+
+// Both halves of an operand's rows.  K-major: all h rows, then all l rows.
+// MN-major: per 64 rows, 8 KB of h and 8 KB of l.
+template <bool PAIR>
+__device__ __forceinline__ void load_halves(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int mn, int row, int rows, int t) {
+  if (!mn) {
+    if (PAIR) tma_3d_pair(dst, map, bar, t, row); else tma_3d(dst, map, bar, t, row);
+  } else {
+    for (int q = 0; q < rows; q += 64) {
+      if (PAIR) tma_3d_pair(dst + q * 256, map, bar, row + q, t);
+      else tma_3d(dst + q * 256, map, bar, row + q, t);
+    }
+  }
+}
+
+// One tile of `out` per unit of work.  PAIR: persistent CTA pairs, 256 x 256.
+// Otherwise a 128 x BN tile of the first product per cluster of L.split CTAs, each
+// with a part of the contraction; the parts are joined in the order of the ranks.
+template <int BN, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant__ Launch32 L) {
+  using C = Cfg<BN, PAIR>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
+  __shared__ __align__(8) uint64_t acc_full[C::kBufs], acc_free[C::kBufs], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const volatile int* vfailed = &failed;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = ctarank();
+  const int size = PAIR ? 2 : L.split;
+  const int first = blockIdx.x / size, step = PAIR ? gridDim.x / 2 : L.units;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int q = 0; q < C::kBufs; ++q) {
+      mbar_init(&acc_full[q], 1);
+      mbar_init(&acc_free[q], C::kArrivals);
+    }
+    mbar_init(&done, 1);
+    failed = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(&tmem_slot)),
+                   "r"(C::kColumns));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(&tmem_slot)),
+                   "r"(C::kColumns));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync();  // barriers of both CTAs are ready
+  fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  // the part of a contraction of nk stages
+  const auto begin = [&](int nk) { return PAIR ? 0 : static_cast<int>((long long)nk * rank / size); };
+  const auto end = [&](int nk) {
+    return PAIR ? nk : static_cast<int>((long long)nk * (rank + 1) / size);
+  };
+
+  if (warp == kEpiWarps) {  // TMA producer
+    const bool one = elect_one();
+    unsigned g = 0;
+    Ring ring;
+    bool ok = true;
+    const uint32_t full0 = PAIR ? map_rank(smem_u32(full), 0) : smem_u32(full);
+    for (int u = first; ok && u < L.units; u += step) {
+      const Prod32& p = L.p[u >= L.units0];
+      int ti, tj;
+      tile_at(p.tiles_i, p.tiles_j, u >= L.units0 ? u - L.units0 : u, ti, tj);
+      const int ja = PAIR ? (tj * 2 + rank) * kTileJ : tj * kTileJ;
+      const int ib = PAIR ? (ti * 2 + rank) * C::kRowsB : ti * BN;
+      const int a_mn = p.a_mn, b_mn = p.b_mn, k1 = end(p.nk);
+      for (int kb = begin(p.nk); kb < k1; ++kb, ++g, ring.next(C::kStages)) {
+        const int s = ring.s;
+        if (g >= C::kStages && !mbar_wait(&empty[s], ring.parity ^ 1, kSpinLimit, vfailed)) {
+          ok = false;
+          break;
+        }
+        if (one) {
+          if (!PAIR || rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * C::kStage);
+          const uint32_t bar = full0 + s * 8, st = smem + s * C::kStage;
+          load_halves<PAIR>(st, &p.a, bar, a_mn, ja, kTileJ, kb * kBK);
+          load_halves<PAIR>(st + 2 * kBytesA, &p.b, bar, b_mn, ib, C::kRowsB, kb * kBK);
+        }
+      }
+    }
+    if (!ok) failed = 1;
+    if (!PAIR || rank == 0)  // the copies in flight land before the CTAs leave
+      for (unsigned k = g > C::kStages ? g - C::kStages : 0; k < g; ++k)
+        if (!mbar_wait(&full[k % C::kStages], (k / C::kStages) & 1, kSpinLimit)) failed = 1;
+  } else if (warp == kEpiWarps + 1) {  // MMA issuer
+    if (!PAIR || rank == 0) {
+      const bool one = elect_one();
+      Ring ring, buf;
+      unsigned chunks = 0;
+      bool ok = true;
+      for (int u = first; ok && u < L.units; u += step) {
+        const Prod32& p = L.p[u >= L.units0];
+        const int a_mn = p.a_mn, b_mn = p.b_mn, k1 = end(p.nk);
+        const Desc da = operand(smem, a_mn, C::kStage, 16384);
+        const Desc db = operand(smem + 2 * kBytesA, b_mn, C::kStage, 16384);
+        const uint32_t la = (a_mn ? 8192 : kBytesA) >> 4, lb = (b_mn ? 8192 : C::kBytesB / 2) >> 4;
+        const uint32_t idesc = p.idesc;
+        for (int kb = begin(p.nk); kb < k1;
+             ++kb, ++chunks, ring.next(C::kStages), buf.next(C::kBufs)) {
+          if (!mbar_wait_cluster(&full[ring.s], ring.parity, kSpinLimit, vfailed) ||
+              (chunks >= C::kBufs &&
+               !mbar_wait_cluster(&acc_free[buf.s], buf.parity ^ 1, kDoneLimit, vfailed))) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          if (one) {
+            const uint32_t d = tmem + buf.s * BN;
+            const uint64_t a0 = da.base + ring.s * da.stage, b0 = db.base + ring.s * db.stage;
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) {
+              const uint64_t ah = a0 + k * da.k, bh = b0 + k * db.k;
+              mma_f16<PAIR>(d, ah + la, bh, idesc, k == 0 ? 0u : 1u);
+              mma_f16<PAIR>(d, ah, bh + lb, idesc, 1u);
+              mma_f16<PAIR>(d, ah, bh, idesc, 1u);
+            }
+            if (PAIR) {
+              commit_pair(&empty[ring.s]);
+              commit_pair(&acc_full[buf.s]);
+            } else {
+              mma_commit(&empty[ring.s]);
+              mma_commit(&acc_full[buf.s]);
+            }
+          }
+        }
+      }
+      if (!ok) failed = 1;
+      if (one) {  // every MMA has finished before tensor memory is freed
+        if (PAIR) commit_pair(&done); else mma_commit(&done);
+      }
+    }
+    if (!mbar_wait(&done, 0, kDoneLimit)) failed = 1;
+  } else {
+    constexpr int kCols = C::kCols;
+    const int quad = warp & 3, col0 = (warp >> 2) * kCols;
+    const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + col0;
+    Ring buf;
+    bool ok = true;
+    for (int u = first; u < L.units; u += step) {
+      const Prod32& p = L.p[u >= L.units0];
+      int ti, tj;
+      tile_at(p.tiles_i, p.tiles_j, u >= L.units0 ? u - L.units0 : u, ti, tj);
+      const int j0 = (PAIR ? (tj * 2 + rank) * kTileJ : tj * kTileJ) + quad * 32;
+      const int i0 = ti * BN + col0;
+      const int chunks = end(p.nk) - begin(p.nk);
+      float acc[kCols];
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[k] = 0.f;
+      for (int kb = 0; ok && kb < chunks; ++kb, buf.next(C::kBufs)) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf.s], buf.parity, kDoneLimit, vfailed));
+        if (!ok) break;
+        fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < kCols; c += 32) {
+          uint32_t r[16], s[16];
+          tmem_ld16(base + buf.s * BN + c, r);
+          tmem_ld16(base + buf.s * BN + c + 16, s);
+          tmem_wait_ld(r, s);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            acc[c + k] = __fadd_rn(acc[c + k], __uint_as_float(r[k]));
+            acc[c + 16 + k] = __fadd_rn(acc[c + 16 + k], __uint_as_float(s[k]));
+          }
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                             map_rank(smem_u32(&acc_free[buf.s]), 0))
+                         : "memory");
+          else
+            mbar_arrive(&acc_free[buf.s]);
+        }
+      }
+      if (!ok) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] = NAN;
+      }
+      if (!PAIR && size > 1) {  // partial sums where the stages were
+#pragma unroll
+        for (int k = 0; k < kCols; ++k)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(
+                           smem + ((col0 + k) * kTileJ + quad * 32 + lane) * 4),
+                       "f"(acc[k])
+                       : "memory");
+        break;
+      }
+      const Epilogue e = p.epi;
+      const int I = p.I, J = p.J, j = j0 + (lane & ~3);
+      const int ea = j0 + lane < J ? scale_exp(__ldg(p.most_a + j0 + lane)) : 0;
+      float bias[4];
+      bias_at<float>(e, J, j, bias);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        if (i0 + c < I) {  // warp-uniform
+          const int eb = i0 + c + (lane & 15) < I
+                             ? scale_exp(__ldg(p.most_b + i0 + c + (lane & 15))) : 0;
+          float v[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            v[k] = scaled(acc[c + k], ea + __shfl_sync(0xffffffffu, eb, k));
+          transpose16(v, lane);
+          emit<float, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v);
+        }
+      }
+    }
+    if (!ok) failed = 1;
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (PAIR || size > 1) cluster_sync();
+  if (!PAIR && size > 1) {
+    if (warp < kEpiWarps) {
+      const Prod32& p = L.p[0];
+      int ti, tj;
+      tile_at(p.tiles_i, p.tiles_j, first, ti, tj);
+      const Epilogue e = p.epi;
+      const int i0 = ti * BN, j = tj * kTileJ + lane * 4;
+      const int columns = min(BN, p.I - i0);
+      float bias[4];
+      int ea[4];
+      bias_at<float>(e, p.J, j, bias);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ea[k] = j + k < p.J ? scale_exp(__ldg(p.most_a + j + k)) : 0;
+      for (int c = rank * kEpiWarps + warp; c < columns; c += size * kEpiWarps) {
+        const uint32_t at = smem + (c * kTileJ + lane * 4) * 4;
+        float v[4] = {};
+        for (int k = 0; k < size; ++k) {
+          const float4 t = peer_f32x4(map_rank(at, k));
+          v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+        }
+        const int eb = scale_exp(__ldg(p.most_b + i0 + c));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = scaled(v[k], ea[k] + eb);
+        emit<float, 1>(e, p.I, p.J, i0 + c, j, bias, v);
+      }
+    }
+    cluster_sync();  // no CTA leaves while its partial sums are read
+  }
+  if (warp == 0) {
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"(C::kColumns));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"(C::kColumns));
+  }
+  if (threadIdx.x == 0 && failed) atomicExch(&g_f32_fault, 1);
+}
+
+// ---- host ----
+constexpr long long kTcLeast = 1LL << 26;  // M N K from which the tensor cores are used
+
+long long pad8(long long n) { return (n + 7) / 8 * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t halves_bytes(long long rows, long long cols) { return up256(rows * pad8(cols) * 4); }
+
+// Both halves of a row-major (rows x cols) operand: planes of rows x ld.
+struct Halves {
+  __half* p;
+  int rows, cols;
+  long long ld, plane;
+  uint32_t* most;  // of the rows (or columns) that the product does not sum over
+  bool mn;
+};
+
+struct Arena {
+  uint8_t* at;
+  template <typename T>
+  T* take(size_t bytes) {
+    T* p = reinterpret_cast<T*>(at);
+    at += up256(bytes);
+    return p;
+  }
+};
+
+Halves make_halves(Arena& ws, int rows, int cols, bool mn, uint32_t* most) {
+  Halves h{ws.take<__half>(halves_bytes(rows, cols)), rows, cols, pad8(cols), 0, most, mn};
+  h.plane = h.rows * h.ld;
+  return h;
+}
+
+int make_map(CUtensorMap* map, const Halves& h, int box_rows, const char* who) {
+  const auto fn = encode_fn();
+  if (!fn) return fail(VCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
+  const cuuint64_t dims[3] = {(cuuint64_t)h.cols, (cuuint64_t)h.rows, 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)h.ld * 2, (cuuint64_t)h.plane * 2};
+  const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, 2}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, h.p, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VCB_ERR_CUDA, "%s: tensor map encode failed (%d)", who, (int)r);
+  return VCB_OK;
+}
+
+struct Plan32 {
+  bool pair;
+  int bn, split;
+};
+
+// As the 16-bit products' plan: rounds of tiles over the SMs times the stages'
+// cycles (12 MMAs: 1,536 for a pair's tile, 768 for 64 or 128 columns), plus start
+// and epilogue.
+Plan32 plan_of(int I, int J, int T) {
+  const int sms = sm_count();
+  const auto ceil = [](long long a, long long b) { return (a + b - 1) / b; };
+  const long long nk = std::max<long long>(1, ceil(T, kBK));
+  Plan32 best{true, 256, 1};
+  double least = static_cast<double>(ceil(ceil(I, 256) * ceil(J, 256), sms / 2)) * (nk * 1540 + 4000) + 4000;
+  for (int bn : {64, 128}) {
+    const long long tiles = ceil(I, bn) * ceil(J, kTileJ);
+    for (int split : {1, 2, 4, 8}) {
+      if (split > nk) break;
+      const double t = static_cast<double>(ceil(tiles * split, sms)) *
+                           (ceil(nk, split) * (bn == 64 ? 800 : 1000) + 4000 + 20.0 * bn) +
+                       (split > 1 ? 1500 + 8.0 * bn : 0);
+      if (t < least) least = t, best = {false, bn, split};
+    }
+  }
+  return best;
+}
+
+int set_prod(Prod32& r, int I, int J, int T, const Halves& a, const Halves& b, const Plan32& plan,
+             const Epilogue& epi, const char* who) {
+  r.I = I, r.J = J;
+  r.a_mn = a.mn, r.b_mn = b.mn;
+  const int tj = plan.pair ? 256 : kTileJ;
+  r.tiles_j = (J + tj - 1) / tj;
+  r.tiles_i = (I + plan.bn - 1) / plan.bn;
+  r.nk = std::max(1, (T + kBK - 1) / kBK);
+  r.idesc = idesc_16(VCB_F16, tj, plan.bn, a.mn, b.mn);
+  r.most_a = a.most, r.most_b = b.most;
+  r.epi = epi;
+  r.epi.vec = vector_rows(epi, 4);
+  int rc = make_map(&r.a, a, a.mn ? kBK : kTileJ, who);
+  if (!rc) rc = make_map(&r.b, b, b.mn ? kBK : plan.pair ? kTileJ : plan.bn, who);
+  return rc;
+}
+
+template <int BN, bool PAIR>
+int launch(const Launch32& L, cudaStream_t st, const char* who) {
+  using C = Cfg<BN, PAIR>;
+  g_launched = true;
+  const auto kernel = f32_kernel<BN, PAIR>;
+  const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
+  if (rc) return rc;
+  const int size = PAIR ? 2 : L.split;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return check_launch(who);
+}
+
+int launch_plan(const Launch32& L, const Plan32& plan, cudaStream_t st, const char* who) {
+  if (plan.pair) return launch<256, true>(L, st, who);
+  return plan.bn == 64 ? launch<64, false>(L, st, who) : launch<128, false>(L, st, who);
+}
+
+bool vec16(const void* p, long long ld) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0;
+}
+
+bool fits(long long M, long long N, long long K) {
+  const long long most = 1LL << 28;
+  return M * N * K >= kTcLeast && M < most && N < most && K < most && (M + 63) / 64 * ((N + 127) / 128) < most &&
+         (M + 63) / 64 * ((K + 127) / 128) < most && (N + 63) / 64 * ((K + 127) / 128) < most;
+}
+
+}  // namespace
+
+bool f32_forward_fits(const Fwd& f) { return f.type == VCB_F32 && fits(f.M, f.N, f.K); }
+
+size_t f32_forward_bytes(int M, int N, int K) {
+  if (!fits(M, N, K)) return 0;
+  return halves_bytes(M, K) + halves_bytes(N, K) + up256(M * 4LL) + up256(N * 4LL) + 256;
+}
+
+int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
+  const char* who = "vcb_linear_forward";
+  Arena arena{reinterpret_cast<uint8_t*>(up256(reinterpret_cast<size_t>(ws)))};
+  const Halves w = make_halves(arena, f.N, f.K, false, arena.take<uint32_t>(f.N * 4LL));
+  const Halves x = make_halves(arena, f.M, f.K, false, arena.take<uint32_t>(f.M * 4LL));
+  RowJobs jobs{};
+  const auto job = [](const void* p, long long ld, const Halves& h) {
+    return RowJob{static_cast<const float*>(p), ld, h.rows, h.cols, vec16(p, ld), h.p, h.ld,
+                  h.plane, h.most};
+  };
+  jobs.j[0] = job(f.w, f.ldw, w);
+  jobs.j[1] = job(f.x, f.ldx, x);
+  const long long rows = static_cast<long long>(f.N) + f.M;
+  // a warp per row while that keeps a row in registers, else a CTA
+  if (f.K <= 512)
+    rows_kernel<32><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(jobs);
+  else
+    rows_kernel<256><<<static_cast<unsigned>(rows), 256, 0, st>>>(jobs);
+  int rc = check_launch(who);
+  if (rc) return rc;
+  const Plan32 plan = plan_of(f.M, f.N, f.K);
+  Launch32 L{};
+  rc = set_prod(L.p[0], f.M, f.N, f.K, w, x, plan,
+                {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0}, who);
+  if (rc) return rc;
+  L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
+  L.split = plan.split;
+  return launch_plan(L, plan, st, who);
+}
+
+bool f32_backward_fits(const Bwd& b) {
+  return b.type == VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K);
+}
+
+size_t f32_backward_bytes(int M, int N, int K) {
+  if (!fits(M, N, K)) return 0;
+  return 2 * halves_bytes(M, N) + halves_bytes(N, K) + halves_bytes(M, K) + up256(M * 4LL) +
+         up256(N * 4LL) + 2 * up256(K * 4LL) + 256;
+}
+
+int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
+  const char* who = "vcb_linear_backward";
+  Arena arena{reinterpret_cast<uint8_t*>(up256(reinterpret_cast<size_t>(ws)))};
+  uint32_t* row_most = arena.take<uint32_t>(b.M * 4LL);
+  const Halves dzr = make_halves(arena, b.M, b.N, false, row_most);
+  const Halves dzc = make_halves(arena, b.M, b.N, true, arena.take<uint32_t>(b.N * 4LL));
+  const Halves w = make_halves(arena, b.N, b.K, true, arena.take<uint32_t>(b.K * 4LL));
+  const Halves x = make_halves(arena, b.M, b.K, true, arena.take<uint32_t>(b.K * 4LL));
+  ColJobs jobs{};
+  long long strips = 0, tall = 0;
+  const auto add = [&](const void* p, long long ld, const Halves& h) -> ColJob& {
+    ColJob& q = jobs.j[jobs.count++];
+    q.src = static_cast<const float*>(p);
+    q.ld = ld, q.rows = h.rows, q.cols = h.cols, q.vec = vec16(p, ld);
+    q.strips = (h.cols + 127) / 128;
+    q.col_most = h.most, q.by_col = h.p, q.ldh = h.ld, q.plane = h.plane;
+    strips += q.strips;
+    tall = std::max(tall, q.rows);
+    return q;
+  };
+  ColJob& dz = add(b.dy, b.lddy, dzc);
+  dz.act = b.act, dz.z = static_cast<const float*>(b.z), dz.ldz = b.ldz;
+  if (b.act != VCB_ACT_NONE) dz.vec = dz.vec && vec16(b.z, b.ldz);
+  dz.sum = static_cast<float*>(b.db);
+  if (b.dx) dz.by_row = dzr.p, dz.row_most = row_most;
+  if (!b.dw) dz.by_col = nullptr;
+  if (b.dx) add(b.w, b.ldw, w);
+  if (b.dw) add(b.x, b.ldx, x);
+  if (strips * kStripCluster > 0x7fffffffLL || (tall + kHalvesRows - 1) / kHalvesRows > 65535)
+    return fail(VCB_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d", who, b.M, b.N, b.K);
+  cudaError_t e = cudaSuccess;
+  if (b.dx) e = cudaMemsetAsync(row_most, 0, b.M * 4LL, st);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  scales_kernel<<<static_cast<unsigned>(strips * kStripCluster), kStripThreads, 0, st>>>(jobs);
+  int rc = check_launch(who);
+  if (rc) return rc;
+  halves_kernel<<<dim3(static_cast<unsigned>(strips),
+                       static_cast<unsigned>((tall + kHalvesRows - 1) / kHalvesRows)),
+                  kStripThreads, 0, st>>>(jobs);
+  rc = check_launch(who);
+  if (rc) return rc;
+  const Plan32 px = plan_of(b.M, b.K, b.N), pw = plan_of(b.N, b.K, b.M);
+  const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
+  const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+  Launch32 L{};
+  if (b.dx) {
+    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, px, ex, who);
+    if (rc) return rc;
+    L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
+    L.split = px.split;
+    if (!(b.dw && px.pair && pw.pair)) {  // two pairs share a launch
+      rc = launch_plan(L, px, st, who);
+      if (rc || !b.dw) return rc;
+      L.units0 = L.units = 0;
+    }
+  }
+  Prod32& p = L.p[L.units ? 1 : 0];
+  rc = set_prod(p, b.N, b.K, b.M, x, dzc, pw, ew, who);
+  if (rc) return rc;
+  L.units += p.tiles_i * p.tiles_j;
+  if (!L.units0) L.units0 = L.units;
+  L.split = pw.split;
+  return launch_plan(L, pw, st, who);
+}
+
+int f32_fault_take(cudaStream_t st, int* was_set) {
+  *was_set = 0;
+  if (!g_launched) return VCB_OK;
+  int h = 0;
+  cudaError_t e =
+      cudaMemcpyFromSymbolAsync(&h, g_f32_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && h) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_f32_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  *was_set = h;
+  return cuda_fail(e, "vcb_fault_check");
+}
+
+}  // namespace lin
+}  // namespace vcb

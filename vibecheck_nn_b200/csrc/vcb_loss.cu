@@ -26,7 +26,7 @@ namespace vcb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+
 constexpr int kCountCtas = 64;     // most partial counts of labelled rows
 constexpr int kHeader = 128;       // words: partial counts, then the ticket
 constexpr int kTicket = kCountCtas;
@@ -67,10 +67,15 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// 1 / max(1, labelled rows)
+// 1 / max(1, labelled rows).  A launch of one CTA (parts == 1 and counts == 0)
+// counts its few rows by itself.
 __device__ __forceinline__ float inv_count(const CeArgs& a) {
   int n = 0;
-  for (int i = threadIdx.x & 31; i < a.counts; i += 32) n += a.header[i];
+  if (a.counts == 0) {
+    for (int i = threadIdx.x & 31; i < a.R; i += 32) n += a.y[i] != a.ignore;
+  } else {
+    for (int i = threadIdx.x & 31; i < a.counts; i += 32) n += a.header[i];
+  }
   n = __reduce_add_sync(0xffffffffu, n);
   return 1.f / static_cast<float>(max(n, 1));
 }
@@ -92,6 +97,10 @@ __device__ __forceinline__ float row_loss(float m, float s, float xy) {
 __device__ void finish(const CeArgs& a, int part, double value, float inv) {
   __shared__ int last;
   __shared__ double sums[32];
+  if (a.counts == 0) {
+    if (threadIdx.x == 0) *a.loss = static_cast<float>(value * inv);
+    return;
+  }
   if (threadIdx.x == 0) {
     a.part[part] = value;
     __threadfence();
@@ -317,10 +326,24 @@ __global__ void __launch_bounds__(512) ce_row_kernel(const CeArgs a) {
   if (rank == 0) finish(a, static_cast<int>(r), value, inv);
 }
 
+int launch_count(CeArgs& a, cudaStream_t st) {
+  a.counts = std::min(kCountCtas, (a.R + 4095) / 4096);
+  ce_count_kernel<<<a.counts, 1024, 0, st>>>(a.R, a.y, a.ignore, a.header);
+  return check_launch("vcb_cross_entropy");
+}
+
 template <typename T, int G, int PER>
 int launch_small(CeArgs a, cudaStream_t st) {
   const int rows = 256 / G;
-  a.parts = static_cast<int>(std::min<long long>((a.R + rows - 1LL) / rows, sm_count() * 16LL));
+  // up to four rows per group of lanes: one CTA and no count before it cost less
+  // than a second launch
+  if (a.R <= 4 * rows) {
+    a.parts = 1, a.counts = 0;
+  } else {
+    a.parts = static_cast<int>(std::min<long long>((a.R + rows - 1LL) / rows, sm_count() * 16LL));
+    const int rc = launch_count(a, st);
+    if (rc) return rc;
+  }
   ce_small_kernel<T, G, PER><<<a.parts, 256, 0, st>>>(a);
   return check_launch("vcb_cross_entropy");
 }
@@ -342,6 +365,8 @@ int launch(CeArgs a, cudaStream_t st) {
   if (static_cast<long long>(a.R) * size > 0x7fffffffLL)
     return fail(VCB_ERR_UNSUPPORTED, "vcb_cross_entropy: R=%d C=%d", a.R, a.C);
   a.parts = a.R;
+  const int rc0 = launch_count(a, st);
+  if (rc0) return rc0;
   const auto kernel = staged ? ce_row_kernel<T, true> : ce_row_kernel<T, false>;
   if (staged) {
     const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
@@ -394,10 +419,6 @@ extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void*
   a.y = reinterpret_cast<const long long*>(labels);
   a.header = static_cast<int*>(workspace);
   a.part = reinterpret_cast<double*>(a.header + kHeader);
-  a.counts = std::min(kCountCtas, (R + 4095) / 4096);
-  ce_count_kernel<<<a.counts, 1024, 0, st>>>(R, a.y, a.ignore, a.header);
-  const int rc = check_launch("vcb_cross_entropy");
-  if (rc) return rc;
   if (type == VCB_F32) return launch<float>(a, st);
   if (type == VCB_BF16) return launch<__nv_bfloat16>(a, st);
   return launch<__half>(a, st);

@@ -17,6 +17,8 @@ can ask ``_lib.fault_check`` whether a bounded device wait ran out.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -27,7 +29,8 @@ ACTS = {'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3}
 
 def type_of(t, name):
     """vcb_dtype of a CUDA tensor; refuses what the kernels do not take."""
-    _lib.require_cuda(t, name)
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _lib.require_cuda(t, name)
     code = TYPES.get(t.dtype)
     if code is None:
         raise _lib.UnsupportedInput(f'vibecheck_nn_b200: {name} must be float32, bfloat16 or '
@@ -40,16 +43,24 @@ def rows_of(t, cols, like, name):
     stride); copies only what no row stride describes."""
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f'{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}')
-    if t.dim() < 1 or t.shape[-1] != cols:
+    dim = t.dim()
+    if dim < 1 or t.shape[-1] != cols:
         raise ValueError(f'{name}: shape {tuple(t.shape)}, expected (..., {cols})')
-    if t.dim() != 2:
-        t = t.reshape(-1, cols) if cols else t.new_empty((t.shape[:-1].numel(), 0))
+    if dim == 2 and t.is_contiguous():
+        return t, cols
+    if dim != 2:
+        t = t.reshape(t.shape[:-1].numel(), cols)
     rows = t.shape[0]
     ld = t.stride(0) if rows > 1 else cols
     if (cols > 1 and t.stride(1) != 1) or ld < cols:
         t = t.contiguous()
         ld = cols
     return t, ld
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(entry, *sizes):
+    return getattr(_lib.lib(), entry)(*sizes)
 
 
 def _act(act):
@@ -77,30 +88,34 @@ def linear_forward(x, weight, bias=None, act='none', residual=None, keep=False):
     ty = type_of(x, 'x')
     code = _act(act)
     N, K = _weight(x, weight)
-    lead = x.shape[:-1]
     x2, ldx = rows_of(x, K, x, 'x')
     w2, ldw = rows_of(weight, K, x, 'weight')
     M = x2.shape[0]
+    flat = x2.dim() == x.dim()
     if bias is not None:
         bias = _vector(bias, N, x, 'bias')
     r2, ldr = None, 0
     if residual is not None:
-        if residual.shape != (*lead, N):
-            raise ValueError(f'residual: shape {tuple(residual.shape)}, expected {(*lead, N)}')
+        if residual.shape[:-1] != x.shape[:-1]:
+            raise ValueError(f'residual: shape {tuple(residual.shape)}, expected '
+                             f'{(*x.shape[:-1], N)}')
         r2, ldr = rows_of(residual, N, x, 'residual')
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if keep else None
+    y = x.new_empty((M, N))
+    z = x.new_empty((M, N)) if keep else None
+    xp, wp = x2.data_ptr(), w2.data_ptr()
+    size = x.element_size()
+    nbytes = _workspace_bytes('vcb_linear_forward_workspace', M, N, K, ty,
+                              not (xp | wp | ldx * size | ldw * size) & 15)
+    ws = _lib.workspace(nbytes, x.device)
     with _lib.on_device(x.device):
-        L = _lib.lib()
-        nbytes = L.vcb_linear_forward_workspace(M, N, K, ty)
-        ws = _lib.workspace(nbytes, x.device)
-        rc = L.vcb_linear_forward(M, N, K, ty, x2.data_ptr(), ldx, w2.data_ptr(), ldw,
-                                  _p(bias), code, _p(r2), ldr, y.data_ptr(), N, _p(z), N,
-                                  _p(ws), nbytes, _lib.raw_stream(x.device))
-    _lib.check(rc, 'vcb_linear_forward')
-    if x.dim() != 2:
-        y = y.view(*lead, N)
-        z = z.view(*lead, N) if keep else None
+        rc = _lib.lib().vcb_linear_forward(M, N, K, ty, xp, ldx, wp, ldw, _p(bias), code, _p(r2),
+                                           ldr, y.data_ptr(), N, _p(z), N, _p(ws), nbytes,
+                                           _lib.raw_stream(x.device))
+    if rc:
+        _lib.check(rc, 'vcb_linear_forward')
+    if not flat:
+        y = y.view(*x.shape[:-1], N)
+        z = z.view(*x.shape[:-1], N) if keep else None
     return (y, z) if keep else y
 
 
@@ -112,7 +127,7 @@ def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, Tr
     ty = type_of(x, 'x')
     code = _act(act)
     N, K = _weight(x, weight)
-    if dy.shape != (*x.shape[:-1], N):
+    if dy.shape[:-1] != x.shape[:-1] or dy.shape[-1:] != (N,):
         raise ValueError(f'dy: shape {tuple(dy.shape)}, expected {(*x.shape[:-1], N)}')
     g2, ldg = rows_of(dy, N, x, 'dy')
     x2, ldx = rows_of(x, K, x, 'x')
@@ -123,18 +138,20 @@ def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, Tr
             raise ValueError(f'act {act!r} needs z of shape {tuple(dy.shape)}')
         z2, ldz = rows_of(z, N, x, 'z')
     M = x2.shape[0]
-    new = lambda *s: torch.empty(s, dtype=x.dtype, device=x.device)  # noqa: E731
-    dx = new(M, K) if need[0] else None
-    dw = new(N, K) if need[1] else None
-    db = new(N) if bias else None
+    dx = x.new_empty((M, K)) if need[0] else None
+    dw = x.new_empty((N, K)) if need[1] else None
+    db = x.new_empty((N,)) if bias else None
+    gp, xp, wp = g2.data_ptr(), x2.data_ptr(), w2.data_ptr()
+    size = x.element_size()
+    nbytes = _workspace_bytes('vcb_linear_backward_workspace', M, N, K, ty, code,
+                              not (gp | xp | wp | (ldg | ldx | ldw) * size) & 15)
+    ws = _lib.workspace(nbytes, x.device)
     with _lib.on_device(x.device):
-        L = _lib.lib()
-        nbytes = L.vcb_linear_backward_workspace(M, N, K, ty)
-        ws = _lib.workspace(nbytes, x.device)
-        rc = L.vcb_linear_backward(M, N, K, ty, g2.data_ptr(), ldg, x2.data_ptr(), ldx,
-                                   w2.data_ptr(), ldw, _p(z2), ldz, code, _p(dx), K, _p(dw), K,
-                                   _p(db), _p(ws), nbytes, _lib.raw_stream(x.device))
-    _lib.check(rc, 'vcb_linear_backward')
+        rc = _lib.lib().vcb_linear_backward(M, N, K, ty, gp, ldg, xp, ldx, wp, ldw, _p(z2), ldz,
+                                            code, _p(dx), K, _p(dw), K, _p(db), _p(ws), nbytes,
+                                            _lib.raw_stream(x.device))
+    if rc:
+        _lib.check(rc, 'vcb_linear_backward')
     if dx is not None and x.dim() != 2:
         dx = dx.view(x.shape)
     return dx, dw, db

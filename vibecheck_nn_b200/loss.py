@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import rows_of, type_of
+from .linear import _workspace_bytes, rows_of, type_of
 
 
 def cross_entropy_grad(logits, labels, ignore_index=-100):
@@ -30,16 +30,16 @@ def cross_entropy_grad(logits, labels, ignore_index=-100):
     x2, ld = rows_of(logits, C, logits, 'logits')
     labels = labels.contiguous()
     R = x2.shape[0]
-    grad = torch.empty((R, C), dtype=logits.dtype, device=logits.device)
-    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    grad = logits.new_empty((R, C))
+    loss = logits.new_empty((), dtype=torch.float32)
+    nbytes = _workspace_bytes('vcb_cross_entropy_workspace', R)
+    ws = _lib.workspace(nbytes, logits.device)
     with _lib.on_device(logits.device):
-        L = _lib.lib()
-        nbytes = L.vcb_cross_entropy_workspace(R)
-        ws = _lib.workspace(nbytes, logits.device)
-        rc = L.vcb_cross_entropy(R, C, ty, x2.data_ptr(), ld, labels.data_ptr(), int(ignore_index),
-                                 loss.data_ptr(), grad.data_ptr(), C, ws.data_ptr(), nbytes,
-                                 _lib.raw_stream(logits.device))
-    _lib.check(rc, 'vcb_cross_entropy')
+        rc = _lib.lib().vcb_cross_entropy(R, C, ty, x2.data_ptr(), ld, labels.data_ptr(),
+                                          int(ignore_index), loss.data_ptr(), grad.data_ptr(), C,
+                                          ws.data_ptr(), nbytes, _lib.raw_stream(logits.device))
+    if rc:
+        _lib.check(rc, 'vcb_cross_entropy')
     return loss, grad if logits.dim() == 2 else grad.view(logits.shape)
 
 

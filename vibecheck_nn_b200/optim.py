@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .linear import type_of
+from .linear import TYPES, type_of
 
 BLOCK = 256
 _MASK32 = 0xFFFFFFFF
@@ -78,34 +78,46 @@ class AdamW:
         grads = [p.grad for p in ps] if grads is None else list(grads)
         if len(grads) != len(ps):
             raise ValueError(f'{len(grads)} gradients for {len(ps)} parameters')
-        kinds = {}
+        groups = self._groups(grads)
+        self.t += 1
+        opts = self._opts()
+        m, v = self.m.data_ptr(), self.v.data_ptr()
+        ms, vs = _p(self.m_scale), _p(self.v_scale)
+        with _lib.on_device(self.device):
+            L, st = _lib.lib(), _lib.raw_stream(self.device)
+            for pt, gt, idx, gp in groups:
+                tab = self._table if len(gp) == len(ps) else self._table[idx]
+                tab['p'] = [ps[i].data_ptr() for i in idx]
+                tab['g'] = gp
+                rc = L.vcb_adamw(len(gp), tab.ctypes.data, pt, gt, self.state_bits, m, v, ms, vs,
+                                 ctypes.byref(opts), st)
+                if rc:
+                    _lib.check(rc, 'vcb_adamw')
+        torch.autograd.graph.increment_version(ps)
+
+    def _groups(self, grads):
+        """[(weights' type, gradients' type, indices, gradient pointers)], one
+        entry per launch."""
+        here = self.device.index
+        groups = {}
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if g is None:
                 continue
-            if g.shape != shape or g.device != self.device:
+            if g.shape != shape or g.get_device() != here:
                 raise ValueError(f'gradient {i}: {tuple(g.shape)} on {g.device}, expected '
                                  f'{tuple(shape)} on {self.device}')
             if not g.is_contiguous():
-                grads[i] = g = g.contiguous()
-            kinds.setdefault((self._types[i], g.dtype), []).append(i)
-        for pt, dtype in kinds:
-            if dtype != torch.float32 and dtype != ps[kinds[pt, dtype][0]].dtype:
-                raise _lib.UnsupportedInput(
-                    f'vibecheck_nn_b200: gradient of type {dtype}; the weights\' or float32')
-        self.t += 1
-        opts = self._opts()
-        with _lib.on_device(self.device):
-            L, st = _lib.lib(), _lib.raw_stream(self.device)
-            for (pt, dtype), idx in kinds.items():
-                tab = self._table if len(idx) == len(ps) else self._table[idx]
-                tab['p'] = [ps[i].data_ptr() for i in idx]
-                tab['g'] = [grads[i].data_ptr() for i in idx]
-                gt = 0 if dtype == torch.float32 else pt
-                rc = L.vcb_adamw(len(idx), tab.ctypes.data, pt, gt, self.state_bits,
-                                 self.m.data_ptr(), self.v.data_ptr(), _p(self.m_scale),
-                                 _p(self.v_scale), ctypes.byref(opts), st)
-                _lib.check(rc, 'vcb_adamw')
-        torch.autograd.graph.increment_version(ps)
+                grads[i] = g = g.contiguous()  # grads keeps it until the launch
+            key = (self._types[i], g.dtype)
+            group = groups.get(key)
+            if group is None:
+                if g.dtype != torch.float32 and g.dtype != self.params[i].dtype:
+                    raise _lib.UnsupportedInput(f'vibecheck_nn_b200: gradient {i} of type '
+                                                f'{g.dtype}; the weight\'s or float32')
+                group = groups[key] = (key[0], TYPES[g.dtype], [], [])
+            group[2].append(i)
+            group[3].append(g.data_ptr())
+        return groups.values()
 
     def moments(self):
         """(m, v) of all tensors as flat float32 buffers (the state itself
