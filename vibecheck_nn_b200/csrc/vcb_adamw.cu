@@ -54,82 +54,178 @@ struct State {
   vcb_adamw_opts o;
 };
 
-__device__ __forceinline__ float sqrt_fast(float x) {
+// Approximate square root and reciprocal; what lies below the normal range
+// counts as 0.
+__device__ __forceinline__ float sqrt_flush(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Larger of the two, NaN when either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float rcp_flush(float x) {
   float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Largest of the three magnitudes, NaN when one is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Two floats in one instruction: the kernel is bound by issue slots.  Each
+// result is rounded by itself, as by the scalar instructions.
+struct F2 {
+  float x, y;
+};
+
+#define VCB_F2_OP2(name, op)                                                           \
+  __device__ __forceinline__ F2 name(F2 a, F2 b) {                                     \
+    F2 r;                                                                              \
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t" op \
+        " r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"                                      \
+        : "=f"(r.x), "=f"(r.y)                                                         \
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));                                     \
+    return r;                                                                          \
+  }
+VCB_F2_OP2(mul2, "mul.rn.f32x2")
+VCB_F2_OP2(add2, "add.rn.f32x2")
+VCB_F2_OP2(add2_rz, "add.rz.f32x2")
+#undef VCB_F2_OP2
+
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+__device__ __forceinline__ F2 both(float x) { return {x, x}; }
+
+// Sums of products are added one by one: an add.f32x2 of a mul.f32x2 becomes one
+// fma, whose single rounding gives other codes.
+__device__ __forceinline__ F2 sum_of(F2 a, F2 b) {
+  return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)};
 }
 
 // 32 noise bits of an element: three multiply-xorshift rounds (multiplicative
 // hashing) with the fractional bits of the golden ratio, sqrt 2 and sqrt 3.
-__device__ __forceinline__ uint32_t noise(uint32_t index, uint32_t key) {
-  uint32_t x = (index + key) * 0x9E3779B9u;
+// x: (index + key) kGolden.
+constexpr uint32_t kGolden = 0x9E3779B9u;
+__device__ __forceinline__ uint32_t noise(uint32_t x) {
   x = (x ^ (x >> 16)) * 0x6A09E667u;
   x = (x ^ (x >> 15)) * 0xBB67AE85u;
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ float four(float c) {
-  const float q = __fmul_rn(c, c);
-  return __fmul_rn(q, q);
+// Conversions between small integers and floats go by the mantissa of 2^23 + n,
+// not by the conversion instructions: those share a pipe of an eighth of the
+// rate with the square roots, and the twelve of them per element were what bound
+// the kernel.
+constexpr float kBig = 8388608.f;  // 2^23
+
+// 2^23 + byte / half word k of w.
+__device__ __forceinline__ float big_byte(uint32_t w, int k) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 | k));
+}
+__device__ __forceinline__ float big_half(uint32_t w, int k) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, k ? 0x7432 : 0x7410));
 }
 
-__device__ __forceinline__ float m_value(int8_t code, float scale) {
-  const float c = code;
-  return __fmul_rn(scale, __fmul_rn(__fmul_rn(c, fabsf(c)), 1.f / 16129.f));
+// floor(x) for 0 <= x < 2^22.
+__device__ __forceinline__ F2 floor2(F2 x) { return add2(add2_rz(x, both(kBig)), both(-kBig)); }
+
+// The low bytes of four integers held as floats, each 2^23 + n.
+__device__ __forceinline__ uint32_t pack4(F2 n, F2 k) {
+  const uint32_t a = __byte_perm(__float_as_uint(n.x), __float_as_uint(n.y), 0x0040);
+  const uint32_t b = __byte_perm(__float_as_uint(k.x), __float_as_uint(k.y), 0x0040);
+  return __byte_perm(a, b, 0x5410);
 }
 
-__device__ __forceinline__ float v_value(uint8_t code, float scale) {
-  return __fmul_rn(scale, __fmul_rn(four(code), static_cast<float>(1.0 / 4228250625.0)));
+__device__ __forceinline__ F2 four(F2 c) {
+  const F2 q = mul2(c, c);
+  return mul2(q, q);
 }
 
-// The largest c with c^2 <= y, or the next one with the probability
-// (y - c^2) / (2c + 1): the approximate root is off by one at most.
-__device__ __forceinline__ int8_t m_code(float m, float inv, float r) {
-  const float y = __fmul_rn(__fmul_rn(fabsf(m), inv), 16129.f);
-  float c = fminf(floorf(sqrt_fast(y)), 126.f);
-  if (c * c > y) c -= 1.f;
-  if ((c + 1.f) * (c + 1.f) <= y && c < 126.f) c += 1.f;
-  if (__fmul_rn(r, 2.f * c + 1.f) < __fsub_rn(y, c * c)) c += 1.f;
-  return static_cast<int8_t>(m < 0.f ? -static_cast<int>(c) : static_cast<int>(c));
+// Moments of the codes k and k + 1 of a word; signed codes come as c + 128 (the
+// sign bit flipped in all four bytes).
+__device__ __forceinline__ F2 m_value(uint32_t flipped, int k, float scale) {
+  const F2 c = add2({big_byte(flipped, k), big_byte(flipped, k + 1)}, both(-kBig - 128.f));
+  return mul2(both(scale), mul2(mul2(c, {fabsf(c.x), fabsf(c.y)}), both(1.f / 16129.f)));
 }
 
-__device__ __forceinline__ uint8_t v_code(float v, float inv, float r) {
-  const float y = __fmul_rn(__fmul_rn(v, inv), 4228250625.f);
-  float c = fminf(floorf(sqrt_fast(sqrt_fast(y))), 254.f);
-  if (four(c) > y) c -= 1.f;
-  if (four(c + 1.f) <= y && c < 254.f) c += 1.f;
-  const float lo = four(c);
-  if (__fmul_rn(r, __fsub_rn(four(c + 1.f), lo)) < __fsub_rn(y, lo)) c += 1.f;
-  if (y > 0.f && c < 1.f) c = 1.f;
-  return static_cast<uint8_t>(c);
+__device__ __forceinline__ F2 v_value(uint32_t codes, int k, float scale) {
+  const F2 c = add2({big_byte(codes, k), big_byte(codes, k + 1)}, both(-kBig));
+  return mul2(both(scale), mul2(four(c), both(static_cast<float>(1.0 / 4228250625.0))));
 }
 
+// Square roots here are approximate; a factor just above 1 keeps a root from
+// falling below its integer, and one comparison takes back what that adds.
+constexpr float kAbove = 1.f + 0x1p-20f;
+
+// The codes of |m| / M = y / 127^2: the largest c with c^2 <= y, or the next one
+// with the probability (y - c^2) / (2c + 1).  r: 16 random bits.  Returns 2^23 +
+// 128 + the signed code.
+__device__ __forceinline__ F2 m_code(F2 m, float inv, F2 r) {
+  const F2 y = mul2(mul2({fabsf(m.x), fabsf(m.y)}, both(inv)), both(16129.f));
+  F2 c = floor2(mul2({sqrt_flush(y.x), sqrt_flush(y.y)}, both(kAbove)));
+  const F2 q = mul2(c, c);
+  if (q.x > y.x) c.x -= 1.f;
+  if (q.y > y.y) c.y -= 1.f;
+  const F2 odds = mul2(r, fma2(both(2.f), c, both(1.f)));
+  const F2 rest = mul2(fma2({-c.x, -c.y}, c, y), both(65536.f));
+  if (odds.x < rest.x) c.x += 1.f;
+  if (odds.y < rest.y) c.y += 1.f;
+  c = {copysignf(fminf(c.x, 127.f), m.x), copysignf(fminf(c.y, 127.f), m.y)};
+  return add2(c, both(kBig + 128.f));
+}
+
+// The codes of v / V = y / 255^4; root: about y^(1/4), kAbove included.  Returns
+// 2^23 + code.
+__device__ __forceinline__ F2 v_code(F2 v, float inv, F2 root, F2 r) {
+  const F2 y = mul2(mul2(v, both(inv)), both(4228250625.f));
+  F2 c = floor2(root);
+  const F2 q = four(c);
+  if (q.x > y.x) c.x -= 1.f;
+  if (q.y > y.y) c.y -= 1.f;
+  const F2 lo = four(c), minus = {-lo.x, -lo.y};
+  const F2 odds = mul2(r, sum_of(four(add2(c, both(1.f))), minus));
+  const F2 rest = mul2(sum_of(y, minus), both(65536.f));
+  if (odds.x < rest.x) c.x += 1.f;
+  if (odds.y < rest.y) c.y += 1.f;
+  c = {fminf(c.x, 255.f), fminf(c.y, 255.f)};
+  if (y.x > 0.f) c.x = fmaxf(c.x, 1.f);
+  if (y.y > 0.f) c.y = fmaxf(c.y, 1.f);
+  return add2(c, both(kBig));
+}
+
+// Four elements of a tensor, of which `live` exist; `whole`: all do, and their
+// address is that of a vector.
 template <typename T>
-__device__ __forceinline__ void get4(const T* p, int live, bool vec, float (&v)[4]) {
-  if (vec && live >= 4) {
-    load4(p, v);
+__device__ __forceinline__ void get4(const T* p, int live, bool whole, F2 (&v)[2]) {
+  float t[4];
+  if (whole) {
+    load4(p, t);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < live ? to_f32(p[i]) : 0.f;
+    for (int i = 0; i < 4; ++i) t[i] = i < live ? to_f32(p[i]) : 0.f;
   }
+  v[0] = {t[0], t[1]}, v[1] = {t[2], t[3]};
 }
 
 template <typename T>
-__device__ __forceinline__ void put4(T* p, int live, bool vec, const float (&v)[4]) {
-  if (vec && live >= 4) {
-    store4(p, v);
+__device__ __forceinline__ void put4(T* p, int live, bool whole, const F2 (&v)[2]) {
+  const float t[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+  if (whole) {
+    store4(p, t);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (i < live) p[i] = from_f32<T>(v[i]);
+      if (i < live) p[i] = from_f32<T>(t[i]);
   }
 }
 
@@ -146,19 +242,18 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long at = static_cast<long long>(blockIdx.x - e.first) * kChunk + warp * kBlock;
   if (at >= e.n) return;
-  const bool vec = e.vec;
   PT* p = static_cast<PT*>(e.p) + at;
   const GT* g = static_cast<const GT*>(e.g) + at;
   const long long off = e.off + at;  // of this block in the state
-  const long long left = e.n - at;
-  int live[2];
-  float pv[2][4], gv[2][4], m[2][4], v[2][4];
+  const int left = static_cast<int>(min(e.n - at, static_cast<long long>(kBlock)));
+  const bool whole = e.vec && left == kBlock;  // of the warp
+  // per lane two groups of four, each in two pairs
+  F2 pv[2][2], gv[2][2], m[2][2], v[2][2], root[2][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = h * 128 + lane * 4;
-    live[h] = static_cast<int>(max(0LL, min(4LL, left - i)));
-    get4(p + i, live[h], vec, pv[h]);
-    get4(g + i, live[h], vec, gv[h]);
+    get4(p + i, left - i, whole, pv[h]);
+    get4(g + i, left - i, whole, gv[h]);
   }
   float ms = 0.f, vs = 0.f;
   if (BITS == 8) {
@@ -169,15 +264,17 @@ __global__ void __launch_bounds__(kWarps * 32)
   for (int h = 0; h < 2; ++h) {
     const long long i = off + h * 128 + lane * 4;
     if (BITS == 8) {
-      const char4 mc = *reinterpret_cast<const char4*>(static_cast<const int8_t*>(s.m) + i);
-      const uchar4 vc = *reinterpret_cast<const uchar4*>(static_cast<const uint8_t*>(s.v) + i);
-      m[h][0] = m_value(mc.x, ms), m[h][1] = m_value(mc.y, ms);
-      m[h][2] = m_value(mc.z, ms), m[h][3] = m_value(mc.w, ms);
-      v[h][0] = v_value(vc.x, vs), v[h][1] = v_value(vc.y, vs);
-      v[h][2] = v_value(vc.z, vs), v[h][3] = v_value(vc.w, vs);
+      const uint32_t mc =
+          *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(s.m) + i) ^ 0x80808080u;
+      const uint32_t vc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s.v) + i);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[h][j] = m_value(mc, 2 * j, ms);
+        v[h][j] = v_value(vc, 2 * j, vs);
+      }
     } else {
-      load4(static_cast<const float*>(s.m) + i, m[h]);
-      load4(static_cast<const float*>(s.v) + i, v[h]);
+      get4(static_cast<const float*>(s.m) + i, 4, true, m[h]);
+      get4(static_cast<const float*>(s.v) + i, 4, true, v[h]);
     }
   }
   const vcb_adamw_opts& o = s.o;
@@ -185,47 +282,51 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float gj = gv[h][j];
-      // each product and sum rounded by itself: the codes of an 8-bit state
-      // do not depend on how a compiler contracts them
-      m[h][j] = __fadd_rn(__fmul_rn(m[h][j], o.b1), __fmul_rn(gj, o.c1));
-      v[h][j] = __fadd_rn(__fmul_rn(v[h][j], o.b2), __fmul_rn(__fmul_rn(gj, o.c2), gj));
-      const float d = __fdividef(m[h][j], sqrt_fast(v[h][j]) * o.root + o.eps);
-      pv[h][j] = __fsub_rn(__fmul_rn(pv[h][j], o.keep), __fmul_rn(d, o.size));
+    for (int j = 0; j < 2; ++j) {
+      const F2 gj = gv[h][j];
+      m[h][j] = sum_of(mul2(m[h][j], both(o.b1)), mul2(gj, both(o.c1)));
+      v[h][j] = sum_of(mul2(v[h][j], both(o.b2)), mul2(mul2(gj, both(o.c2)), gj));
+      root[h][j] = {sqrt_flush(v[h][j].x), sqrt_flush(v[h][j].y)};
+      const F2 d = fma2(root[h][j], both(o.root), both(o.eps));
+      const F2 step = mul2(mul2(m[h][j], {rcp_flush(d.x), rcp_flush(d.y)}), both(-o.size));
+      pv[h][j] = add2(mul2(pv[h][j], both(o.keep)), step);
       if (BITS == 8) {
-        big = max_nan(big, fabsf(m[h][j]));
-        most = max_nan(most, v[h][j]);
+        big = max_nan(big, m[h][j].x, m[h][j].y);
+        most = max_nan(most, v[h][j].x, v[h][j].y);
       }
     }
-    put4(p + h * 128 + lane * 4, live[h], vec, pv[h]);
+    const int i = h * 128 + lane * 4;
+    put4(p + i, left - i, whole, pv[h]);
   }
   if (BITS == 8) {
 #pragma unroll
     for (int k = 16; k; k >>= 1) {
-      big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, k));
-      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, k));
+      big = max_nan(big, big, __shfl_xor_sync(0xffffffffu, big, k));
+      most = max_nan(most, most, __shfl_xor_sync(0xffffffffu, most, k));
     }
     // a scale below the normal range counts as zero; NaN and infinity stay and
     // mark the whole block
     if (big < FLT_MIN) big = 0.f;
     if (most < FLT_MIN) most = 0.f;
     const float im = big > 0.f ? __frcp_rn(big) : 0.f, iv = most > 0.f ? __frcp_rn(most) : 0.f;
+    // y^(1/4) = sqrt(sqrt(v) sqrt(255^4 / V))
+    const F2 up = both(sqrtf(iv) * (65025.f * kAbove));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const long long i = off + h * 128 + lane * 4;
-      int8_t mc[4];
-      uint8_t vc[4];
+      const uint32_t x0 = (static_cast<uint32_t>(i) + o.key) * kGolden;
+      F2 mc[2], vc[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t x = noise(static_cast<uint32_t>(i + j), o.key);
-        mc[j] = m_code(m[h][j], im, static_cast<float>(x >> 16) * (1.f / 65536.f));
-        vc[j] = v_code(v[h][j], iv, static_cast<float>(x & 0xFFFFu) * (1.f / 65536.f));
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = noise(x0 + 2 * j * kGolden), y = noise(x0 + (2 * j + 1) * kGolden);
+        const F2 t = mul2(root[h][j], up);
+        mc[j] = m_code(m[h][j], im, add2({big_half(x, 1), big_half(y, 1)}, both(-kBig)));
+        vc[j] = v_code(v[h][j], iv, {sqrt_flush(t.x), sqrt_flush(t.y)},
+                       add2({big_half(x, 0), big_half(y, 0)}, both(-kBig)));
       }
-      *reinterpret_cast<char4*>(static_cast<int8_t*>(s.m) + i) =
-          make_char4(mc[0], mc[1], mc[2], mc[3]);
-      *reinterpret_cast<uchar4*>(static_cast<uint8_t*>(s.v) + i) =
-          make_uchar4(vc[0], vc[1], vc[2], vc[3]);
+      *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(s.m) + i) =
+          pack4(mc[0], mc[1]) ^ 0x80808080u;
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(s.v) + i) = pack4(vc[0], vc[1]);
     }
     if (lane == 0) {
       s.ms[off / kBlock] = big;
@@ -235,8 +336,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const long long i = off + h * 128 + lane * 4;
-      store4(static_cast<float*>(s.m) + i, m[h]);
-      store4(static_cast<float*>(s.v) + i, v[h]);
+      put4(static_cast<float*>(s.m) + i, 4, true, m[h]);
+      put4(static_cast<float*>(s.v) + i, 4, true, v[h]);
     }
   }
 }
@@ -250,10 +351,10 @@ __global__ void __launch_bounds__(256)
   if (q >= quads) return;
   const long long i = q * 4;
   const float a = ms[i / kBlock], b = vs[i / kBlock];
-  const char4 mc = *reinterpret_cast<const char4*>(m + i);
-  const uchar4 vc = *reinterpret_cast<const uchar4*>(v + i);
-  store4(mo + i, {m_value(mc.x, a), m_value(mc.y, a), m_value(mc.z, a), m_value(mc.w, a)});
-  store4(vo + i, {v_value(vc.x, b), v_value(vc.y, b), v_value(vc.z, b), v_value(vc.w, b)});
+  const uint32_t mc = *reinterpret_cast<const uint32_t*>(m + i) ^ 0x80808080u;
+  const uint32_t vc = *reinterpret_cast<const uint32_t*>(v + i);
+  put4(mo + i, 4, true, {m_value(mc, 0, a), m_value(mc, 2, a)});
+  put4(vo + i, 4, true, {v_value(vc, 0, b), v_value(vc, 2, b)});
 }
 
 template <typename PT, typename GT, int BITS>
