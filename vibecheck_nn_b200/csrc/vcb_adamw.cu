@@ -230,7 +230,7 @@ __device__ __forceinline__ void put4(T* p, int live, bool whole, const F2 (&v)[2
 }
 
 template <typename PT, typename GT, int BITS, int CAP>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 5)
     adamw_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ State s) {
   // the tensor of this CTA: the last whose first CTA is not behind it
   int lo = 0, hi = tab.count - 1;

@@ -182,4 +182,5 @@ int tc_fault_take(cudaStream_t st, int* was_set);
 int f32_fault_take(cudaStream_t st, int* was_set);
 
 }  // namespace lin
+
 }  // namespace vcb
