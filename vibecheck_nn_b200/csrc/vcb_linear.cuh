@@ -3,6 +3,8 @@
 // tensor-core translation unit.
 #pragma once
 
+#include <type_traits>
+
 #include "vcb_common.cuh"
 #include "vcb_types.cuh"
 
@@ -90,39 +92,61 @@ __device__ __forceinline__ void transpose16(float (&v)[16], int lane) {
   }
 }
 
+// Four elements of a row at column j, as they lie.
+template <typename T>
+struct Four {
+  typename std::conditional<sizeof(T) == 4, float4, uint2>::type raw;
+};
+
+// Residuals of the rows i, i + 4, .. (N of them), columns j .. j + 3.  Fetched ahead
+// of the chunk that adds them: their way from HBM would otherwise be waited for in
+// every chunk.
+template <typename T, int N>
+struct Residual {
+  Four<T> v[N];
+  __device__ __forceinline__ void fetch(const Epilogue& e, int I, int J, int i, int j) {
+    if (!e.res || j >= J) return;
+    const bool vec = e.vec && j + 4 <= J;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      if (i + 4 * q >= I) break;
+      const T* at = static_cast<const T*>(e.res) + (i + 4 * q) * e.ldr + j;
+      if (vec) {
+        v[q].raw = __ldcs(reinterpret_cast<const decltype(v[q].raw)*>(at));
+      } else {
+        T t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = j + k < J ? at[k] : from_f32<T>(0.f);
+        v[q].raw = *reinterpret_cast<const decltype(v[q].raw)*>(t);
+      }
+    }
+  }
+  __device__ __forceinline__ void add(float (&out)[4 * N]) const {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      T t[4];
+      *reinterpret_cast<decltype(v[q].raw)*>(t) = v[q].raw;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[4 * q + k] += to_f32(t[k]);
+    }
+  }
+};
+
 // Rows i, i + 4, .. (N of them), columns j .. j + 3 of the output: bias,
 // pre-activation, act, residual, one rounding.
 template <typename T, int N>
 __device__ __forceinline__ void emit(const Epilogue& e, int I, int J, int i, int j,
-                                     const float (&bias)[4], float (&v)[4 * N]) {
+                                     const float (&bias)[4], float (&v)[4 * N],
+                                     const Residual<T, N>& res) {
   if (j >= J) return;
   const bool vec = e.vec && j + 4 <= J;
-  float r[4 * N];
-  if (e.res) {
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-      const T* at = static_cast<const T*>(e.res) + (i + 4 * q) * e.ldr + j;
-      float t[4] = {};
-      if (i + 4 * q < I) {
-        if (vec) {
-          load4(at, t);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (j + k < J) t[k] = to_f32(at[k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) r[4 * q + k] = t[k];
-    }
-  }
   const auto put = [&](void* base, long long ld) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       if (i + 4 * q >= I) break;
       T* at = static_cast<T*>(base) + (i + 4 * q) * ld + j;
       if (vec) {
-        store4(at, {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+        store4_stream(at, {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -139,11 +163,40 @@ __device__ __forceinline__ void emit(const Epilogue& e, int I, int J, int i, int
     case VCB_ACT_SILU: act_all<VCB_ACT_SILU>(v); break;
     default: break;
   }
-  if (e.res) {
-#pragma unroll
-    for (int c = 0; c < 4 * N; ++c) v[c] += r[c];
-  }
+  if (e.res) res.add(v);
   put(e.out, e.ldo);
+}
+
+// N consecutive rows from i of column j.
+template <typename T, int N>
+__device__ __forceinline__ void emit_column(const Epilogue& e, int I, int J, int i, int j,
+                                            float bias, float (&v)[N]) {
+  const int n = min(N, I - i);
+  if (j >= J || n <= 0) return;
+  float r[N];
+  if (e.res) {
+    const T* at = static_cast<const T*>(e.res) + i * e.ldr + j;
+#pragma unroll
+    for (int c = 0; c < N; ++c) r[c] = c < n ? to_f32(__ldcs(at + c * e.ldr)) : 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < N; ++c) v[c] += bias;
+  if (e.z) {
+    T* at = static_cast<T*>(e.z) + i * e.ldz + j;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < n) __stcs(at + c * e.ldz, from_f32<T>(v[c]));
+  }
+  switch (e.act) {
+    case VCB_ACT_RELU: act_all<VCB_ACT_RELU>(v); break;
+    case VCB_ACT_GELU: act_all<VCB_ACT_GELU>(v); break;
+    case VCB_ACT_SILU: act_all<VCB_ACT_SILU>(v); break;
+    default: break;
+  }
+  T* at = static_cast<T*>(e.out) + i * e.ldo + j;
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+    if (c < n) __stcs(at + c * e.ldo, from_f32<T>(e.res ? v[c] + r[c] : v[c]));
 }
 
 struct Fwd {

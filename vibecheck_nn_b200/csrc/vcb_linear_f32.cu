@@ -537,11 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
                        : "memory");
         break;
       }
-      const Epilogue e = p.epi;
-      const int I = p.I, J = p.J, j = j0 + (lane & ~3);
-      const int ea = j0 + lane < J ? scale_exp(__ldg(p.most_a + j0 + lane)) : 0;
-      float bias[4];
-      bias_at<float>(e, J, j, bias);
+      // a lane keeps its column: a warp's accesses are 32 neighbouring floats
+      const int I = p.I, J = p.J, j = j0 + lane;
+      const int ea = j < J ? scale_exp(__ldg(p.most_a + j)) : 0;
+      const float bias = p.epi.bias && j < J ? static_cast<const float*>(p.epi.bias)[j] : 0.f;
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
         if (i0 + c < I) {  // warp-uniform
@@ -551,8 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
 #pragma unroll
           for (int k = 0; k < 16; ++k)
             v[k] = scaled(acc[c + k], ea + __shfl_sync(0xffffffffu, eb, k));
-          transpose16(v, lane);
-          emit<float, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v);
+          emit_column<float, 16>(p.epi, I, J, i0 + c, j, bias, v);
         }
       }
     }
@@ -584,7 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
         const int eb = scale_exp(__ldg(p.most_b + i0 + c));
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = scaled(v[k], ea[k] + eb);
-        emit<float, 1>(e, p.I, p.J, i0 + c, j, bias, v);
+        Residual<float, 1> res;
+        res.fetch(e, p.I, p.J, i0 + c, j);
+        emit<float, 1>(e, p.I, p.J, i0 + c, j, bias, v, res);
       }
     }
     cluster_sync();  // no CTA leaves while its partial sums are read

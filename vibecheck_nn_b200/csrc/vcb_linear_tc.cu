@@ -58,29 +58,69 @@ struct Launch {
   int stages;
 };
 
-// Epilogue of one warp: lanes 32 (warp % 4).. of the accumulator at `acc`,
-// every other chunk of 16 columns (warp / 4).  `ok` false: NaN instead.
+// Epilogue of one warp: lanes 32 (warp % 4).. of the accumulator at `acc`, every
+// other chunk of 16 columns (warp / 4).  Residuals are fetched two chunks ahead.
+// `ok` false: NaN instead.
 template <typename T>
-__device__ __forceinline__ void tile_epilogue(const Prod& p, uint32_t acc, int warp, int lane,
-                                              int j0, int i0, bool ok) {
-  const Epilogue e = p.epi;
-  const int I = p.I, J = p.J, bn = p.bn;
-  const int j = j0 + (warp & 3) * 32 + (lane & ~3);
-  float bias[4];
-  bias_at<T>(e, J, j, bias);
-  const uint32_t base = acc + ((uint32_t)((warp & 3) * 32) << 16);
-  for (int c = (warp >> 2) * 16; c < bn; c += 32) {
-    if (i0 + c >= I) break;  // warp-uniform
-    uint32_t r[16];
+struct TileEpilogue {
+  const Epilogue& e;
+  int I, J, bn, i0, lane, j, first;
+  Residual<T, 4> res[2];
+
+  __device__ __forceinline__ TileEpilogue(const Prod& p, int warp, int lane_, int j0, int i0_)
+      : e(p.epi), I(p.I), J(p.J), bn(p.bn), i0(i0_), lane(lane_),
+        j(j0 + (warp & 3) * 32 + (lane_ & ~3)), first((warp >> 2) * 16) {
+    // before the accumulator is ready
+    fetch(res[0], first);
+    fetch(res[1], first + 32);
+  }
+  __device__ __forceinline__ void fetch(Residual<T, 4>& r, int c) {
+    if (c < bn) r.fetch(e, I, J, i0 + c + (lane & 3), j);
+  }
+  __device__ __forceinline__ void chunk(uint32_t at, int c, const float (&bias)[4],
+                                        Residual<T, 4>& r, bool ok) {
+    if (c >= bn || i0 + c >= I) return;  // warp-uniform
+    uint32_t raw[16];
     if (ok) {
-      tmem_ld16(base + c, r);
-      tmem_wait_ld(r);
+      tmem_ld16(at + c, raw);
+      tmem_wait_ld(raw);
     }
     float v[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(r[k]) : NAN;
+    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
     transpose16(v, lane);
-    emit<T, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v);
+    emit<T, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v, r);
+    fetch(r, c + 64);
+  }
+  __device__ __forceinline__ void run(uint32_t acc, int warp, bool ok) {
+    float bias[4];
+    bias_at<T>(e, J, j, bias);
+    const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int c = first; c < bn; c += 64) {
+      chunk(at, c, bias, res[0], ok);
+      chunk(at, c + 32, bias, res[1], ok);
+    }
+  }
+};
+
+// The same where rows take no vectors: a lane keeps its column, so a warp's stores
+// and loads are 32 neighbouring elements.
+template <typename T>
+__device__ __forceinline__ void column_epilogue(const Prod& p, uint32_t acc, int warp, int lane,
+                                                int j0, int i0, bool ok) {
+  const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
+  const int j = j0 + (warp & 3) * 32 + lane, bn = p.bn, I = p.I;
+  const float bias = p.epi.bias && j < p.J ? to_f32(static_cast<const T*>(p.epi.bias)[j]) : 0.f;
+  for (int c = (warp >> 2) * 16; c < bn && i0 + c < I; c += 32) {
+    uint32_t raw[16];
+    if (ok) {
+      tmem_ld16(at + c, raw);
+      tmem_wait_ld(raw);
+    }
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
+    emit_column<T, 16>(p.epi, I, p.J, i0 + c, j, bias, v);
   }
 }
 
@@ -199,12 +239,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Prod& p = L.p[u >= L.units0];
       int ti, tj;
       tile_at(p.tiles_i, p.tiles_j, u >= L.units0 ? u - L.units0 : u, ti, tj);
-      const int q = t & 1;
-      ok = ok && mbar_wait(&acc_full[q], (t >> 1) & 1, kDoneLimit, vfailed);
-      ok = __all_sync(0xffffffffu, ok);
-      fence_after_sync();
-      tile_epilogue<T>(p, tmem + q * 256, warp, lane, (tj * 2 + rank) * kTileJ, ti * 2 * kTileJ,
-                       ok);
+      const int q = t & 1, j0 = (tj * 2 + rank) * kTileJ, i0 = ti * 2 * kTileJ;
+      const auto ready = [&] {
+        ok = ok && mbar_wait(&acc_full[q], (t >> 1) & 1, kDoneLimit, vfailed);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_after_sync();
+      };
+      if (p.epi.vec) {
+        TileEpilogue<T> epilogue(p, warp, lane, j0, i0);
+        ready();
+        epilogue.run(tmem + q * 256, warp, ok);
+      } else {
+        ready();
+        column_epilogue<T>(p, tmem + q * 256, warp, lane, j0, i0, ok);
+      }
       fence_before_sync();
       __syncwarp();
       if (lane == 0)
@@ -316,12 +364,20 @@ __global__ void __launch_bounds__(kThreads)
       if (!mbar_wait(&acc_full, 0, kDoneLimit)) failed = 1;
     }
   } else {
-    ok = mbar_wait(&acc_full, 0, kDoneLimit) && !*vfailed;
-    ok = __all_sync(0xffffffffu, ok);
-    fence_after_sync();
-    if (parts == 1) {
-      if (!idle) tile_epilogue<T>(p, tmem, warp, lane, j0, i0, ok);
+    const auto ready = [&] {
+      ok = mbar_wait(&acc_full, 0, kDoneLimit) && !*vfailed;
+      ok = __all_sync(0xffffffffu, ok);
+      fence_after_sync();
+    };
+    if (parts == 1 && !p.epi.vec) {
+      ready();
+      if (!idle) column_epilogue<T>(p, tmem, warp, lane, j0, i0, ok);
+    } else if (parts == 1) {
+      TileEpilogue<T> epilogue(p, warp, lane, j0, idle ? p.I : i0);
+      ready();
+      epilogue.run(tmem, warp, ok);
     } else {
+      ready();
       // partial sums where the stages were, a column's 128 rows together
       const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       for (int c = (warp >> 2) * 16; c < p.bn && i0 + c < p.I; c += 32) {
@@ -358,7 +414,9 @@ __global__ void __launch_bounds__(kThreads)
         const float4 t = peer_f32x4(map_rank(at, k));
         v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
       }
-      emit<T, 1>(e, p.I, p.J, i0 + c, j, bias, v);
+      Residual<T, 1> res;
+      res.fetch(e, p.I, p.J, i0 + c, j);
+      emit<T, 1>(e, p.I, p.J, i0 + c, j, bias, v, res);
     }
   }
   cluster_sync();  // no CTA leaves while its partial sums are read
@@ -374,7 +432,7 @@ struct Copy {
 };
 
 struct Prep {
-  int M, N, act, strips;  // strips of 128 columns of dy, 0 for none
+  int M, N, act, strips;  // strips of 32 columns of dy, 0 for none
   const void *dy, *z;
   void *dz, *db;          // either may be NULL
   long long lddy, ldz, lddz;
@@ -382,28 +440,52 @@ struct Prep {
   int copies;
 };
 
-constexpr int kPrepCluster = 8, kPrepThreads = 256;
+constexpr int kPrepCluster = 8, kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
+constexpr int kStrip = 32;  // columns
 
-// A cluster of 8 CTAs per strip: each sums its eighth of the rows (a warp per
-// row, 4 columns per lane), rank 0 adds the eight sums in order.  Bound by HBM:
-// dy and z are read and dz is written once.  The remaining CTAs copy.
+// Four elements at p, `align` bytes aligned (8, 4 or 2); 0 from `left` on.
+template <typename T>
+__device__ __forceinline__ void four_at(const T* p, int align, int left, float (&v)[4]) {
+  T e[4];
+  if (align == 8 && left >= 4) {
+    *reinterpret_cast<uint2*>(e) = __ldcs(reinterpret_cast<const uint2*>(p));
+  } else if (align >= 4 && left >= 4) {
+    reinterpret_cast<uint32_t*>(e)[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    reinterpret_cast<uint32_t*>(e)[1] = __ldcs(reinterpret_cast<const uint32_t*>(p) + 1);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = i < left ? p[i] : from_f32<T>(0.f);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
+}
+
+// Alignment of all rows of a 16-bit matrix at columns that are multiples of 4.
+__device__ __forceinline__ int rows_align(const void* p, long long ld) {
+  const unsigned bits = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) |
+                        static_cast<unsigned>(ld * 2);
+  return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+}
+
+// A cluster of 8 CTAs per strip of 32 columns: each sums its eighth of the rows (8
+// lanes per row, 4 columns per lane), rank 0 adds the eight sums in order.  Bound by
+// HBM: dy and z are read and dz is written once; strips are narrow so that a matrix
+// of 2,000 columns keeps every SM reading.  The remaining CTAs copy.
 template <typename T>
 __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThreads)
     prep_kernel(const __grid_constant__ Prep a) {
-  __shared__ float part[kPrepThreads / 32][128];
-  __shared__ float mine[128];
+  __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int strip = blockIdx.x / kPrepCluster;
   if (strip < a.strips) {
-    const int rank = blockIdx.x % kPrepCluster, c = strip * 128 + lane * 4;
+    const int rank = blockIdx.x % kPrepCluster, c = strip * kStrip + (lane & 7) * 4;
     const long long r0 = static_cast<long long>(a.M) * rank / kPrepCluster;
     const long long r1 = static_cast<long long>(a.M) * (rank + 1) / kPrepCluster;
-    const T *dy = static_cast<const T*>(a.dy), *z = static_cast<const T*>(a.z);
-    const bool vy = reinterpret_cast<uintptr_t>(dy) % 8 == 0 && a.lddy % 4 == 0 && c + 4 <= a.N;
-    const bool vz = reinterpret_cast<uintptr_t>(z) % 8 == 0 && a.ldz % 4 == 0 && c + 4 <= a.N;
+    const T *dy = static_cast<const T*>(a.dy) + c, *z = static_cast<const T*>(a.z) + c;
+    const int ay = rows_align(a.dy, a.lddy), az = rows_align(a.z, a.ldz), left = a.N - c;
     float sum[4] = {};
-    constexpr int U = 4, W = kPrepThreads / 32;
-    for (long long r = r0 + warp; r < r1; r += U * W) {
+    constexpr int U = 4, W = kPrepWarps * 4;  // rows in flight, rows of a CTA's step
+    for (long long r = r0 + warp * 4 + (lane >> 3); r < r1; r += U * W) {
       float g[U][4], t[U][4];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
@@ -411,21 +493,8 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[k][i] = t[k][i] = 0.f;
         if (row >= r1) continue;
-        if (vy) {
-          load4(dy + row * a.lddy + c, g[k]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + i < a.N) g[k][i] = to_f32(dy[row * a.lddy + c + i]);
-        }
-        if (a.act == VCB_ACT_NONE) continue;
-        if (vz) {
-          load4(z + row * a.ldz + c, t[k]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + i < a.N) t[k][i] = to_f32(z[row * a.ldz + c + i]);
-        }
+        four_at(dy + row * a.lddy, ay, left, g[k]);
+        if (a.act != VCB_ACT_NONE) four_at(z + row * a.ldz, az, left, t[k]);
       }
 #pragma unroll
       for (int k = 0; k < U; ++k) {
@@ -437,22 +506,26 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
           sum[i] += g[k][i];
         }
         // lddz is a multiple of 8, so a vector that crosses N stays in its row
-        if (a.dz && c < a.N) store4(static_cast<T*>(a.dz) + row * a.lddz + c, g[k]);
+        if (a.dz && left > 0) store4(static_cast<T*>(a.dz) + row * a.lddz + c, g[k]);
       }
     }
     if (a.db) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[warp][lane * 4 + i] = sum[i];
+      for (int i = 0; i < 4; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+        if (lane < 8) part[warp][lane * 4 + i] = sum[i];
+      }
       __syncthreads();
-      if (threadIdx.x < 128) {
+      if (threadIdx.x < kStrip) {
         float v = 0.f;
-        for (int w = 0; w < kPrepThreads / 32; ++w) v += part[w][threadIdx.x];
+        for (int w = 0; w < kPrepWarps; ++w) v += part[w][threadIdx.x];
         mine[threadIdx.x] = v;
       }
     }
     cluster_sync();
-    if (a.db && rank == 0 && threadIdx.x < 128) {
-      const int col = strip * 128 + threadIdx.x;
+    if (a.db && rank == 0 && threadIdx.x < kStrip) {
+      const int col = strip * kStrip + threadIdx.x;
       float v = 0.f;
       for (int k = 0; k < kPrepCluster; ++k) v += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
       if (col < a.N) static_cast<T*>(a.db)[col] = from_f32<T>(v);
@@ -470,11 +543,21 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
       const long long row = v / vecs;
       const int c = static_cast<int>(v - row * vecs) * 8;
       const uint16_t* src = static_cast<const uint16_t*>(q.src) + row * q.lds + c;
-      __align__(16) uint16_t e[8];
+      uint4 o;
+      if (c + 8 > q.cols) {
+        __align__(16) uint16_t e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(q.dst) + row * q.ldd + c) =
-          *reinterpret_cast<const uint4*>(e);
+        for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
+        o = *reinterpret_cast<const uint4*>(e);
+      } else if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+        o = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {  // the six elements between the first and the last as aligned words
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(src + 1);
+        const uint32_t a0 = src[0], w0 = w[0], w1 = w[1], w2 = w[2], a7 = src[7];
+        o = make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16, w2 >> 16 | a7 << 16);
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(q.dst) + row * q.ldd + c) = o;
     }
   }
 }
@@ -707,7 +790,7 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
     prep.dz = arena.take(matrix_bytes(b.M, b.N));
     dz = {prep.dz, prep.lddz, false};
   }
-  if (prep.dz || prep.db) prep.strips = (b.N + 127) / 128;
+  if (prep.dz || prep.db) prep.strips = (b.N + kStrip - 1) / kStrip;
   Operand w{}, x{};
   if (b.dx) w = readable(b.w, b.ldw, b.N, b.K, true, prep, arena);
   if (b.dw) x = readable(b.x, b.ldx, b.M, b.K, true, prep, arena);
