@@ -472,7 +472,7 @@ __device__ __forceinline__ int rows_align(const void* p, long long ld) {
 // HBM: dy and z are read and dz is written once; strips are narrow so that a matrix
 // of 2,000 columns keeps every SM reading.  The remaining CTAs copy.
 template <typename T>
-__global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThreads)
+__global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThreads, 5)
     prep_kernel(const __grid_constant__ Prep a) {
   __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -484,7 +484,7 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
     const T *dy = static_cast<const T*>(a.dy) + c, *z = static_cast<const T*>(a.z) + c;
     const int ay = rows_align(a.dy, a.lddy), az = rows_align(a.z, a.ldz), left = a.N - c;
     float sum[4] = {};
-    constexpr int U = 4, W = kPrepWarps * 4;  // rows in flight, rows of a CTA's step
+    constexpr int U = 2, W = kPrepWarps * 4;  // rows in flight, rows of a CTA's step
     for (long long r = r0 + warp * 4 + (lane >> 3); r < r1; r += U * W) {
       float g[U][4], t[U][4];
 #pragma unroll
@@ -533,31 +533,35 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
     cluster_sync();  // no CTA leaves while its sums are read
     return;
   }
-  // copies: eight elements per thread, written as one 16-byte vector
-  const long long t0 = (blockIdx.x - a.strips * kPrepCluster) * (long long)kPrepThreads + threadIdx.x;
-  const long long nt = (gridDim.x - a.strips * kPrepCluster) * (long long)kPrepThreads;
+  // copies: a warp per row, eight elements per lane, written as one 16-byte vector
+  const int first = (blockIdx.x - a.strips * kPrepCluster) * kPrepWarps + warp;
+  const int step = (gridDim.x - a.strips * kPrepCluster) * kPrepWarps;
   for (int k = 0; k < a.copies; ++k) {
     const Copy& q = a.copy[k];
-    const long long vecs = (q.cols + 7) / 8, all = q.rows * vecs;
-    for (long long v = t0; v < all; v += nt) {
-      const long long row = v / vecs;
-      const int c = static_cast<int>(v - row * vecs) * 8;
-      const uint16_t* src = static_cast<const uint16_t*>(q.src) + row * q.lds + c;
-      uint4 o;
-      if (c + 8 > q.cols) {
-        __align__(16) uint16_t e[8];
+    for (long long row = first; row < q.rows; row += step) {
+      const uint16_t* in = static_cast<const uint16_t*>(q.src) + row * q.lds;
+      uint16_t* out = static_cast<uint16_t*>(q.dst) + row * q.ldd;
+      const bool odd = reinterpret_cast<uintptr_t>(in) % 4 != 0;
+#pragma unroll 4
+      for (int c = lane * 8; c < q.cols; c += 256) {
+        const uint16_t* src = in + c;
+        uint4 o;
+        if (c + 8 > q.cols) {
+          __align__(16) uint16_t e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
-        o = *reinterpret_cast<const uint4*>(e);
-      } else if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
-        o = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {  // the six elements between the first and the last as aligned words
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(src + 1);
-        const uint32_t a0 = src[0], w0 = w[0], w1 = w[1], w2 = w[2], a7 = src[7];
-        o = make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16, w2 >> 16 | a7 << 16);
+          for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
+          o = *reinterpret_cast<const uint4*>(e);
+        } else if (!odd) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+          o = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {  // the six elements between the first and the last as aligned words
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(src + 1);
+          const uint32_t a0 = src[0], w0 = w[0], w1 = w[1], w2 = w[2], a7 = src[7];
+          o = make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16,
+                         w2 >> 16 | a7 << 16);
+        }
+        *reinterpret_cast<uint4*>(out + c) = o;
       }
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(q.dst) + row * q.ldd + c) = o;
     }
   }
 }
@@ -728,10 +732,9 @@ Operand readable(const void* p, long long ld, int rows, int cols, bool mn, Prep&
 }
 
 int launch_prep(const Prep& a, int type, cudaStream_t st, const char* who) {
-  long long vecs = 0;
-  for (int k = 0; k < a.copies; ++k) vecs += a.copy[k].rows * ((a.copy[k].cols + 7) / 8);
-  const long long ctas = std::min<long long>((vecs + kPrepThreads - 1) / kPrepThreads,
-                                             4LL * sm_count());
+  long long rows = 0;
+  for (int k = 0; k < a.copies; ++k) rows = std::max(rows, a.copy[k].rows);
+  const long long ctas = std::min<long long>((rows + kPrepWarps - 1) / kPrepWarps, 5LL * sm_count());
   const long long grid =
       (a.strips + (ctas + kPrepCluster - 1) / kPrepCluster) * (long long)kPrepCluster;
   if (grid == 0) return VCB_OK;
