@@ -6,21 +6,26 @@
 // This file has the kernel for small products and the entry points.  Both
 // gradients (and db) of a small layer leave in one launch.
 //
-// Small products are bound by latency: a 32 x 64 tile per CTA of 512 threads,
-// four groups of 128 threads each taking a quarter of every 64-deep step of
-// the contraction (16 warps hide each other's loads), added in order at the
-// end.  Accumulation is in fp32 whatever the type.
-#include "vcb_linear.cuh"
-
+// Small products are bound by latency, so a product of few tiles is spread as wide
+// as it goes: a 32 x 32 tile per CTA of 256 threads, four groups of 64 threads each
+// taking a quarter of every 64-deep step of the contraction, and the contraction cut
+// over up to 8 CTAs of a cluster when there are few tiles.  Groups are joined through
+// shared memory and CTAs through distributed shared memory, in order.  Operands lie
+// in shared memory by row, four entries of the contraction to a 16-byte chunk, chunks
+// XOR-ed with the row: writes and reads are free of bank conflicts whichever index of
+// the operand is contiguous.  A thread owns rows and columns 8 apart.  Accumulation is in fp32 whatever the
+// type.
 #include <algorithm>
+
+#include "vcb_linear_tc.cuh"
 
 namespace vcb {
 namespace lin {
 namespace {
 
-constexpr int kTI = 32, kTJ = 64, kTT = 64;  // tile rows, columns, contraction step
-constexpr int kGroups = 4, kSmallThreads = 128 * kGroups;
-constexpr int kPitchA = kTI + 4, kPitchB = kTJ + 4;
+constexpr int kTI = 32, kTJ = 32, kTT = 64;  // tile rows, columns, contraction step
+constexpr int kTile = kTI * kTJ;
+constexpr int kGroups = 4, kSmallThreads = 64 * kGroups;
 
 // One product out(i, j) = sum_t A(i, t) B(t, j) of a launch, and where its
 // tiles start in the grid.
@@ -28,157 +33,226 @@ struct Small {
   int I, J, T;
   const void *a, *a2, *b;  // a2: pre-activation beside the gradient a, or NULL
   long long lda, lda2, ldb;
-  int a_t, b_t;  // the contraction index is the contiguous one
+  int a_t, b_t;      // the contraction index is the contiguous one
+  int va, vb;        // ... and four of its entries are a vector
   int act;
-  void *out, *sum, *z;  // sum: row sums of A (db), or NULL
-  long long ldo, ldz, ldr;
-  const void *bias, *res;
-  int epilogue;  // apply bias, act and res
+  void* sum;         // row sums of A (db), or NULL
+  Epilogue epi;      // out may be NULL
   int tiles_j, tiles;
 };
 
 struct SmallPair {
   Small p[2];
+  int split;  // CTAs (a cluster) per tile
 };
 
+// Entries t .. t + 3 of a row: `step` elements apart, `left` of them exist.
 template <typename T>
-__device__ __forceinline__ float a_value(const Small& s, int i, int t) {
-  if (i >= s.I || t >= s.T) return 0.f;
-  const long long r = s.a_t ? i : t, c = s.a_t ? t : i;
-  const float v = to_f32(static_cast<const T*>(s.a)[r * s.lda + c]);
-  if (!s.a2) return v;
-  return act_grad(v, to_f32(static_cast<const T*>(s.a2)[r * s.lda2 + c]), s.act);
+__device__ __forceinline__ void quad(const T* p, long long step, bool vec, int left,
+                                     float (&v)[4]) {
+  if (vec && left >= 4) {
+    load4(p, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = k < left ? to_f32(p[k * step]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ int chunk_at(int row, int chunk) {
+  return row * kTT + ((chunk ^ (row & 7)) << 2);
 }
 
 template <typename T>
-__device__ __forceinline__ float b_value(const Small& s, int t, int j) {
-  if (j >= s.J || t >= s.T) return 0.f;
-  const long long at = s.b_t ? static_cast<long long>(j) * s.ldb + t
-                             : static_cast<long long>(t) * s.ldb + j;
-  return to_f32(static_cast<const T*>(s.b)[at]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_constant__ SmallPair pair) {
-  constexpr int kStageA = kTT * kPitchA, kStageB = kTT * kPitchB;
-  constexpr int kJoin = (kGroups - 1) * 128 * 16;
-  __shared__ float buf[kStageA + kStageB > kJoin ? kStageA + kStageB : kJoin];
-  __shared__ float row_sum[kGroups][kTI];
-  float *sa = buf, *sb = buf + kStageA;
-  const int second = static_cast<int>(blockIdx.x) >= pair.p[0].tiles;
+__global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_constant__ SmallPair pair) {
+  // operands of a step; then the groups' sums; then this CTA's sum of the tile
+  __shared__ __align__(16) float buf[(kTI + kTJ) * kTT > kGroups * kTile ? (kTI + kTJ) * kTT
+                                                                        : kGroups * kTile];
+  __shared__ float row_sum[kTT / 4][kTI], row_mine[kTI];
+  float *sa = buf, *sb = buf + kTI * kTT;
+  const int size = pair.split, lg = 31 - __clz(size);
+  const int rank = blockIdx.x & (size - 1), unit = blockIdx.x >> lg;
+  const int second = unit >= pair.p[0].tiles;
   const Small& s = pair.p[second];
-  const int tile = blockIdx.x - (second ? pair.p[0].tiles : 0);
+  const int tile = unit - (second ? pair.p[0].tiles : 0);
   const int i0 = tile / s.tiles_j * kTI, j0 = tile % s.tiles_j * kTJ;
-  const int tid = threadIdx.x, group = tid >> 7, in = tid & 127;
-  const int ty = in >> 4, tx = in & 15;
-  constexpr int NA = kTI * kTT / kSmallThreads, NB = kTJ * kTT / kSmallThreads;
-  float ra[NA], rb[NB];
-  // neighbouring threads read neighbouring elements, whichever index they run over
-  auto fetch = [&](int t0) {
+  const int tid = threadIdx.x, group = tid >> 6, in = tid & 63, ty = in >> 3, tx = in & 7;
+  const int steps = (s.T + kTT - 1) / kTT;
+  const int s0 = steps * rank >> lg, s1 = steps * (rank + 1) >> lg;
+  // this thread's two quads of A and of B: lanes run along the contiguous index
+  const auto row_of = [&](int contiguous_t, int q) {
+    return contiguous_t ? (tid >> 4) + 16 * q : tid & 31;
+  };
+  const auto chunk_of = [&](int contiguous_t, int q) {
+    return contiguous_t ? tid & 15 : (tid >> 5) + 8 * q;
+  };
+  const long long ta = s.a_t ? 1 : s.lda, ta2 = s.a_t ? 1 : s.lda2, tb = s.b_t ? 1 : s.ldb;
+  const T *pa[2], *pa2[2], *pb[2];
 #pragma unroll
-    for (int k = 0; k < NA; ++k) {
-      const int e = tid + k * kSmallThreads;
-      const int i = s.a_t ? e / kTT : e % kTI, t = s.a_t ? e % kTT : e / kTI;
-      ra[k] = a_value<T>(s, i0 + i, t0 + t);
-    }
+  for (int q = 0; q < 2; ++q) {
+    const int ra = i0 + row_of(s.a_t, q), ca = (s0 * 16 + chunk_of(s.a_t, q)) * 4;
+    const int rb = j0 + row_of(s.b_t, q), cb = (s0 * 16 + chunk_of(s.b_t, q)) * 4;
+    pa[q] = static_cast<const T*>(s.a) + (s.a_t ? ra * s.lda : ra) + ca * ta;
+    pa2[q] = static_cast<const T*>(s.a2) + (s.a_t ? ra * s.lda2 : ra) + ca * ta2;
+    pb[q] = static_cast<const T*>(s.b) + (s.b_t ? rb * s.ldb : rb) + cb * tb;
+  }
+  float fa[2][4], fb[2][4];
+  const auto fetch = [&](int step) {
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int e = tid + k * kSmallThreads;
-      const int j = s.b_t ? e / kTT : e % kTJ, t = s.b_t ? e % kTT : e / kTJ;
-      rb[k] = b_value<T>(s, t0 + t, j0 + j);
+    for (int q = 0; q < 2; ++q) {
+      const int la = i0 + row_of(s.a_t, q) < s.I ? s.T - (step * 16 + chunk_of(s.a_t, q)) * 4 : 0;
+      quad(pa[q], ta, s.va, la, fa[q]);
+      pa[q] += kTT * ta;
+      if (s.a2) {
+        float z[4];
+        quad(pa2[q], ta2, s.va, la, z);
+        pa2[q] += kTT * ta2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) fa[q][k] = act_grad(fa[q][k], z[k], s.act);
+      }
+      quad(pb[q], tb, s.vb,
+           j0 + row_of(s.b_t, q) < s.J ? s.T - (step * 16 + chunk_of(s.b_t, q)) * 4 : 0, fb[q]);
+      pb[q] += kTT * tb;
     }
   };
-  float acc[4][4] = {}, rs[4] = {};
-  const bool sums = s.sum && j0 == 0 && tx == 0;
-  fetch(0);
-  for (int t0 = 0; t0 < s.T; t0 += kTT) {
+  float acc[4][4] = {}, rs = 0.f;
+  const bool sums = s.sum && j0 == 0;
+  if (s0 < s1) fetch(s0);
+  for (int step = s0; step < s1; ++step) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NA; ++k) {
-      const int e = tid + k * kSmallThreads;
-      const int i = s.a_t ? e / kTT : e % kTI, t = s.a_t ? e % kTT : e / kTI;
-      sa[t * kPitchA + i] = ra[k];
-    }
-#pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int e = tid + k * kSmallThreads;
-      const int j = s.b_t ? e / kTT : e % kTJ, t = s.b_t ? e % kTT : e / kTJ;
-      sb[t * kPitchB + j] = rb[k];
+    for (int q = 0; q < 2; ++q) {
+      *reinterpret_cast<float4*>(sa + chunk_at(row_of(s.a_t, q), chunk_of(s.a_t, q))) =
+          make_float4(fa[q][0], fa[q][1], fa[q][2], fa[q][3]);
+      *reinterpret_cast<float4*>(sb + chunk_at(row_of(s.b_t, q), chunk_of(s.b_t, q))) =
+          make_float4(fb[q][0], fb[q][1], fb[q][2], fb[q][3]);
     }
     __syncthreads();
-    if (t0 + kTT < s.T) fetch(t0 + kTT);
+    if (step + 1 < s1) fetch(step + 1);
+    if (sums) {
 #pragma unroll
-    for (int k = 0; k < kTT / kGroups; ++k) {
-      const int t = group * (kTT / kGroups) + k;
-      const float4 av = *reinterpret_cast<const float4*>(sa + t * kPitchA + ty * 4);
-      const float4 bv = *reinterpret_cast<const float4*>(sb + t * kPitchB + tx * 4);
-      const float a4[4] = {av.x, av.y, av.z, av.w}, b4[4] = {bv.x, bv.y, bv.z, bv.w};
+      for (int q = 0; q < 2; ++q) {
+        const float4 v =
+            *reinterpret_cast<const float4*>(sa + chunk_at(tid & 31, (tid >> 5) + 8 * q));
+        rs += (v.x + v.y) + (v.z + v.w);
+      }
+    }
+#pragma unroll 2
+    for (int c = group * 4; c < group * 4 + 4; ++c) {
+      // rows 8 apart share their place in the XOR
+      const float* at_a = sa + ty * kTT + ((c ^ ty) << 2);
+      const float* at_b = sb + tx * kTT + ((c ^ tx) << 2);
+      float4 bv[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bv[k] = *reinterpret_cast<const float4*>(at_b + 8 * kTT * k);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const float4 av = *reinterpret_cast<const float4*>(at_a + 8 * kTT * i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a4[i], b4[j], acc[i][j]);
-        if (sums) rs[i] += a4[i];
+        for (int j = 0; j < 4; ++j) {
+          acc[i][j] = fmaf(av.x, bv[j].x, acc[i][j]);
+          acc[i][j] = fmaf(av.y, bv[j].y, acc[i][j]);
+          acc[i][j] = fmaf(av.z, bv[j].z, acc[i][j]);
+          acc[i][j] = fmaf(av.w, bv[j].w, acc[i][j]);
+        }
       }
     }
   }
+  // the four groups' sums, in order
   __syncthreads();
-  if (group > 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) buf[((group - 1) * 16 + i) * 128 + in] = acc[i >> 2][i & 3];
-  }
-  if (sums) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) row_sum[group][ty * 4 + i] = rs[i];
-  }
+  for (int k = 0; k < 16; ++k)
+    buf[group * kTile + (ty + 8 * (k >> 2)) * kTJ + tx + 8 * (k & 3)] = acc[k >> 2][k & 3];
+  if (sums) row_sum[tid >> 5][tid & 31] = rs;
   __syncthreads();
-  if (s.sum && j0 == 0 && tid < kTI && i0 + tid < s.I) {
-    float v = 0.f;
+  constexpr int kEntries = kTile / kSmallThreads;
+  float v[kEntries], db = 0.f;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) v += row_sum[k][tid];
-    static_cast<T*>(s.sum)[i0 + tid] = from_f32<T>(v);
+  for (int k = 0; k < kEntries; ++k) {
+    v[k] = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) v[k] += buf[g * kTile + tid + k * kSmallThreads];
   }
-  if (group > 0 || !s.out) return;
+  if (sums && tid < kTI) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long r = i0 + ty * 4 + i;
-    if (r >= s.I) break;
+    for (int k = 0; k < kSmallThreads / 32; ++k) db += row_sum[k][tid];
+  }
+  const auto put = [&](int e, float value) {
+    const int i = i0 + e / kTJ, j = j0 + e % kTJ;
+    if (!s.epi.out || i >= s.I || j >= s.J) return;
+    float one[1] = {value};
+    emit_column<T, 1>(s.epi, s.I, s.J, i, j,
+                      s.epi.bias ? to_f32(static_cast<const T*>(s.epi.bias)[j]) : 0.f, one);
+  };
+  if (size == 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = j0 + tx * 4 + j;
-      if (c >= s.J) break;
-      float v = acc[i][j];
+    for (int k = 0; k < kEntries; ++k) put(tid + k * kSmallThreads, v[k]);
+  } else {
+    // the CTAs of the cluster, in order; each finishes its share of the tile
+    __syncthreads();
 #pragma unroll
-      for (int k = 0; k < kGroups - 1; ++k) v += buf[(k * 16 + i * 4 + j) * 128 + in];
-      if (s.epilogue) {
-        if (s.bias) v += to_f32(static_cast<const T*>(s.bias)[c]);
-        if (s.z) static_cast<T*>(s.z)[r * s.ldz + c] = from_f32<T>(v);
-        v = act_value(v, s.act);
-        if (s.res) v += to_f32(static_cast<const T*>(s.res)[r * s.ldr + c]);
-      }
-      static_cast<T*>(s.out)[r * s.ldo + c] = from_f32<T>(v);
+    for (int k = 0; k < kEntries; ++k) buf[tid + k * kSmallThreads] = v[k];
+    if (sums && tid < kTI) row_mine[tid] = db;
+    cluster_sync();
+    const int share = kTile >> lg;
+    for (int k = tid; k < share; k += kSmallThreads) {
+      const int e = rank * share + k;
+      float sum = 0.f;
+      for (int g = 0; g < size; ++g) sum += peer_f32(map_rank(smem_u32(buf + e), g));
+      put(e, sum);
     }
+    if (sums && rank == 0 && tid < kTI) {
+      db = 0.f;
+      for (int g = 0; g < size; ++g) db += peer_f32(map_rank(smem_u32(row_mine + tid), g));
+    }
+    cluster_sync();  // no CTA leaves while its sums are read
   }
+  if (sums && rank == 0 && tid < kTI && i0 + tid < s.I)
+    static_cast<T*>(s.sum)[i0 + tid] = from_f32<T>(db);
 }
 
 int tiles_of(Small& s) {
-  if (!s.sum && (!s.out || s.J == 0)) return s.tiles = 0;
-  s.tiles_j = s.out ? std::max(1, (s.J + kTJ - 1) / kTJ) : 1;
+  if (!s.sum && (!s.epi.out || s.J == 0)) return s.tiles = 0;
+  s.tiles_j = s.epi.out ? std::max(1, (s.J + kTJ - 1) / kTJ) : 1;
   const long long n = static_cast<long long>((s.I + kTI - 1) / kTI) * s.tiles_j;
-  s.tiles = n > 0x3fffffff ? -1 : static_cast<int>(n);
+  s.tiles = n > 0x07ffffff ? -1 : static_cast<int>(n);
   return s.tiles;
 }
 
-int launch_small(const SmallPair& pair, int type, cudaStream_t st, const char* who) {
-  if (pair.p[0].tiles < 0 || pair.p[1].tiles < 0)
-    return fail(VCB_ERR_UNSUPPORTED, "%s: too many output tiles", who);
-  const unsigned grid = pair.p[0].tiles + pair.p[1].tiles;
-  if (grid == 0) return VCB_OK;
-  if (type == VCB_F32)
-    small_kernel<float><<<grid, kSmallThreads, 0, st>>>(pair);
-  else if (type == VCB_BF16)
-    small_kernel<__nv_bfloat16><<<grid, kSmallThreads, 0, st>>>(pair);
-  else
-    small_kernel<__half><<<grid, kSmallThreads, 0, st>>>(pair);
+// Rows of four-element vectors (of the type's size).
+bool vectors(const void* p, long long ld, int type) {
+  const int b = 4 * dtype_bytes(type);
+  return reinterpret_cast<uintptr_t>(p) % b == 0 && ld % 4 == 0;
+}
+
+int launch_small(SmallPair& pair, int type, cudaStream_t st, const char* who) {
+  int steps = 1;
+  for (Small& s : pair.p) {
+    if (s.tiles < 0) return fail(VCB_ERR_UNSUPPORTED, "%s: too many output tiles", who);
+    s.va = s.a_t && vectors(s.a, s.lda, type) && (!s.a2 || vectors(s.a2, s.lda2, type));
+    s.vb = s.b_t && vectors(s.b, s.ldb, type);
+    if (s.tiles) steps = std::max(steps, (s.T + kTT - 1) / kTT);
+  }
+  const int tiles = pair.p[0].tiles + pair.p[1].tiles;
+  if (tiles == 0) return VCB_OK;
+  // a cluster per tile while four CTAs per SM hold all of them and each has a step
+  pair.split = 1;
+  while (pair.split < 8 && 2 * pair.split <= steps && 2LL * pair.split * tiles <= 4LL * sm_count())
+    pair.split *= 2;
+  const auto kernel = type == VCB_F32    ? small_kernel<float>
+                      : type == VCB_BF16 ? small_kernel<__nv_bfloat16>
+                                         : small_kernel<__half>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * pair.split));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = pair.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, pair);
+  if (e != cudaSuccess) return cuda_fail(e, who);
   return check_launch(who);
 }
 
@@ -188,8 +262,7 @@ int small_forward(const Fwd& f, cudaStream_t st) {
   s.I = f.M, s.J = f.N, s.T = f.K;
   s.a = f.x, s.lda = f.ldx, s.a_t = 1;
   s.b = f.w, s.ldb = f.ldw, s.b_t = 1;
-  s.act = f.act, s.out = f.y, s.ldo = f.ldy, s.z = f.z, s.ldz = f.ldz;
-  s.bias = f.bias, s.res = f.res, s.ldr = f.ldr, s.epilogue = 1;
+  s.epi = {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
   tiles_of(s);
   return launch_small(pair, f.type, st, "vcb_linear_forward");
 }
@@ -201,13 +274,14 @@ int small_backward(const Bwd& b, cudaStream_t st) {
   x.I = b.M, x.J = b.K, x.T = b.N;
   x.a = b.dy, x.lda = b.lddy, x.a2 = z, x.lda2 = b.ldz, x.a_t = 1, x.act = b.act;
   x.b = b.w, x.ldb = b.ldw, x.b_t = 0;
-  x.out = b.dx, x.ldo = b.lddx;
+  x.epi = {b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
   if (b.dx) tiles_of(x);
   Small& w = pair.p[1];
   w.I = b.N, w.J = b.K, w.T = b.M;
   w.a = b.dy, w.lda = b.lddy, w.a2 = z, w.lda2 = b.ldz, w.a_t = 0, w.act = b.act;
   w.b = b.x, w.ldb = b.ldx, w.b_t = 0;
-  w.out = b.dw, w.ldo = b.lddw, w.sum = b.db;
+  w.epi = {b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+  w.sum = b.db;
   if (b.dw || b.db) tiles_of(w);
   return launch_small(pair, b.type, st, "vcb_linear_backward");
 }
