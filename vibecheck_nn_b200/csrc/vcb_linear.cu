@@ -293,6 +293,23 @@ namespace {
 bool misaligned(const void* p, int type) {
   return reinterpret_cast<uintptr_t>(p) % dtype_bytes(type) != 0;
 }
+// Which calls take the kernels for few rows (vcb_linear_rows.cu).  Forward in us,
+// others against them: fp32 1 x 4096 x 4096 62 against 7.7, 8 x 4096 x 4096 37
+// against 26, 16 x 1024 x 1024 7.7 against 5.4 but 16 x 4096 x 4096 37 against 48;
+// bf16 8 x 1024 x 1024 5.9 against 4.5, 1 x 4096 x 4096 equal, 4 x 4096 x 4096 8.8
+// against 25.  Backward: fp32 16 x 1024 x 1024 36 against 14, 16 x 256 x 256 6.7
+// against 8.8; bf16 4 x 4096 x 4096 44 against 27, 16 x 1024 x 1024 10 against 17.
+bool few_rows_forward(long long M, long long N, long long K, int type) {
+  if (M <= 0 || N <= 0 || K <= 0) return false;
+  if (type == VCB_F32) return M <= 8 || (M <= lin::kFewRows && N * K <= (1 << 20));
+  return M <= 8 && M * N * K <= (1 << 23);
+}
+
+bool few_rows_backward(long long M, long long N, long long K, int type) {
+  if (M <= 0 || N <= 0 || K <= 0) return false;
+  if (M <= 4) return true;
+  return type == VCB_F32 && M <= lin::kFewRows && N * K >= (1 << 18);
+}
 }  // namespace
 }  // namespace vcb
 
@@ -300,14 +317,14 @@ using namespace vcb;
 
 extern "C" size_t vcb_linear_forward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
                                                int32_t rows16) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || few_rows_forward(M, N, K, type)) return 0;
   if (type == VCB_F32) return lin::f32_forward_bytes(M, N, K);
   return rows16 ? 0 : lin::tc_forward_bytes(M, N, K);
 }
 
 extern "C" size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
                                                 int32_t act, int32_t rows16) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || few_rows_backward(M, N, K, type)) return 0;
   if (type == VCB_F32) return lin::f32_backward_bytes(M, N, K);
   return lin::tc_backward_bytes(M, N, K, act, rows16);
 }
@@ -336,6 +353,7 @@ extern "C" int vcb_linear_forward(int32_t M, int32_t N, int32_t K, int32_t type,
       misaligned(z, type))
     return fail(VCB_ERR_INVALID, "vcb_linear_forward: NULL or misaligned pointer");
   const lin::Fwd f{M, N, K, type, act, ldx, ldw, ldr, ldy, ldz, x, w, bias, residual, y, z};
+  if (few_rows_forward(M, N, K, type)) return lin::rows_forward(f, static_cast<cudaStream_t>(stream));
   const bool f32 = lin::f32_forward_fits(f);
   if (!f32 && !lin::tc_forward_fits(f)) return lin::small_forward(f, static_cast<cudaStream_t>(stream));
   const int rc = check_workspace(workspace, workspace_bytes,
@@ -362,6 +380,7 @@ extern "C" int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type
       misaligned(dx, type) || misaligned(dw, type) || misaligned(db, type))
     return fail(VCB_ERR_INVALID, "vcb_linear_backward: NULL or misaligned pointer");
   const lin::Bwd b{M, N, K, type, act, lddy, ldx, ldw, ldz, lddx, lddw, dy, x, w, z, dx, dw, db};
+  if (few_rows_backward(M, N, K, type)) return lin::rows_backward(b, static_cast<cudaStream_t>(stream));
   const bool f32 = lin::f32_backward_fits(b);
   if (!f32 && !lin::tc_backward_fits(b)) return lin::small_backward(b, static_cast<cudaStream_t>(stream));
   const int rc = check_workspace(workspace, workspace_bytes,

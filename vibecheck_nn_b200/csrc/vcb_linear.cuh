@@ -213,6 +213,11 @@ struct Bwd {
   void *dx, *dw, *db;
 };
 
+// Up to kFewRows rows (vcb_linear_rows.cu): M, N, K > 0.
+constexpr int kFewRows = 16;
+int rows_forward(const Fwd& f, cudaStream_t st);
+int rows_backward(const Bwd& b, cudaStream_t st);
+
 // Tensor-core paths (vcb_linear_tc.cu: 16-bit types; vcb_linear_f32.cu).  `bytes`: what they need
 // of the workspace; the launch functions take one that large, 16-byte aligned.
 bool tc_forward_fits(const Fwd& f);

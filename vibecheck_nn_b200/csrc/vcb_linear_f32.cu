@@ -601,7 +601,10 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
 }
 
 // ---- host ----
-constexpr long long kTcLeast = 1LL << 26;  // M N K from which the tensor cores are used
+// M N K from which the tensor cores are used.  Forward: 64 x 1024 x 1024 (2^26) 12.6
+// us against 15.4 on the FP32 units, 64 x 512 x 512 9.9 against 5.8.  Backward, with
+// two more launches: 512^3 (2^27) 38 against 46, 256 x 512 x 512 39 against 23.
+constexpr long long kTcLeast = 1LL << 26, kTcLeastBackward = 1LL << 27;
 
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -722,18 +725,18 @@ bool vec16(const void* p, long long ld) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0;
 }
 
-bool fits(long long M, long long N, long long K) {
+bool fits(long long M, long long N, long long K, long long least) {
   const long long most = 1LL << 28;
-  return M * N * K >= kTcLeast && M < most && N < most && K < most && (M + 63) / 64 * ((N + 127) / 128) < most &&
+  return M * N * K >= least && M < most && N < most && K < most && (M + 63) / 64 * ((N + 127) / 128) < most &&
          (M + 63) / 64 * ((K + 127) / 128) < most && (N + 63) / 64 * ((K + 127) / 128) < most;
 }
 
 }  // namespace
 
-bool f32_forward_fits(const Fwd& f) { return f.type == VCB_F32 && fits(f.M, f.N, f.K); }
+bool f32_forward_fits(const Fwd& f) { return f.type == VCB_F32 && fits(f.M, f.N, f.K, kTcLeast); }
 
 size_t f32_forward_bytes(int M, int N, int K) {
-  if (!fits(M, N, K)) return 0;
+  if (!fits(M, N, K, kTcLeast)) return 0;
   return halves_bytes(M, K) + halves_bytes(N, K) + up256(M * 4LL) + up256(N * 4LL) + 256;
 }
 
@@ -768,11 +771,11 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
 }
 
 bool f32_backward_fits(const Bwd& b) {
-  return b.type == VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K);
+  return b.type == VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K, kTcLeastBackward);
 }
 
 size_t f32_backward_bytes(int M, int N, int K) {
-  if (!fits(M, N, K)) return 0;
+  if (!fits(M, N, K, kTcLeastBackward)) return 0;
   return 2 * halves_bytes(M, N) + halves_bytes(N, K) + halves_bytes(M, K) + up256(M * 4LL) +
          up256(N * 4LL) + 2 * up256(K * 4LL) + 256;
 }

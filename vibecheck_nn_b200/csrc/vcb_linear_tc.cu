@@ -693,7 +693,9 @@ int launch_type(Launch& L, const Plan& plan, int type, cudaStream_t st, const ch
 
 namespace {
 
-constexpr long long kTcLeast = 1LL << 24;  // M N K from which the tensor cores are used
+// M N K from which the tensor cores are used: bf16 64 x 256 x 256 (2^22) 4.9 us
+// against 5.4 on the FP32 units, 8 x 1024 x 1024 backward 10 against 45.
+constexpr long long kTcLeast = 1LL << 20;
 
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 size_t matrix_bytes(long long rows, long long cols) {
