@@ -302,6 +302,11 @@ struct Launch32 {
   int units0, units, split;
 };
 
+// Sixteen epilogue warps: what they do at a tile's end (scales, activation, stores)
+// runs beside two stages of the next tile's MMAs only, so it is spread as wide as
+// registers allow.
+constexpr int kEpi = 16, kF32Threads = (kEpi + 2) * 32;
+
 template <int BN, bool PAIR>
 struct Cfg {
   static constexpr int kRowsB = PAIR ? BN / 2 : BN;
@@ -311,8 +316,8 @@ struct Cfg {
   static constexpr int kSmem = kStages * kStage + 1024;
   static constexpr int kBufs = BN == 256 ? 2 : 4;
   static constexpr int kColumns = kBufs * BN;  // of tensor memory
-  static constexpr int kCols = BN / 2;         // of an epilogue thread
-  static constexpr int kArrivals = kEpiWarps * (PAIR ? 2 : 1);
+  static constexpr int kCols = BN / (kEpi / 4);  // of an epilogue thread
+  static constexpr int kArrivals = kEpi * (PAIR ? 2 : 1);
 };
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
@@ -352,7 +357,7 @@ __device__ __forceinline__ void load_halves(uint32_t dst, const CUtensorMap* map
 // Otherwise a 128 x BN tile of the first product per cluster of L.split CTAs, each
 // with a part of the contraction; the parts are joined in the order of the ranks.
 template <int BN, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant__ Launch32 L) {
+__global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_constant__ Launch32 L) {
   using C = Cfg<BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -402,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
     return PAIR ? nk : static_cast<int>((long long)nk * (rank + 1) / size);
   };
 
-  if (warp == kEpiWarps) {  // TMA producer
+  if (warp == kEpi) {  // TMA producer
     const bool one = elect_one();
     unsigned g = 0;
     Ring ring;
@@ -433,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
     if (!PAIR || rank == 0)  // the copies in flight land before the CTAs leave
       for (unsigned k = g > C::kStages ? g - C::kStages : 0; k < g; ++k)
         if (!mbar_wait(&full[k % C::kStages], (k / C::kStages) & 1, kSpinLimit)) failed = 1;
-  } else if (warp == kEpiWarps + 1) {  // MMA issuer
+  } else if (warp == kEpi + 1) {  // MMA issuer
     if (!PAIR || rank == 0) {
       const bool one = elect_one();
       Ring ring, buf;
@@ -448,9 +453,9 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
         const uint32_t idesc = p.idesc;
         for (int kb = begin(p.nk); kb < k1;
              ++kb, ++chunks, ring.next(C::kStages), buf.next(C::kBufs)) {
-          if (!mbar_wait_cluster(&full[ring.s], ring.parity, kSpinLimit, vfailed) ||
+          if (!mbar_wait(&full[ring.s], ring.parity, kSpinLimit, vfailed) ||
               (chunks >= C::kBufs &&
-               !mbar_wait_cluster(&acc_free[buf.s], buf.parity ^ 1, kDoneLimit, vfailed))) {
+               !mbar_wait(&acc_free[buf.s], buf.parity ^ 1, kDoneLimit, vfailed))) {
             ok = false;
             break;
           }
@@ -502,24 +507,19 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
         if (!ok) break;
         fence_after_sync();
 #pragma unroll
-        for (int c = 0; c < kCols; c += 32) {
-          uint32_t r[16], s[16];
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t r[16];
           tmem_ld16(base + buf.s * BN + c, r);
-          tmem_ld16(base + buf.s * BN + c + 16, s);
-          tmem_wait_ld(r, s);
+          tmem_wait_ld(r);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
+          for (int k = 0; k < 16; ++k)
             acc[c + k] = __fadd_rn(acc[c + k], __uint_as_float(r[k]));
-            acc[c + 16 + k] = __fadd_rn(acc[c + 16 + k], __uint_as_float(s[k]));
-          }
         }
         fence_before_sync();
         __syncwarp();
         if (lane == 0) {
           if (PAIR)
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                             map_rank(smem_u32(&acc_free[buf.s]), 0))
-                         : "memory");
+            arrive_leader(&acc_free[buf.s]);
           else
             mbar_arrive(&acc_free[buf.s]);
         }
@@ -537,20 +537,23 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
                        : "memory");
         break;
       }
-      // a lane keeps its column: a warp's accesses are 32 neighbouring floats
-      const int I = p.I, J = p.J, j = j0 + lane;
-      const int ea = j < J ? scale_exp(__ldg(p.most_a + j)) : 0;
-      const float bias = p.epi.bias && j < J ? static_cast<const float*>(p.epi.bias)[j] : 0.f;
+      const int I = p.I, J = p.J, j = j0 + (lane & ~3);
+      const int ea = j0 + lane < J ? scale_exp(__ldg(p.most_a + j0 + lane)) : 0;
+      float bias[4];
+      bias_at<float>(p.epi, J, j, bias);
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
         if (i0 + c < I) {  // warp-uniform
           const int eb = i0 + c + (lane & 15) < I
                              ? scale_exp(__ldg(p.most_b + i0 + c + (lane & 15))) : 0;
+          Residual<float, 4> res;
+          res.fetch(p.epi, I, J, i0 + c + (lane & 3), j);
           float v[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k)
             v[k] = scaled(acc[c + k], ea + __shfl_sync(0xffffffffu, eb, k));
-          emit_column<float, 16>(p.epi, I, J, i0 + c, j, bias, v);
+          transpose16(v, lane);
+          emit<float, 4>(p.epi, I, J, i0 + c + (lane & 3), j, bias, v, res);
         }
       }
     }
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
   __syncthreads();
   if (PAIR || size > 1) cluster_sync();
   if (!PAIR && size > 1) {
-    if (warp < kEpiWarps) {
+    if (warp < kEpi) {
       const Prod32& p = L.p[0];
       int ti, tj;
       tile_at(p.tiles_i, p.tiles_j, first, ti, tj);
@@ -572,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const __grid_constant_
       bias_at<float>(e, p.J, j, bias);
 #pragma unroll
       for (int k = 0; k < 4; ++k) ea[k] = j + k < p.J ? scale_exp(__ldg(p.most_a + j + k)) : 0;
-      for (int c = rank * kEpiWarps + warp; c < columns; c += size * kEpiWarps) {
+      for (int c = rank * kEpi + warp; c < columns; c += size * kEpi) {
         const uint32_t at = smem + (c * kTileJ + lane * 4) * 4;
         float v[4] = {};
         for (int k = 0; k < size; ++k) {
@@ -702,7 +705,7 @@ int launch(const Launch32& L, cudaStream_t st, const char* who) {
   const int size = PAIR ? 2 : L.split;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kF32Threads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];

@@ -210,13 +210,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Desc da = operand(smem, p.a_mn, kPairStage);
         const Desc db = operand(smem + kBytesA, p.b_mn, kPairStage);
         const uint32_t idesc = p.idesc;
-        if (t >= 2 && !mbar_wait_cluster(&acc_free[q], ((t >> 1) - 1) & 1, kDoneLimit, vfailed)) {
+        if (t >= 2 && !mbar_wait(&acc_free[q], ((t >> 1) - 1) & 1, kDoneLimit, vfailed)) {
           ok = false;
           break;
         }
         for (int kb = 0; kb < nk; ++kb, ring.next(kPairStages)) {
           const int s = ring.s;
-          if (!mbar_wait_cluster(&full[s], ring.parity, kSpinLimit, vfailed)) {
+          if (!mbar_wait(&full[s], ring.parity, kSpinLimit, vfailed)) {
             ok = false;
             break;
           }
@@ -256,9 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       fence_before_sync();
       __syncwarp();
       if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                         map_rank(smem_u32(&acc_free[q]), 0))
-                     : "memory");
+        arrive_leader(&acc_free[q]);
     }
     if (!ok) failed = 1;
   }

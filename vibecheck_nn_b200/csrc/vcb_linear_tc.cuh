@@ -55,22 +55,13 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   return r;
 }
 
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, unsigned parity, unsigned limit,
-                                                  const volatile int* abort) {
-  const uint32_t a = smem_u32(bar);
-  for (unsigned i = 0; i < limit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((i & 255) == 255 && *abort) return false;
-  }
-  return false;
+// Arrive on `bar` of the pair's first CTA.  Relaxed: what it hands over are reads of
+// tensor memory that have completed (a release would fence all memory, some 500
+// cycles each time).
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                   map_rank(smem_u32(bar), 0))
+               : "memory");
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
