@@ -708,35 +708,32 @@ size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t ty
  * ignore_index of logsumexp(x_r) - x_r,label, 0 when there is none; ignored
  * rows get gradient 0.  A row whose logits are all -inf has loss +inf and
  * gradient 0; a row whose label is outside [0, C) becomes NaN, and so does the
- * loss.  workspace: vcb_cross_entropy_workspace(R) bytes, 16-byte aligned. */
+ * loss.  workspace: vcb_cross_entropy_workspace bytes, 16-byte aligned (NULL when
+ * that is 0). */
 int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
                       const int64_t* labels, int64_t ignore_index, float* loss, void* grad,
                       int64_t ldg, void* workspace, size_t workspace_bytes, void* stream);
-size_t vcb_cross_entropy_workspace(int32_t R);
+size_t vcb_cross_entropy_workspace(int32_t R, int32_t C);
 
-/* One AdamW step over `count` tensors.  Tensor i's moments are the elements
- * [off, off + n) of the state, off a multiple of 256.  state_bits 32: m and v
- * are fp32 and the scales unused; 8: m int8 and v uint8 codes with one fp32
- * scale per 256 elements,
+/* One AdamW step over `count` tensors: tensor i has n[i] weights at p[i] and
+ * gradients at g[i], and its moments are the elements [off[i], off[i] + n[i]) of
+ * the state, off[i] a multiple of 256.  state_bits 32: m and v are fp32 and the
+ * scales unused; 8: m int8 and v uint8 codes with one fp32 scale per 256
+ * elements,
  *   m = m_scale sgn(c) (c / 127)^2,   v = v_scale (c / 255)^4.
  * Constants of step t: b1, c1 = 1 - b1, b2, c2 = 1 - b2, eps, size = lr / (1 -
  * b1^t), root = (1 - b2^t)^-1/2, keep = 1 - lr * weight_decay, and the key of
  * the 8-bit codes' rounding noise.  Gradients have the weights' type or fp32.
- * `tensors` is read before the call returns. */
-typedef struct {
-  void* p;
-  const void* g;
-  int64_t n, off;
-} vcb_adamw_tensor;
-
+ * The four arrays are host memory, read before the call returns. */
 typedef struct {
   float b1, c1, b2, c2, eps, size, root, keep;
   uint32_t key;
 } vcb_adamw_opts;
 
-int vcb_adamw(int32_t count, const vcb_adamw_tensor* tensors, int32_t p_type, int32_t g_type,
-              int32_t state_bits, void* m, void* v, float* m_scale, float* v_scale,
-              const vcb_adamw_opts* opts, void* stream);
+int vcb_adamw(int32_t count, void* const* p, const void* const* g, const int64_t* n,
+              const int64_t* off, int32_t p_type, int32_t g_type, int32_t state_bits, void* m,
+              void* v, float* m_scale, float* v_scale, const vcb_adamw_opts* opts,
+              void* stream);
 
 /* The values that n (a multiple of 256) elements of an 8-bit state stand for. */
 int vcb_adamw_values(int64_t n, const void* m, const void* v, const float* m_scale,

@@ -153,7 +153,7 @@ def test_refusals():
             bad()
     lib = _lib.lib()
     p = x.data_ptr()
-    assert lib.vcb_cross_entropy(2, 4, 0, p, 4, y.data_ptr(), -100, p, p, 4, None, 0, None) \
+    assert lib.vcb_cross_entropy(300, 4, 0, p, 4, y.data_ptr(), -100, p, p, 4, None, 0, None) \
         == _lib.VCB_ERR_INVALID
     assert lib.vcb_cross_entropy(2, 4, 0, p, 3, y.data_ptr(), -100, p, p, 4, p, 1 << 20, None) \
         == _lib.VCB_ERR_INVALID

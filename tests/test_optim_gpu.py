@@ -224,7 +224,8 @@ def test_refusals():
     lib = _lib.lib()
     o = _lib.VcbAdamwOpts()
     import ctypes
-    assert lib.vcb_adamw(1, None, 0, 0, 32, None, None, None, None, ctypes.byref(o), None) \
+    none = (None,) * 4
+    assert lib.vcb_adamw(1, *none, 0, 0, 32, None, None, None, None, ctypes.byref(o), None) \
         == _lib.VCB_ERR_INVALID
-    assert lib.vcb_adamw(0, None, 0, 0, 16, None, None, None, None, ctypes.byref(o), None) \
+    assert lib.vcb_adamw(0, *none, 0, 0, 16, None, None, None, None, ctypes.byref(o), None) \
         == _lib.VCB_ERR_INVALID

@@ -140,8 +140,9 @@ SIGNATURES = {
                             _P, _P, ctypes.c_size_t, _P],
     'vcb_linear_backward_workspace': [_I, _I, _I, _I, _I, _I],
     'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
-    'vcb_cross_entropy_workspace': [_I],
-    'vcb_adamw': [_I, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts), _P],
+    'vcb_cross_entropy_workspace': [_I, _I],
+    'vcb_adamw': [_I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts),
+                  _P],
     'vcb_adamw_values': [_L, _P, _P, _P, _P, _P, _P, _P],
     'vcb_bab_step': [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P,
                      _P, _P, _P, _P, _P],
@@ -245,29 +246,13 @@ def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class _Here:
-    """Context manager that does nothing (the tensor's device is current)."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on_device(device):
-    """Makes ``device`` current for a launch on its stream."""
-    if device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
-
-
-def raw_stream(device):
-    """The current stream of ``device`` as an integer handle."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def launch(index, fn, *args):
+    """``fn(*args, stream)`` with CUDA device ``index`` current and its current
+    stream as the last argument."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def require_cuda(t, name='tensor'):

@@ -357,23 +357,31 @@ __global__ void __launch_bounds__(256)
   put4(vo + i, 4, true, {v_value(vc, 0, b), v_value(vc, 2, b)});
 }
 
+// The tensors of a call: arrays of `count`.
+struct Tensors {
+  int count;
+  void* const* p;
+  const void* const* g;
+  const int64_t *n, *off;
+};
+
 template <typename PT, typename GT, int BITS>
-int launch(const vcb_adamw_tensor* t, int count, const State& s, cudaStream_t st) {
+int launch(const Tensors& t, const State& s, cudaStream_t st) {
   const int pb = sizeof(PT), gb = sizeof(GT);
-  for (int a = 0; a < count;) {
+  for (int a = 0; a < t.count;) {
     Table<kLargeTable> tab;
     tab.count = 0;
     long long ctas = 0;
-    for (; a < count && tab.count < kLargeTable; ++a) {
-      if (t[a].n == 0) continue;
-      const long long own = (t[a].n + kChunk - 1) / kChunk;
+    for (; a < t.count && tab.count < kLargeTable; ++a) {
+      if (t.n[a] == 0) continue;
+      const long long own = (t.n[a] + kChunk - 1) / kChunk;
       if (ctas + own > 0x7fffffffLL) {
         if (tab.count == 0) return fail(VCB_ERR_UNSUPPORTED, "vcb_adamw: tensor %d too large", a);
         break;
       }
-      const bool vec = reinterpret_cast<uintptr_t>(t[a].p) % (4 * pb) == 0 &&
-                       reinterpret_cast<uintptr_t>(t[a].g) % (4 * gb) == 0;
-      tab.e[tab.count++] = {t[a].p, t[a].g, t[a].n, t[a].off, static_cast<int>(ctas), vec};
+      const bool vec = reinterpret_cast<uintptr_t>(t.p[a]) % (4 * pb) == 0 &&
+                       reinterpret_cast<uintptr_t>(t.g[a]) % (4 * gb) == 0;
+      tab.e[tab.count++] = {t.p[a], t.g[a], t.n[a], t.off[a], static_cast<int>(ctas), vec};
       ctas += own;
     }
     if (tab.count == 0) break;
@@ -394,14 +402,13 @@ int launch(const vcb_adamw_tensor* t, int count, const State& s, cudaStream_t st
 }
 
 template <int BITS>
-int dispatch(const vcb_adamw_tensor* t, int count, int pt, int gt, const State& s,
-             cudaStream_t st) {
-  if (pt == VCB_F32) return launch<float, float, BITS>(t, count, s, st);
+int dispatch(const Tensors& t, int pt, int gt, const State& s, cudaStream_t st) {
+  if (pt == VCB_F32) return launch<float, float, BITS>(t, s, st);
   if (pt == VCB_BF16)
-    return gt == VCB_F32 ? launch<__nv_bfloat16, float, BITS>(t, count, s, st)
-                         : launch<__nv_bfloat16, __nv_bfloat16, BITS>(t, count, s, st);
-  return gt == VCB_F32 ? launch<__half, float, BITS>(t, count, s, st)
-                       : launch<__half, __half, BITS>(t, count, s, st);
+    return gt == VCB_F32 ? launch<__nv_bfloat16, float, BITS>(t, s, st)
+                         : launch<__nv_bfloat16, __nv_bfloat16, BITS>(t, s, st);
+  return gt == VCB_F32 ? launch<__half, float, BITS>(t, s, st)
+                       : launch<__half, __half, BITS>(t, s, st);
 }
 
 }  // namespace
@@ -409,31 +416,32 @@ int dispatch(const vcb_adamw_tensor* t, int count, int pt, int gt, const State& 
 
 using namespace vcb;
 
-extern "C" int vcb_adamw(int32_t count, const vcb_adamw_tensor* tensors, int32_t p_type,
-                         int32_t g_type, int32_t state_bits, void* m, void* v, float* m_scale,
-                         float* v_scale, const vcb_adamw_opts* opts, void* stream) {
-  if (count < 0 || (count > 0 && !tensors) || !opts || !valid_dtype(p_type) ||
+extern "C" int vcb_adamw(int32_t count, void* const* p, const void* const* g, const int64_t* n,
+                         const int64_t* off, int32_t p_type, int32_t g_type, int32_t state_bits,
+                         void* m, void* v, float* m_scale, float* v_scale,
+                         const vcb_adamw_opts* opts, void* stream) {
+  if (count < 0 || (count > 0 && (!p || !g || !n || !off)) || !opts || !valid_dtype(p_type) ||
       !(g_type == p_type || g_type == VCB_F32) || (state_bits != 8 && state_bits != 32))
     return fail(VCB_ERR_INVALID, "vcb_adamw: count=%d p_type=%d g_type=%d state_bits=%d", count,
                 p_type, g_type, state_bits);
   bool any = false;
   for (int i = 0; i < count; ++i) {
-    const vcb_adamw_tensor& t = tensors[i];
-    if (t.n < 0 || t.off < 0 || t.off % kBlock || (t.n > 0 && (!t.p || !t.g)) ||
-        reinterpret_cast<uintptr_t>(t.p) % dtype_bytes(p_type) ||
-        reinterpret_cast<uintptr_t>(t.g) % dtype_bytes(g_type))
+    if (n[i] < 0 || off[i] < 0 || off[i] % kBlock || (n[i] > 0 && (!p[i] || !g[i])) ||
+        reinterpret_cast<uintptr_t>(p[i]) % dtype_bytes(p_type) ||
+        reinterpret_cast<uintptr_t>(g[i]) % dtype_bytes(g_type))
       return fail(VCB_ERR_INVALID, "vcb_adamw: tensor %d: n=%lld off=%lld", i,
-                  static_cast<long long>(t.n), static_cast<long long>(t.off));
-    any |= t.n > 0;
+                  static_cast<long long>(n[i]), static_cast<long long>(off[i]));
+    any |= n[i] > 0;
   }
   if (!any) return VCB_OK;
   auto off16 = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 != 0; };
   if (!m || !v || off16(m) || off16(v) || (state_bits == 8 && (!m_scale || !v_scale)))
     return fail(VCB_ERR_INVALID, "vcb_adamw: the state must be there and 16-byte aligned");
+  const Tensors t{count, p, g, n, off};
   const State s{m, v, m_scale, v_scale, *opts};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return state_bits == 8 ? dispatch<8>(tensors, count, p_type, g_type, s, st)
-                         : dispatch<32>(tensors, count, p_type, g_type, s, st);
+  return state_bits == 8 ? dispatch<8>(t, p_type, g_type, s, st)
+                         : dispatch<32>(t, p_type, g_type, s, st);
 }
 
 extern "C" int vcb_adamw_values(int64_t n, const void* m, const void* v, const float* m_scale,

@@ -553,12 +553,14 @@ int launch_count(CeArgs& a, cudaStream_t st) {
   return check_launch("vcb_cross_entropy");
 }
 
+// Up to four rows per group of lanes: one CTA and no count before it cost less than
+// a second launch.
+bool single(int R, int C) { return C <= 32 ? R <= 4 * 32 : C <= 128 && R <= 4 * 8; }
+
 template <typename T, int G, int PER>
 int launch_small(CeArgs a, cudaStream_t st) {
   const int rows = 256 / G;
-  // up to four rows per group of lanes: one CTA and no count before it cost less
-  // than a second launch
-  if (a.R <= 4 * rows) {
+  if (single(a.R, a.C)) {
     a.parts = 1, a.counts = 0;
   } else {
     a.parts = static_cast<int>(std::min<long long>((a.R + rows - 1LL) / rows, sm_count() * 16LL));
@@ -637,7 +639,8 @@ int launch(CeArgs a, cudaStream_t st) {
 
 using namespace vcb;
 
-extern "C" size_t vcb_cross_entropy_workspace(int32_t R) {
+extern "C" size_t vcb_cross_entropy_workspace(int32_t R, int32_t C) {
+  if (R <= 0 || single(R, C)) return 0;
   const size_t rows = static_cast<size_t>(std::max(R, 0));
   return kHeader * 4 + (rows / kGroup + 2) / 2 * 8 + rows * sizeof(double);
 }
@@ -655,16 +658,18 @@ extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void*
   if (!logits || !labels || !grad || reinterpret_cast<uintptr_t>(logits) % eb ||
       reinterpret_cast<uintptr_t>(grad) % eb || reinterpret_cast<uintptr_t>(labels) % 8)
     return fail(VCB_ERR_INVALID, "vcb_cross_entropy: NULL or misaligned pointer");
-  if (!workspace || workspace_bytes < vcb_cross_entropy_workspace(R) ||
-      reinterpret_cast<uintptr_t>(workspace) % 16)
+  const size_t need = vcb_cross_entropy_workspace(R, C);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(VCB_ERR_INVALID, "vcb_cross_entropy: workspace of %zu bytes", workspace_bytes);
   CeArgs a{};
   a.R = R, a.C = C, a.ld = ld, a.ldg = ldg, a.ignore = ignore_index;
   a.x = logits, a.g = grad, a.loss = loss;
   a.y = reinterpret_cast<const long long*>(labels);
-  a.header = static_cast<int*>(workspace);
-  a.tickets = a.header + kHeader;
-  a.part = reinterpret_cast<double*>(a.tickets + (R / kGroup + 2) / 2 * 2);
+  if (need) {
+    a.header = static_cast<int*>(workspace);
+    a.tickets = a.header + kHeader;
+    a.part = reinterpret_cast<double*>(a.tickets + (R / kGroup + 2) / 2 * 2);
+  }
   if (type == VCB_F32) return launch<float>(a, st);
   if (type == VCB_BF16) return launch<__nv_bfloat16>(a, st);
   return launch<__half>(a, st);

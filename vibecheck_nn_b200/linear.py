@@ -41,7 +41,7 @@ def type_of(t, name):
 def rows_of(t, cols, like, name):
     """``t`` (..., cols) as rows with unit column stride -> (tensor, row
     stride); copies only what no row stride describes."""
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype != like.dtype or t.get_device() != like.get_device():
         raise ValueError(f'{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}')
     dim = t.dim()
     if dim < 1 or t.shape[-1] != cols:
@@ -73,13 +73,7 @@ def _act(act):
 def _weight(x, weight):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError('weight must be (N, K)')
-    N, K = weight.shape
-    if weight.dtype != x.dtype or weight.device != x.device:
-        raise ValueError(f'weight: {weight.dtype} on {weight.device}, expected {x.dtype} on '
-                         f'{x.device}')
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f'x: shape {tuple(x.shape)}, expected (..., {K})')
-    return N, K
+    return weight.shape
 
 
 def linear_forward(x, weight, bias=None, act='none', residual=None, keep=False):
@@ -107,10 +101,8 @@ def linear_forward(x, weight, bias=None, act='none', residual=None, keep=False):
     nbytes = _workspace_bytes('vcb_linear_forward_workspace', M, N, K, ty,
                               not (xp | wp | ldx * size | ldw * size) & 15)
     ws = _lib.workspace(nbytes, x.device)
-    with _lib.on_device(x.device):
-        rc = _lib.lib().vcb_linear_forward(M, N, K, ty, xp, ldx, wp, ldw, _p(bias), code, _p(r2),
-                                           ldr, y.data_ptr(), N, _p(z), N, _p(ws), nbytes,
-                                           _lib.raw_stream(x.device))
+    rc = _lib.launch(x.get_device(), _lib.lib().vcb_linear_forward, M, N, K, ty, xp, ldx, wp, ldw,
+                     _p(bias), code, _p(r2), ldr, y.data_ptr(), N, _p(z), N, _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_linear_forward')
     if not flat:
@@ -146,10 +138,8 @@ def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, Tr
     nbytes = _workspace_bytes('vcb_linear_backward_workspace', M, N, K, ty, code,
                               not (gp | xp | wp | (ldg | ldx | ldw) * size) & 15)
     ws = _lib.workspace(nbytes, x.device)
-    with _lib.on_device(x.device):
-        rc = _lib.lib().vcb_linear_backward(M, N, K, ty, gp, ldg, xp, ldx, wp, ldw, _p(z2), ldz,
-                                            code, _p(dx), K, _p(dw), K, _p(db), _p(ws), nbytes,
-                                            _lib.raw_stream(x.device))
+    rc = _lib.launch(x.get_device(), _lib.lib().vcb_linear_backward, M, N, K, ty, gp, ldg, xp, ldx,
+                     wp, ldw, _p(z2), ldz, code, _p(dx), K, _p(dw), K, _p(db), _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_linear_backward')
     if dx is not None and x.dim() != 2:
@@ -158,7 +148,7 @@ def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, Tr
 
 
 def _vector(t, n, like, name):
-    if t.dtype != like.dtype or t.device != like.device or t.shape != (n,):
+    if t.dtype != like.dtype or t.get_device() != like.get_device() or t.shape != (n,):
         raise ValueError(f'{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected '
                          f'{like.dtype} ({n},) on {like.device}')
     return t.contiguous()

@@ -14,33 +14,34 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import _workspace_bytes, rows_of, type_of
+from .linear import _p, _workspace_bytes, rows_of, type_of
 
 
 def cross_entropy_grad(logits, labels, ignore_index=-100):
     """(loss, d loss / d logits): loss a float32 scalar on the device, the
     gradient in the logits' type and shape."""
     ty = type_of(logits, 'logits')
-    if logits.dim() < 1 or logits.shape[-1] == 0:
-        raise ValueError(f'logits: shape {tuple(logits.shape)}, expected (..., C) with C > 0')
+    shape = logits.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f'logits: shape {tuple(shape)}, expected (..., C) with C > 0')
+    dev = logits.get_device()
     if not isinstance(labels, torch.Tensor) or labels.dtype != torch.int64 \
-            or labels.device != logits.device or labels.shape != logits.shape[:-1]:
-        raise ValueError(f'labels must be int64 {tuple(logits.shape[:-1])} on {logits.device}')
-    C = logits.shape[-1]
+            or labels.get_device() != dev or labels.shape != shape[:-1]:
+        raise ValueError(f'labels must be int64 {tuple(shape[:-1])} on {logits.device}')
+    C = shape[-1]
     x2, ld = rows_of(logits, C, logits, 'logits')
     labels = labels.contiguous()
     R = x2.shape[0]
     grad = logits.new_empty((R, C))
     loss = logits.new_empty((), dtype=torch.float32)
-    nbytes = _workspace_bytes('vcb_cross_entropy_workspace', R)
+    nbytes = _workspace_bytes('vcb_cross_entropy_workspace', R, C)
     ws = _lib.workspace(nbytes, logits.device)
-    with _lib.on_device(logits.device):
-        rc = _lib.lib().vcb_cross_entropy(R, C, ty, x2.data_ptr(), ld, labels.data_ptr(),
-                                          int(ignore_index), loss.data_ptr(), grad.data_ptr(), C,
-                                          ws.data_ptr(), nbytes, _lib.raw_stream(logits.device))
+    rc = _lib.launch(dev, _lib.lib().vcb_cross_entropy, R, C, ty, x2.data_ptr(), ld,
+                     labels.data_ptr(), int(ignore_index), loss.data_ptr(), grad.data_ptr(), C,
+                     _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_cross_entropy')
-    return loss, grad if logits.dim() == 2 else grad.view(logits.shape)
+    return loss, grad if len(shape) == 2 else grad.view(shape)
 
 
 class _CrossEntropy(torch.autograd.Function):

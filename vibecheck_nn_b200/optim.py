@@ -18,8 +18,8 @@ last place is lost); gradients have the weights' type or float32.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -27,7 +27,6 @@ from .linear import TYPES, type_of
 
 BLOCK = 256
 _MASK32 = 0xFFFFFFFF
-_TABLE = np.dtype([('p', 'u8'), ('g', 'u8'), ('n', 'i8'), ('off', 'i8')])
 
 
 class AdamW:
@@ -46,15 +45,17 @@ class AdamW:
         self.state_bits, self.seed, self.t = state_bits, int(seed), 0
         self.device = self.params[0].device
         self._types = [type_of(p, f'parameter {i}') for i, p in enumerate(self.params)]
+        self._one_type = len(set(self._types)) == 1
         self._shapes = [p.shape for p in self.params]
-        self._table = np.zeros(len(self.params), _TABLE)
-        self.offsets, total = [], 0
+        self._sizes, self.offsets, total = [], [], 0
         for i, p in enumerate(self.params):
             if p.device != self.device or not p.is_contiguous():
                 raise ValueError(f'parameter {i}: must be contiguous on {self.device}')
             self.offsets.append(total)
-            self._table[i] = (0, 0, p.numel(), total)
+            self._sizes.append(p.numel())
             total += -(-p.numel() // BLOCK) * BLOCK
+        self._all = range(len(self.params))
+        self._arrays = array('q', self._sizes), array('q', self.offsets)
         new = lambda n, dt: torch.zeros(n, dtype=dt, device=self.device)  # noqa: E731
         if state_bits == 32:
             self.m, self.v = new(total, torch.float32), new(total, torch.float32)
@@ -83,22 +84,35 @@ class AdamW:
         opts = self._opts()
         m, v = self.m.data_ptr(), self.v.data_ptr()
         ms, vs = _p(self.m_scale), _p(self.v_scale)
-        with _lib.on_device(self.device):
-            L, st = _lib.lib(), _lib.raw_stream(self.device)
-            for pt, gt, idx, gp in groups:
-                tab = self._table if len(gp) == len(ps) else self._table[idx]
-                tab['p'] = [ps[i].data_ptr() for i in idx]
-                tab['g'] = gp
-                rc = L.vcb_adamw(len(gp), tab.ctypes.data, pt, gt, self.state_bits, m, v, ms, vs,
-                                 ctypes.byref(opts), st)
-                if rc:
-                    _lib.check(rc, 'vcb_adamw')
+        step = _lib.lib().vcb_adamw
+        for pt, gt, idx, gp in groups:
+            if idx is self._all:
+                pp, (sizes, offsets) = array('Q', [p.data_ptr() for p in ps]), self._arrays
+            else:
+                pp = array('Q', [ps[i].data_ptr() for i in idx])
+                sizes = array('q', [self._sizes[i] for i in idx])
+                offsets = array('q', [self.offsets[i] for i in idx])
+            gp = array('Q', gp)
+            rc = _lib.launch(self.device.index, step, len(gp), pp.buffer_info()[0],
+                             gp.buffer_info()[0], sizes.buffer_info()[0],
+                             offsets.buffer_info()[0], pt, gt, self.state_bits, m, v, ms, vs,
+                             ctypes.byref(opts))
+            if rc:
+                _lib.check(rc, 'vcb_adamw')
         torch.autograd.graph.increment_version(ps)
 
     def _groups(self, grads):
         """[(weights' type, gradients' type, indices, gradient pointers)], one
         entry per launch."""
         here = self.device.index
+        if not any([g is None for g in grads]):  # usually one type, and nothing to copy
+            first = grads[0].dtype
+            if self._one_type and (first == torch.float32 or first == self.params[0].dtype) \
+                    and [g.shape for g in grads] == self._shapes \
+                    and all([g.dtype is first and g.get_device() == here and g.is_contiguous()
+                             for g in grads]):
+                return [(self._types[0], TYPES[first], self._all,
+                         [g.data_ptr() for g in grads])]
         groups = {}
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if g is None:
@@ -127,11 +141,9 @@ class AdamW:
         n = self.m.numel()
         m = torch.empty(n, dtype=torch.float32, device=self.device)
         v = torch.empty(n, dtype=torch.float32, device=self.device)
-        with _lib.on_device(self.device):
-            rc = _lib.lib().vcb_adamw_values(n, self.m.data_ptr(), self.v.data_ptr(),
-                                             self.m_scale.data_ptr(), self.v_scale.data_ptr(),
-                                             m.data_ptr(), v.data_ptr(),
-                                             _lib.raw_stream(self.device))
+        rc = _lib.launch(self.device.index, _lib.lib().vcb_adamw_values, n, self.m.data_ptr(),
+                         self.v.data_ptr(), self.m_scale.data_ptr(), self.v_scale.data_ptr(),
+                         m.data_ptr(), v.data_ptr())
         _lib.check(rc, 'vcb_adamw_values')
         return m, v
 
