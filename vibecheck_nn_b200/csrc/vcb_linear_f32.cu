@@ -26,6 +26,7 @@
 // with the contraction cut over a cluster for the rest.
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 #include "vcb_linear_tc.cuh"
 
@@ -154,12 +155,12 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJo
 }
 
 // ---- preparation, backward ----
-// A matrix in strips of 128 columns (a warp per row, 4 columns per lane); with z
-// the entries are dz = dy act'(z).
+// A matrix in strips of columns, 4 columns per lane; with z the entries are dz = dy
+// act'(z).
 struct ColJob {
   const float *src, *z;
   long long ld, ldz, rows;
-  int cols, vec, act, strips;
+  int cols, vec, act;
   uint32_t *col_most, *row_most;  // row_most may be NULL; zero on entry
   float* sum;                     // column sums, or NULL
   __half *by_col, *by_row;        // halves with column scales; with row scales, or NULL
@@ -182,39 +183,46 @@ __device__ __forceinline__ void job4(const ColJob& q, long long r, int c, float 
   for (int k = 0; k < 4; ++k) v[k] = act_grad(v[k], t[k], q.act);
 }
 
-// The job and strip of cluster s.
-__device__ __forceinline__ const ColJob& strip_of(const ColJobs& a, int& s) {
+// The job and strip (of `width` columns) of strip s of a launch.
+__device__ __forceinline__ const ColJob& strip_of(const ColJobs& a, int& s, int width = 32) {
   int k = 0;
-  while (k + 1 < a.count && s >= a.j[k].strips) s -= a.j[k++].strips;
+  while (k + 1 < a.count) {
+    const int strips = (a.j[k].cols + width - 1) / width;
+    if (s < strips) break;
+    s -= strips;
+    ++k;
+  }
   return a.j[k];
 }
 
-// Largest entries of every column (a cluster of 8 CTAs per strip, an eighth of the
-// rows each) and of every row (atomic maxima: any order gives the same), column
-// sums in the order of the ranks.
-__global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripThreads)
+// Largest entries of every column (a cluster of 8 CTAs per strip of 32 columns, an
+// eighth of the rows each, 8 lanes per row) and of every row (atomic maxima: any
+// order gives the same), column sums in the order of the ranks.
+__global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripThreads, 4)
     scales_kernel(const __grid_constant__ ColJobs a) {
-  __shared__ float part[kStripWarps][128], sum_mine[128];
-  __shared__ uint32_t most_part[kStripWarps][128], most_mine[128];
+  __shared__ float part[kStripWarps][32], sum_mine[32];
+  __shared__ uint32_t most_part[kStripWarps][32], most_mine[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % kStripCluster;
   int strip = blockIdx.x / kStripCluster;
   const ColJob& q = strip_of(a, strip);
-  const int c = strip * 128 + lane * 4;
+  const int c = strip * 32 + (lane & 7) * 4;
   const long long r0 = q.rows * rank / kStripCluster, r1 = q.rows * (rank + 1) / kStripCluster;
   float sum[4] = {};
   uint32_t most[4] = {};
-  constexpr int U = 4;
-  for (long long r = r0 + warp; r < r1; r += U * kStripWarps) {
+  constexpr int U = 4, W = kStripWarps * 4;  // rows in flight per lane, rows of a CTA's step
+  for (long long base = r0 + warp * 4; base < r1; base += U * W) {
     float v[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const long long r = base + u * W + (lane >> 3);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
-      if (r + u * kStripWarps < r1) job4(q, r + u * kStripWarps, c, v[u]);
+      if (r < r1) job4(q, r, c, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const long long r = base + u * W + (lane >> 3);
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -223,18 +231,26 @@ __global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripTh
         m = more(m, v[u][i]);
       }
       if (q.row_most) {
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0 && r + u * kStripWarps < r1) atomicMax(q.row_most + r + u * kStripWarps, m);
+#pragma unroll
+        for (int k = 4; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
+        if ((lane & 7) == 0 && r < r1) atomicMax(q.row_most + r, m);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    part[warp][lane * 4 + i] = sum[i];
-    most_part[warp][lane * 4 + i] = most[i];
+#pragma unroll
+    for (int k = 8; k < 32; k *= 2) {
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
+      most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], k));
+    }
+    if (lane < 8) {
+      part[warp][lane * 4 + i] = sum[i];
+      most_part[warp][lane * 4 + i] = most[i];
+    }
   }
   __syncthreads();
-  if (threadIdx.x < 128) {
+  if (threadIdx.x < 32) {
     float s = 0.f;
     uint32_t m = 0;
     for (int w = 0; w < kStripWarps; ++w) {
@@ -245,8 +261,8 @@ __global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripTh
     most_mine[threadIdx.x] = m;
   }
   cluster_sync();
-  const int col = strip * 128 + threadIdx.x;
-  if (rank == 0 && threadIdx.x < 128 && col < q.cols) {
+  const int col = strip * 32 + threadIdx.x;
+  if (rank == 0 && threadIdx.x < 32 && col < q.cols) {
     float s = 0.f;
     uint32_t m = 0;
     for (int k = 0; k < kStripCluster; ++k) {
@@ -259,12 +275,12 @@ __global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripTh
   cluster_sync();  // no CTA leaves while its figures are read
 }
 
-constexpr int kHalvesRows = 64;  // rows of a CTA
+constexpr int kHalvesRows = 32;  // rows of a CTA
 
 __global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_constant__ ColJobs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int strip = blockIdx.x;
-  const ColJob& q = strip_of(a, strip);
+  const ColJob& q = strip_of(a, strip, 128);
   const int c = strip * 128 + lane * 4;
   if (c >= q.cols) return;
   float scale[4];
@@ -354,8 +370,8 @@ __device__ __forceinline__ void load_halves(uint32_t dst, const CUtensorMap* map
 }
 
 // One tile of `out` per unit of work.  PAIR: persistent CTA pairs, 256 x 256.
-// Otherwise a 128 x BN tile of the first product per cluster of L.split CTAs, each
-// with a part of the contraction; the parts are joined in the order of the ranks.
+// Otherwise a 128 x BN tile per cluster of L.split CTAs, each with a part of the
+// contraction (none, where it has fewer stages than CTAs); the parts are joined in the order of the ranks.
 template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_constant__ Launch32 L) {
   using C = Cfg<BN, PAIR>;
@@ -564,9 +580,9 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
   if (PAIR || size > 1) cluster_sync();
   if (!PAIR && size > 1) {
     if (warp < kEpi) {
-      const Prod32& p = L.p[0];
+      const Prod32& p = L.p[first >= L.units0];
       int ti, tj;
-      tile_at(p.tiles_i, p.tiles_j, first, ti, tj);
+      tile_at(p.tiles_i, p.tiles_j, first >= L.units0 ? first - L.units0 : first, ti, tj);
       const Epilogue e = p.epi;
       const int i0 = ti * BN, j = tj * kTileJ + lane * 4;
       const int columns = min(BN, p.I - i0);
@@ -659,14 +675,23 @@ struct Plan32 {
 // As the 16-bit products' plan: rounds of tiles over the SMs times the stages'
 // cycles (12 MMAs: 1,536 for a pair's tile, 768 for 64 or 128 columns), plus start
 // and epilogue.
-Plan32 plan_of(int I, int J, int T) {
+struct Shape {
+  int I, J, T;
+};
+
+Plan32 plan_of(std::initializer_list<Shape> products) {
   const int sms = sm_count();
   const auto ceil = [](long long a, long long b) { return (a + b - 1) / b; };
-  const long long nk = std::max<long long>(1, ceil(T, kBK));
+  long long nk = 1, pairs = 0;
+  for (const Shape& s : products) {
+    nk = std::max(nk, ceil(s.T, kBK));
+    pairs += ceil(s.I, 256) * ceil(s.J, 256);
+  }
   Plan32 best{true, 256, 1};
-  double least = static_cast<double>(ceil(ceil(I, 256) * ceil(J, 256), sms / 2)) * (nk * 1540 + 4000) + 4000;
+  double least = static_cast<double>(ceil(pairs, sms / 2)) * (nk * 1540 + 4000) + 4000;
   for (int bn : {64, 128}) {
-    const long long tiles = ceil(I, bn) * ceil(J, kTileJ);
+    long long tiles = 0;
+    for (const Shape& s : products) tiles += ceil(s.I, bn) * ceil(s.J, kTileJ);
     for (int split : {1, 2, 4, 8}) {
       if (split > nk) break;
       const double t = static_cast<double>(ceil(tiles * split, sms)) *
@@ -763,7 +788,7 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
     rows_kernel<256><<<static_cast<unsigned>(rows), 256, 0, st>>>(jobs);
   int rc = check_launch(who);
   if (rc) return rc;
-  const Plan32 plan = plan_of(f.M, f.N, f.K);
+  const Plan32 plan = plan_of({{f.M, f.N, f.K}});
   Launch32 L{};
   rc = set_prod(L.p[0], f.M, f.N, f.K, w, x, plan,
                 {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0}, who);
@@ -792,14 +817,14 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   const Halves w = make_halves(arena, b.N, b.K, true, arena.take<uint32_t>(b.K * 4LL));
   const Halves x = make_halves(arena, b.M, b.K, true, arena.take<uint32_t>(b.K * 4LL));
   ColJobs jobs{};
-  long long strips = 0, tall = 0;
+  long long strips = 0, wide = 0, tall = 0;
   const auto add = [&](const void* p, long long ld, const Halves& h) -> ColJob& {
     ColJob& q = jobs.j[jobs.count++];
     q.src = static_cast<const float*>(p);
     q.ld = ld, q.rows = h.rows, q.cols = h.cols, q.vec = vec16(p, ld);
-    q.strips = (h.cols + 127) / 128;
     q.col_most = h.most, q.by_col = h.p, q.ldh = h.ld, q.plane = h.plane;
-    strips += q.strips;
+    strips += (h.cols + 31) / 32;
+    wide += (h.cols + 127) / 128;
     tall = std::max(tall, q.rows);
     return q;
   };
@@ -819,33 +844,33 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   scales_kernel<<<static_cast<unsigned>(strips * kStripCluster), kStripThreads, 0, st>>>(jobs);
   int rc = check_launch(who);
   if (rc) return rc;
-  halves_kernel<<<dim3(static_cast<unsigned>(strips),
+  halves_kernel<<<dim3(static_cast<unsigned>(wide),
                        static_cast<unsigned>((tall + kHalvesRows - 1) / kHalvesRows)),
                   kStripThreads, 0, st>>>(jobs);
   rc = check_launch(who);
   if (rc) return rc;
-  const Plan32 px = plan_of(b.M, b.K, b.N), pw = plan_of(b.N, b.K, b.M);
-  const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
-  const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+  // both products in one launch
+  const Shape shape_x{b.M, b.K, b.N}, shape_w{b.N, b.K, b.M};
+  const Plan32 plan = b.dx && b.dw ? plan_of({shape_x, shape_w})
+                      : b.dx       ? plan_of({shape_x})
+                                   : plan_of({shape_w});
   Launch32 L{};
+  L.split = plan.split;
   if (b.dx) {
-    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, px, ex, who);
+    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, plan,
+                  {b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0}, who);
     if (rc) return rc;
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
-    L.split = px.split;
-    if (!(b.dw && px.pair && pw.pair)) {  // two pairs share a launch
-      rc = launch_plan(L, px, st, who);
-      if (rc || !b.dw) return rc;
-      L.units0 = L.units = 0;
-    }
   }
-  Prod32& p = L.p[L.units ? 1 : 0];
-  rc = set_prod(p, b.N, b.K, b.M, x, dzc, pw, ew, who);
-  if (rc) return rc;
-  L.units += p.tiles_i * p.tiles_j;
-  if (!L.units0) L.units0 = L.units;
-  L.split = pw.split;
-  return launch_plan(L, pw, st, who);
+  if (b.dw) {
+    Prod32& p = L.p[b.dx ? 1 : 0];
+    rc = set_prod(p, b.N, b.K, b.M, x, dzc, plan,
+                  {b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0}, who);
+    if (rc) return rc;
+    L.units += p.tiles_i * p.tiles_j;
+    if (!b.dx) L.units0 = L.units;
+  }
+  return launch_plan(L, plan, st, who);
 }
 
 int f32_fault_take(cudaStream_t st, int* was_set) {
