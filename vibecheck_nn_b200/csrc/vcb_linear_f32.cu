@@ -170,9 +170,10 @@ struct ColJob {
 struct ColJobs {
   ColJob j[3];
   int count;
+  int cluster;  // CTAs per strip of scales_kernel
 };
 
-constexpr int kStripCluster = 8, kStripThreads = 256, kStripWarps = kStripThreads / 32;
+constexpr int kStripThreads = 256, kStripWarps = kStripThreads / 32;
 
 __device__ __forceinline__ void job4(const ColJob& q, long long r, int c, float (&v)[4]) {
   row4(q.src + r * q.ld, c, q.cols, q.vec, v);
@@ -195,19 +196,19 @@ __device__ __forceinline__ const ColJob& strip_of(const ColJobs& a, int& s, int 
   return a.j[k];
 }
 
-// Largest entries of every column (a cluster of 8 CTAs per strip of 32 columns, an
-// eighth of the rows each, 8 lanes per row) and of every row (atomic maxima: any
+// Largest entries of every column (a cluster of up to 8 CTAs per strip of 32 columns,
+// a part of the rows each, 8 lanes per row) and of every row (atomic maxima: any
 // order gives the same), column sums in the order of the ranks.
-__global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripThreads, 4)
+__global__ void __launch_bounds__(kStripThreads, 4)
     scales_kernel(const __grid_constant__ ColJobs a) {
   __shared__ float part[kStripWarps][32], sum_mine[32];
   __shared__ uint32_t most_part[kStripWarps][32], most_mine[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % kStripCluster;
-  int strip = blockIdx.x / kStripCluster;
+  const int size = a.cluster, rank = blockIdx.x % size;
+  int strip = blockIdx.x / size;
   const ColJob& q = strip_of(a, strip);
   const int c = strip * 32 + (lane & 7) * 4;
-  const long long r0 = q.rows * rank / kStripCluster, r1 = q.rows * (rank + 1) / kStripCluster;
+  const long long r0 = q.rows * rank / size, r1 = q.rows * (rank + 1) / size;
   float sum[4] = {};
   uint32_t most[4] = {};
   constexpr int U = 4, W = kStripWarps * 4;  // rows in flight per lane, rows of a CTA's step
@@ -265,7 +266,7 @@ __global__ void __cluster_dims__(kStripCluster, 1, 1) __launch_bounds__(kStripTh
   if (rank == 0 && threadIdx.x < 32 && col < q.cols) {
     float s = 0.f;
     uint32_t m = 0;
-    for (int k = 0; k < kStripCluster; ++k) {
+    for (int k = 0; k < size; ++k) {
       s += peer_f32(map_rank(smem_u32(sum_mine + threadIdx.x), k));
       m = max(m, __float_as_uint(peer_f32(map_rank(smem_u32(most_mine + threadIdx.x), k))));
     }
@@ -670,6 +671,7 @@ int make_map(CUtensorMap* map, const Halves& h, int box_rows, const char* who) {
 struct Plan32 {
   bool pair;
   int bn, split;
+  double cycles;
 };
 
 // As the 16-bit products' plan: rounds of tiles over the SMs times the stages'
@@ -687,8 +689,7 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
     nk = std::max(nk, ceil(s.T, kBK));
     pairs += ceil(s.I, 256) * ceil(s.J, 256);
   }
-  Plan32 best{true, 256, 1};
-  double least = static_cast<double>(ceil(pairs, sms / 2)) * (nk * 1540 + 4000) + 4000;
+  Plan32 best{true, 256, 1, static_cast<double>(ceil(pairs, sms / 2)) * (nk * 1540 + 4000) + 4000};
   for (int bn : {64, 128}) {
     long long tiles = 0;
     for (const Shape& s : products) tiles += ceil(s.I, bn) * ceil(s.J, kTileJ);
@@ -697,7 +698,7 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
       const double t = static_cast<double>(ceil(tiles * split, sms)) *
                            (ceil(nk, split) * (bn == 64 ? 800 : 1000) + 4000 + 20.0 * bn) +
                        (split > 1 ? 1500 + 8.0 * bn : 0);
-      if (t < least) least = t, best = {false, bn, split};
+      if (t < best.cycles) best = {false, bn, split, t};
     }
   }
   return best;
@@ -836,12 +837,25 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (!b.dw) dz.by_col = nullptr;
   if (b.dx) add(b.w, b.ldw, w);
   if (b.dw) add(b.x, b.ldx, x);
-  if (strips * kStripCluster > 0x7fffffffLL || (tall + kHalvesRows - 1) / kHalvesRows > 65535)
+  if (strips * 8 > 0x7fffffffLL || (tall + kHalvesRows - 1) / kHalvesRows > 65535)
     return fail(VCB_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d", who, b.M, b.N, b.K);
   cudaError_t e = cudaSuccess;
   if (b.dx) e = cudaMemsetAsync(row_most, 0, b.M * 4LL, st);
   if (e != cudaSuccess) return cuda_fail(e, who);
-  scales_kernel<<<static_cast<unsigned>(strips * kStripCluster), kStripThreads, 0, st>>>(jobs);
+  jobs.cluster = 1;  // a CTA's step is 128 rows
+  while (jobs.cluster < 8 && tall > 128 * jobs.cluster) jobs.cluster *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(strips * jobs.cluster));
+  cfg.blockDim = dim3(kStripThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = jobs.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, scales_kernel, jobs);
+  if (e != cudaSuccess) return cuda_fail(e, who);
   int rc = check_launch(who);
   if (rc) return rc;
   halves_kernel<<<dim3(static_cast<unsigned>(wide),
@@ -849,28 +863,34 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
                   kStripThreads, 0, st>>>(jobs);
   rc = check_launch(who);
   if (rc) return rc;
-  // both products in one launch
+  const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
+  const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
   const Shape shape_x{b.M, b.K, b.N}, shape_w{b.N, b.K, b.M};
-  const Plan32 plan = b.dx && b.dw ? plan_of({shape_x, shape_w})
-                      : b.dx       ? plan_of({shape_x})
-                                   : plan_of({shape_w});
+  Plan32 px = plan_of({shape_x}), pw = plan_of({shape_w});
+  const Plan32 both = plan_of({shape_x, shape_w});
+  // One launch for both products unless their shapes want different cuts by more than
+  // a launch costs.
+  const bool together = b.dx && b.dw && both.cycles < px.cycles + pw.cycles + 4000;
+  if (together) px = pw = both;
   Launch32 L{};
-  L.split = plan.split;
   if (b.dx) {
-    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, plan,
-                  {b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0}, who);
+    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, px, ex, who);
     if (rc) return rc;
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
+    L.split = px.split;
+    if (!together) {
+      rc = launch_plan(L, px, st, who);
+      if (rc || !b.dw) return rc;
+      L.units0 = L.units = 0;
+    }
   }
-  if (b.dw) {
-    Prod32& p = L.p[b.dx ? 1 : 0];
-    rc = set_prod(p, b.N, b.K, b.M, x, dzc, plan,
-                  {b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0}, who);
-    if (rc) return rc;
-    L.units += p.tiles_i * p.tiles_j;
-    if (!b.dx) L.units0 = L.units;
-  }
-  return launch_plan(L, plan, st, who);
+  Prod32& p = L.p[together ? 1 : 0];
+  rc = set_prod(p, b.N, b.K, b.M, x, dzc, pw, ew, who);
+  if (rc) return rc;
+  L.units += p.tiles_i * p.tiles_j;
+  if (!together) L.units0 = L.units;
+  L.split = pw.split;
+  return launch_plan(L, pw, st, who);
 }
 
 int f32_fault_take(cudaStream_t st, int* was_set) {

@@ -436,9 +436,10 @@ struct Prep {
   long long lddy, ldz, lddz;
   Copy copy[2];
   int copies;
+  int cluster;  // CTAs per strip
 };
 
-constexpr int kPrepCluster = 8, kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
+constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
 constexpr int kStrip = 32;  // columns
 
 // Four elements at p, `align` bytes aligned (8, 4 or 2); 0 from `left` on.
@@ -465,20 +466,20 @@ __device__ __forceinline__ int rows_align(const void* p, long long ld) {
   return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
 }
 
-// A cluster of 8 CTAs per strip of 32 columns: each sums its eighth of the rows (8
-// lanes per row, 4 columns per lane), rank 0 adds the eight sums in order.  Bound by
+// A cluster of up to 8 CTAs per strip of 32 columns: each sums its part of the rows
+// (8 lanes per row, 4 columns per lane), rank 0 adds the sums in order.  Bound by
 // HBM: dy and z are read and dz is written once; strips are narrow so that a matrix
 // of 2,000 columns keeps every SM reading.  The remaining CTAs copy.
 template <typename T>
-__global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThreads, 5)
+__global__ void __launch_bounds__(kPrepThreads, 5)
     prep_kernel(const __grid_constant__ Prep a) {
   __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int strip = blockIdx.x / kPrepCluster;
+  const int size = a.cluster, strip = blockIdx.x / size;
   if (strip < a.strips) {
-    const int rank = blockIdx.x % kPrepCluster, c = strip * kStrip + (lane & 7) * 4;
-    const long long r0 = static_cast<long long>(a.M) * rank / kPrepCluster;
-    const long long r1 = static_cast<long long>(a.M) * (rank + 1) / kPrepCluster;
+    const int rank = blockIdx.x % size, c = strip * kStrip + (lane & 7) * 4;
+    const long long r0 = static_cast<long long>(a.M) * rank / size;
+    const long long r1 = static_cast<long long>(a.M) * (rank + 1) / size;
     const T *dy = static_cast<const T*>(a.dy) + c, *z = static_cast<const T*>(a.z) + c;
     const int ay = rows_align(a.dy, a.lddy), az = rows_align(a.z, a.ldz), left = a.N - c;
     float sum[4] = {};
@@ -525,15 +526,15 @@ __global__ void __cluster_dims__(kPrepCluster, 1, 1) __launch_bounds__(kPrepThre
     if (a.db && rank == 0 && threadIdx.x < kStrip) {
       const int col = strip * kStrip + threadIdx.x;
       float v = 0.f;
-      for (int k = 0; k < kPrepCluster; ++k) v += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
+      for (int k = 0; k < size; ++k) v += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
       if (col < a.N) static_cast<T*>(a.db)[col] = from_f32<T>(v);
     }
     cluster_sync();  // no CTA leaves while its sums are read
     return;
   }
   // copies: a warp per row, eight elements per lane, written as one 16-byte vector
-  const int first = (blockIdx.x - a.strips * kPrepCluster) * kPrepWarps + warp;
-  const int step = (gridDim.x - a.strips * kPrepCluster) * kPrepWarps;
+  const int first = (blockIdx.x - a.strips * size) * kPrepWarps + warp;
+  const int step = (gridDim.x - a.strips * size) * kPrepWarps;
   for (int k = 0; k < a.copies; ++k) {
     const Copy& q = a.copy[k];
     for (long long row = first; row < q.rows; row += step) {
@@ -731,17 +732,27 @@ Operand readable(const void* p, long long ld, int rows, int cols, bool mn, Prep&
   return {c.dst, c.ldd, mn};
 }
 
-int launch_prep(const Prep& a, int type, cudaStream_t st, const char* who) {
+int launch_prep(Prep& a, int type, cudaStream_t st, const char* who) {
   long long rows = 0;
   for (int k = 0; k < a.copies; ++k) rows = std::max(rows, a.copy[k].rows);
   const long long ctas = std::min<long long>((rows + kPrepWarps - 1) / kPrepWarps, 5LL * sm_count());
-  const long long grid =
-      (a.strips + (ctas + kPrepCluster - 1) / kPrepCluster) * (long long)kPrepCluster;
+  a.cluster = 1;  // a CTA's step is 64 rows
+  while (a.strips && a.cluster < 8 && a.M > 64 * a.cluster) a.cluster *= 2;
+  const long long grid = (a.strips + (ctas + a.cluster - 1) / a.cluster) * (long long)a.cluster;
   if (grid == 0) return VCB_OK;
-  if (type == VCB_BF16)
-    prep_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), kPrepThreads, 0, st>>>(a);
-  else
-    prep_kernel<__half><<<static_cast<unsigned>(grid), kPrepThreads, 0, st>>>(a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kPrepThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const auto kernel = type == VCB_BF16 ? prep_kernel<__nv_bfloat16> : prep_kernel<__half>;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) return cuda_fail(e, who);
   return check_launch(who);
 }
 
@@ -799,11 +810,13 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (b.dw) x = readable(b.x, b.ldx, b.M, b.K, true, prep, arena);
   int rc = launch_prep(prep, b.type, st, who);
   if (rc) return rc;
-  // dX and dW share a launch when both are pairs; otherwise each is cut its own way
+  // dX and dW share a launch when both are pairs or both are not; the contraction of
+  // dW, the rows, is then not cut
   const Plan px = plan_of(b.M, b.K, b.N, true, false), pw = plan_of(b.N, b.K, b.M, true, true);
   Launch L{};
   Operand dzt = dz;
   dzt.mn = true;
+  const bool together = b.dx && b.dw && px.pair == pw.pair;
   if (b.dx) {
     rc = set_prod(L.p[0], b.type, b.M, b.K, b.N, w, dz, px.bn, px.pair, who);
     if (rc) return rc;
@@ -811,7 +824,6 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
     L.p[0].epi.vec = vector_rows(L.p[0].epi, 2);
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
   }
-  const bool together = b.dx && b.dw && px.pair == pw.pair;
   if (b.dx && !together) {
     rc = launch_type(L, px, b.type, st, who);
     if (rc) return rc;
