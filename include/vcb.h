@@ -715,6 +715,13 @@ int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, in
                       int64_t ldg, void* workspace, size_t workspace_bytes, void* stream);
 size_t vcb_cross_entropy_workspace(int32_t R, int32_t C);
 
+/* vcb_linear_forward, vcb_linear_backward and vcb_cross_entropy with their
+ * arguments, in order, as consecutive 64-bit integers (sizes, pointers, the
+ * stream): for bindings that pay for every argument they convert. */
+int vcb_linear_forward_packed(const int64_t* args);
+int vcb_linear_backward_packed(const int64_t* args);
+int vcb_cross_entropy_packed(const int64_t* args);
+
 /* One AdamW step over `count` tensors: tensor i has n[i] weights at p[i] and
  * gradients at g[i], and its moments are the elements [off[i], off[i] + n[i]) of
  * the state, off[i] a multiple of 256.  state_bits 32: m and v are fp32 and the

@@ -27,7 +27,7 @@ def reference(layers, x, y):
             h = torch.relu(h)
     value = torch.nn.functional.cross_entropy(h, y.cpu())
     value.backward()
-    return float(value), [p.grad for p in ps[::2]] + [p.grad for p in ps[1::2]]
+    return float(value.detach()), [p.grad for p in ps[::2]] + [p.grad for p in ps[1::2]]
 
 
 @pytest.mark.parametrize('rows', [1, 33, 700])

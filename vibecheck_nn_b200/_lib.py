@@ -141,6 +141,9 @@ SIGNATURES = {
     'vcb_linear_backward_workspace': [_I, _I, _I, _I, _I, _I],
     'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
     'vcb_cross_entropy_workspace': [_I, _I],
+    'vcb_linear_forward_packed': [ctypes.c_char_p],
+    'vcb_linear_backward_packed': [ctypes.c_char_p],
+    'vcb_cross_entropy_packed': [ctypes.c_char_p],
     'vcb_adamw': [_I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts),
                   _P],
     'vcb_adamw_values': [_L, _P, _P, _P, _P, _P, _P, _P],
@@ -253,6 +256,16 @@ def launch(index, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def launch_packed(index, fn, pack, *args):
+    """As ``launch`` for an entry point that takes its arguments packed
+    (``pack``, a ``struct.Struct.pack``): a fifth of the cost of twenty converted
+    one by one."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
+    with torch.cuda.device(index):
+        return fn(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def require_cuda(t, name='tensor'):

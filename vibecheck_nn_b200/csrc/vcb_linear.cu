@@ -393,3 +393,33 @@ extern "C" int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type
   return (f32 ? lin::f32_backward : lin::tc_backward)(b, workspace,
                                                       static_cast<cudaStream_t>(stream));
 }
+
+// Pointers of a packed argument list.
+template <typename T = void>
+static T* at(int64_t v) {
+  return reinterpret_cast<T*>(static_cast<uintptr_t>(v));
+}
+
+extern "C" int vcb_linear_forward_packed(const int64_t* a) {
+  if (!a) return fail(VCB_ERR_INVALID, "vcb_linear_forward_packed: NULL");
+  const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
+  return vcb_linear_forward(i(0), i(1), i(2), i(3), at(a[4]), a[5], at(a[6]), a[7], at(a[8]), i(9),
+                            at(a[10]), a[11], at(a[12]), a[13], at(a[14]), a[15], at(a[16]),
+                            static_cast<size_t>(a[17]), at(a[18]));
+}
+
+extern "C" int vcb_linear_backward_packed(const int64_t* a) {
+  if (!a) return fail(VCB_ERR_INVALID, "vcb_linear_backward_packed: NULL");
+  const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
+  return vcb_linear_backward(i(0), i(1), i(2), i(3), at(a[4]), a[5], at(a[6]), a[7], at(a[8]), a[9],
+                             at(a[10]), a[11], i(12), at(a[13]), a[14], at(a[15]), a[16],
+                             at(a[17]), at(a[18]), static_cast<size_t>(a[19]), at(a[20]));
+}
+
+extern "C" int vcb_cross_entropy_packed(const int64_t* a) {
+  if (!a) return fail(VCB_ERR_INVALID, "vcb_cross_entropy_packed: NULL");
+  const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
+  return vcb_cross_entropy(i(0), i(1), i(2), at(a[3]), a[4], at<const int64_t>(a[5]), a[6],
+                           at<float>(a[7]), at(a[8]), a[9], at(a[10]), static_cast<size_t>(a[11]),
+                           at(a[12]));
+}

@@ -18,12 +18,15 @@ can ask ``_lib.fault_check`` whether a bounded device wait ran out.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
 from . import _lib
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# argument lists of the packed entry points
+_FORWARD, _BACKWARD = struct.Struct('19q').pack, struct.Struct('21q').pack
 ACTS = {'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3}
 
 
@@ -101,8 +104,9 @@ def linear_forward(x, weight, bias=None, act='none', residual=None, keep=False):
     nbytes = _workspace_bytes('vcb_linear_forward_workspace', M, N, K, ty,
                               not (xp | wp | ldx * size | ldw * size) & 15)
     ws = _lib.workspace(nbytes, x.device)
-    rc = _lib.launch(x.get_device(), _lib.lib().vcb_linear_forward, M, N, K, ty, xp, ldx, wp, ldw,
-                     _p(bias), code, _p(r2), ldr, y.data_ptr(), N, _p(z), N, _p(ws), nbytes)
+    rc = _lib.launch_packed(x.get_device(), _lib.lib().vcb_linear_forward_packed, _FORWARD,
+                            M, N, K, ty, xp, ldx, wp, ldw, _p(bias), code, _p(r2), ldr,
+                            y.data_ptr(), N, _p(z), N, _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_linear_forward')
     if not flat:
@@ -138,8 +142,9 @@ def linear_backward(dy, x, weight, z=None, act='none', bias=True, need=(True, Tr
     nbytes = _workspace_bytes('vcb_linear_backward_workspace', M, N, K, ty, code,
                               not (gp | xp | wp | (ldg | ldx | ldw) * size) & 15)
     ws = _lib.workspace(nbytes, x.device)
-    rc = _lib.launch(x.get_device(), _lib.lib().vcb_linear_backward, M, N, K, ty, gp, ldg, xp, ldx,
-                     wp, ldw, _p(z2), ldz, code, _p(dx), K, _p(dw), K, _p(db), _p(ws), nbytes)
+    rc = _lib.launch_packed(x.get_device(), _lib.lib().vcb_linear_backward_packed, _BACKWARD,
+                            M, N, K, ty, gp, ldg, xp, ldx, wp, ldw, _p(z2), ldz, code, _p(dx), K,
+                            _p(dw), K, _p(db), _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_linear_backward')
     if dx is not None and x.dim() != 2:
@@ -155,7 +160,7 @@ def _vector(t, n, like, name):
 
 
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 class _Linear(torch.autograd.Function):

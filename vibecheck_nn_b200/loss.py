@@ -11,10 +11,14 @@ labelled row the loss is 0.  A row whose logits are all ``-inf`` has loss
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
 from .linear import _p, _workspace_bytes, rows_of, type_of
+
+_ARGS = struct.Struct('13q').pack
 
 
 def cross_entropy_grad(logits, labels, ignore_index=-100):
@@ -36,9 +40,9 @@ def cross_entropy_grad(logits, labels, ignore_index=-100):
     loss = logits.new_empty((), dtype=torch.float32)
     nbytes = _workspace_bytes('vcb_cross_entropy_workspace', R, C)
     ws = _lib.workspace(nbytes, logits.device)
-    rc = _lib.launch(dev, _lib.lib().vcb_cross_entropy, R, C, ty, x2.data_ptr(), ld,
-                     labels.data_ptr(), int(ignore_index), loss.data_ptr(), grad.data_ptr(), C,
-                     _p(ws), nbytes)
+    rc = _lib.launch_packed(dev, _lib.lib().vcb_cross_entropy_packed, _ARGS, R, C, ty,
+                            x2.data_ptr(), ld, labels.data_ptr(), int(ignore_index),
+                            loss.data_ptr(), grad.data_ptr(), C, _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_cross_entropy')
     return loss, grad if len(shape) == 2 else grad.view(shape)
