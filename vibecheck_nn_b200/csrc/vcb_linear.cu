@@ -180,8 +180,10 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
     const int i = i0 + e / kTJ, j = j0 + e % kTJ;
     if (!s.epi.out || i >= s.I || j >= s.J) return;
     float one[1] = {value};
+    ColumnResidual<T, 1> res;
+    res.fetch(s.epi, s.I, s.J, i, j);
     emit_column<T, 1>(s.epi, s.I, s.J, i, j,
-                      s.epi.bias ? to_f32(static_cast<const T*>(s.epi.bias)[j]) : 0.f, one);
+                      s.epi.bias ? to_f32(static_cast<const T*>(s.epi.bias)[j]) : 0.f, one, res);
   };
   if (size == 1) {
 #pragma unroll

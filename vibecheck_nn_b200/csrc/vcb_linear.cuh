@@ -167,18 +167,26 @@ __device__ __forceinline__ void emit(const Epilogue& e, int I, int J, int i, int
   put(e.out, e.ldo);
 }
 
+// Residuals of N consecutive rows from i of column j.
+template <typename T, int N>
+struct ColumnResidual {
+  T v[N];
+  __device__ __forceinline__ void fetch(const Epilogue& e, int I, int J, int i, int j) {
+    if (!e.res || j >= J) return;
+    const T* at = static_cast<const T*>(e.res) + i * e.ldr + j;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (i + c < I) v[c] = __ldcs(at + c * e.ldr);
+  }
+};
+
 // N consecutive rows from i of column j.
 template <typename T, int N>
 __device__ __forceinline__ void emit_column(const Epilogue& e, int I, int J, int i, int j,
-                                            float bias, float (&v)[N]) {
+                                            float bias, float (&v)[N],
+                                            const ColumnResidual<T, N>& res) {
   const int n = min(N, I - i);
   if (j >= J || n <= 0) return;
-  float r[N];
-  if (e.res) {
-    const T* at = static_cast<const T*>(e.res) + i * e.ldr + j;
-#pragma unroll
-    for (int c = 0; c < N; ++c) r[c] = c < n ? to_f32(__ldcs(at + c * e.ldr)) : 0.f;
-  }
 #pragma unroll
   for (int c = 0; c < N; ++c) v[c] += bias;
   if (e.z) {
@@ -196,7 +204,7 @@ __device__ __forceinline__ void emit_column(const Epilogue& e, int I, int J, int
   T* at = static_cast<T*>(e.out) + i * e.ldo + j;
 #pragma unroll
   for (int c = 0; c < N; ++c)
-    if (c < n) __stcs(at + c * e.ldo, from_f32<T>(e.res ? v[c] + r[c] : v[c]));
+    if (c < n) __stcs(at + c * e.ldo, from_f32<T>(e.res ? v[c] + to_f32(res.v[c]) : v[c]));
 }
 
 struct Fwd {

@@ -107,7 +107,10 @@ __global__ void __launch_bounds__(kRowThreads) rows_forward_kernel(const __grid_
 #pragma unroll
   for (int k = 0; k < kRowWarps; ++k) v[0] += part[k][t];
   const Epilogue e{f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
-  emit_column<T, 1>(e, f.M, f.N, m, n, f.bias ? to_f32(static_cast<const T*>(f.bias)[n]) : 0.f, v);
+  ColumnResidual<T, 1> res;
+  res.fetch(e, f.M, f.N, m, n);
+  emit_column<T, 1>(e, f.M, f.N, m, n, f.bias ? to_f32(static_cast<const T*>(f.bias)[n]) : 0.f, v,
+                    res);
 }
 
 struct RowsBwd {

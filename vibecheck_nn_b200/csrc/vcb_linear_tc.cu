@@ -106,12 +106,23 @@ struct TileEpilogue {
 // The same where rows take no vectors: a lane keeps its column, so a warp's stores
 // and loads are 32 neighbouring elements.
 template <typename T>
-__device__ __forceinline__ void column_epilogue(const Prod& p, uint32_t acc, int warp, int lane,
-                                                int j0, int i0, bool ok) {
-  const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-  const int j = j0 + (warp & 3) * 32 + lane, bn = p.bn, I = p.I;
-  const float bias = p.epi.bias && j < p.J ? to_f32(static_cast<const T*>(p.epi.bias)[j]) : 0.f;
-  for (int c = (warp >> 2) * 16; c < bn && i0 + c < I; c += 32) {
+struct ColumnEpilogue {
+  const Epilogue& e;
+  int I, J, bn, i0, j, first;
+  float bias;
+  ColumnResidual<T, 16> res;
+
+  __device__ __forceinline__ ColumnEpilogue(const Prod& p, int warp, int lane, int j0, int i0_)
+      : e(p.epi), I(p.I), J(p.J), bn(p.bn), i0(i0_), j(j0 + (warp & 3) * 32 + lane),
+        first((warp >> 2) * 16) {
+    bias = e.bias && j < J ? to_f32(static_cast<const T*>(e.bias)[j]) : 0.f;
+    fetch(first);
+  }
+  __device__ __forceinline__ void fetch(int c) {
+    if (c < bn) res.fetch(e, I, J, i0 + c, j);
+  }
+  __device__ __forceinline__ void chunk(uint32_t at, int c, bool ok) {
+    if (c >= bn || i0 + c >= I) return;  // warp-uniform
     uint32_t raw[16];
     if (ok) {
       tmem_ld16(at + c, raw);
@@ -120,9 +131,14 @@ __device__ __forceinline__ void column_epilogue(const Prod& p, uint32_t acc, int
     float v[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
-    emit_column<T, 16>(p.epi, I, p.J, i0 + c, j, bias, v);
+    emit_column<T, 16>(e, I, J, i0 + c, j, bias, v, res);
+    fetch(c + 32);
   }
-}
+  __device__ __forceinline__ void run(uint32_t acc, int warp, bool ok) {
+    const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int c = first; c < bn; c += 32) chunk(at, c, ok);
+  }
+};
 
 constexpr int kPairStages = 6;
 constexpr int kPairStage = 2 * kBytesA;  // per CTA: 128 rows of A and 128 of B
@@ -250,8 +266,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ready();
         epilogue.run(tmem + q * 256, warp, ok);
       } else {
+        ColumnEpilogue<T> epilogue(p, warp, lane, j0, i0);
         ready();
-        column_epilogue<T>(p, tmem + q * 256, warp, lane, j0, i0, ok);
+        epilogue.run(tmem + q * 256, warp, ok);
       }
       fence_before_sync();
       __syncwarp();
@@ -368,8 +385,9 @@ __global__ void __launch_bounds__(kThreads)
       fence_after_sync();
     };
     if (parts == 1 && !p.epi.vec) {
+      ColumnEpilogue<T> epilogue(p, warp, lane, j0, idle ? p.I : i0);
       ready();
-      if (!idle) column_epilogue<T>(p, tmem, warp, lane, j0, i0, ok);
+      epilogue.run(tmem, warp, ok);
     } else if (parts == 1) {
       TileEpilogue<T> epilogue(p, warp, lane, j0, idle ? p.I : i0);
       ready();
@@ -466,6 +484,24 @@ __device__ __forceinline__ int rows_align(const void* p, long long ld) {
   return bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
 }
 
+// Eight elements at p, 2-byte aligned; 0 from `left` on.
+__device__ __forceinline__ uint4 eight_at(const uint16_t* p, int left) {
+  if (left < 8) {
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < left) w[i / 2] |= static_cast<uint32_t>(p[i]) << 16 * (i % 2);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const bool odd = reinterpret_cast<uintptr_t>(p) % 4 != 0;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p + odd);
+  const uint32_t w0 = __ldcs(w), w1 = __ldcs(w + 1), w2 = __ldcs(w + 2);
+  if (!odd) return make_uint4(w0, w1, w2, __ldcs(w + 3));
+  // the six elements between the first and the last as aligned words
+  const uint32_t a0 = p[0], a7 = p[7];
+  return make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16, w2 >> 16 | a7 << 16);
+}
+
 // A cluster of up to 8 CTAs per strip of 32 columns: each sums its part of the rows
 // (8 lanes per row, 4 columns per lane), rank 0 adds the sums in order.  Bound by
 // HBM: dy and z are read and dz is written once; strips are narrow so that a matrix
@@ -532,35 +568,31 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
     cluster_sync();  // no CTA leaves while its sums are read
     return;
   }
-  // copies: a warp per row, eight elements per lane, written as one 16-byte vector
-  const int first = (blockIdx.x - a.strips * size) * kPrepWarps + warp;
-  const int step = (gridDim.x - a.strips * size) * kPrepWarps;
+  // copies: eight elements per thread, written as one 16-byte vector; neighbouring
+  // threads take neighbouring vectors of all rows, four of them in flight
+  const long long first = (long long)(blockIdx.x - a.strips * size) * kPrepThreads + threadIdx.x;
+  const long long step = (long long)(gridDim.x - a.strips * size) * kPrepThreads;
   for (int k = 0; k < a.copies; ++k) {
     const Copy& q = a.copy[k];
-    for (long long row = first; row < q.rows; row += step) {
-      const uint16_t* in = static_cast<const uint16_t*>(q.src) + row * q.lds;
-      uint16_t* out = static_cast<uint16_t*>(q.dst) + row * q.ldd;
-      const bool odd = reinterpret_cast<uintptr_t>(in) % 4 != 0;
-#pragma unroll 4
-      for (int c = lane * 8; c < q.cols; c += 256) {
-        const uint16_t* src = in + c;
-        uint4 o;
-        if (c + 8 > q.cols) {
-          __align__(16) uint16_t e[8];
+    const int nv = (q.cols + 7) / 8;
+    long long row = first / nv;
+    int v = static_cast<int>(first - row * nv);
+    const long long down = step / nv;
+    const int right = static_cast<int>(step - down * nv);
+    constexpr int U = 4;
+    while (row < q.rows) {
+      uint4 o[U];
+      uint16_t* out[U];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = c + i < q.cols ? src[i] : 0;
-          o = *reinterpret_cast<const uint4*>(e);
-        } else if (!odd) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
-          o = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {  // the six elements between the first and the last as aligned words
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(src + 1);
-          const uint32_t a0 = src[0], w0 = w[0], w1 = w[1], w2 = w[2], a7 = src[7];
-          o = make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16,
-                         w2 >> 16 | a7 << 16);
-        }
-        *reinterpret_cast<uint4*>(out + c) = o;
+      for (int u = 0; u < U; ++u) {
+        out[u] = row < q.rows ? static_cast<uint16_t*>(q.dst) + row * q.ldd + v * 8 : nullptr;
+        if (out[u]) o[u] = eight_at(static_cast<const uint16_t*>(q.src) + row * q.lds + v * 8, q.cols - v * 8);
+        row += down, v += right;
+        if (v >= nv) v -= nv, ++row;
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (out[u]) *reinterpret_cast<uint4*>(out[u]) = o[u];
     }
   }
 }
@@ -733,9 +765,11 @@ Operand readable(const void* p, long long ld, int rows, int cols, bool mn, Prep&
 }
 
 int launch_prep(Prep& a, int type, cudaStream_t st, const char* who) {
-  long long rows = 0;
-  for (int k = 0; k < a.copies; ++k) rows = std::max(rows, a.copy[k].rows);
-  const long long ctas = std::min<long long>((rows + kPrepWarps - 1) / kPrepWarps, 5LL * sm_count());
+  long long vectors = 0;
+  for (int k = 0; k < a.copies; ++k)
+    vectors = std::max(vectors, a.copy[k].rows * ((a.copy[k].cols + 7LL) / 8));
+  const long long ctas =
+      std::min<long long>((vectors + kPrepThreads - 1) / kPrepThreads, 4LL * sm_count());
   a.cluster = 1;  // a CTA's step is 64 rows
   while (a.strips && a.cluster < 8 && a.M > 64 * a.cluster) a.cluster *= 2;
   const long long grid = (a.strips + (ctas + a.cluster - 1) / a.cluster) * (long long)a.cluster;
