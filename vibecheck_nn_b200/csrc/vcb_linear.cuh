@@ -75,10 +75,11 @@ __device__ __forceinline__ void bias_at(const Epilogue& e, int J, int j, float (
 
 // v[c] of lane l: column c of row l.  Afterwards v[4 q + k] is column 4 q + l % 4
 // of row (l - l % 4) + k: four lanes have traded 4 x 4 blocks.
-__device__ __forceinline__ void transpose16(float (&v)[16], int lane) {
+template <int N>
+__device__ __forceinline__ void transpose4(float (&v)[N], int lane) {
   const bool odd = lane & 1, high = lane & 2;
 #pragma unroll
-  for (int q = 0; q < 16; q += 4) {
+  for (int q = 0; q < N; q += 4) {
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
       const float got = __shfl_xor_sync(0xffffffffu, odd ? v[q + k] : v[q + k + 1], 1);

@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
 #pragma unroll
           for (int k = 0; k < 16; ++k)
             v[k] = scaled(acc[c + k], ea + __shfl_sync(0xffffffffu, eb, k));
-          transpose16(v, lane);
+          transpose4(v, lane);
           emit<float, 4>(p.epi, I, J, i0 + c + (lane & 3), j, bias, v, res);
         }
       }

@@ -58,94 +58,99 @@ struct Launch {
   int stages;
 };
 
-// Epilogue of one warp: lanes 32 (warp % 4).. of the accumulator at `acc`, every
-// other chunk of 16 columns (warp / 4).  Residuals are fetched two chunks ahead.
-// `ok` false: NaN instead.
-template <typename T>
+// W columns of the accumulator, NaN if !ok.
+template <int W>
+__device__ __forceinline__ void accumulator(uint32_t at, bool ok, float (&v)[W]) {
+  uint32_t raw[W];
+  if (ok) {
+    if constexpr (W == 16) tmem_ld16(at, raw); else tmem_ld8(at, raw);
+    tmem_wait_ld(raw);
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
+}
+
+// Epilogue of one of WARPS warps: lanes 32 (warp % 4).. of the accumulator at `acc`,
+// chunk warp / 4 of W columns and every (WARPS / 4)th from there.  Residuals are
+// fetched two chunks ahead.  `ok` false: NaN instead.
+template <typename T, int W, int WARPS>
 struct TileEpilogue {
+  static constexpr int kStep = WARPS / 4 * W;
   const Epilogue& e;
   int I, J, bn, i0, lane, j, first;
-  Residual<T, 4> res[2];
+  Residual<T, W / 4> res[2];
 
   __device__ __forceinline__ TileEpilogue(const Prod& p, int warp, int lane_, int j0, int i0_)
       : e(p.epi), I(p.I), J(p.J), bn(p.bn), i0(i0_), lane(lane_),
-        j(j0 + (warp & 3) * 32 + (lane_ & ~3)), first((warp >> 2) * 16) {
+        j(j0 + (warp & 3) * 32 + (lane_ & ~3)), first((warp >> 2) * W) {
     // before the accumulator is ready
     fetch(res[0], first);
-    fetch(res[1], first + 32);
+    fetch(res[1], first + kStep);
   }
-  __device__ __forceinline__ void fetch(Residual<T, 4>& r, int c) {
+  __device__ __forceinline__ void fetch(Residual<T, W / 4>& r, int c) {
     if (c < bn) r.fetch(e, I, J, i0 + c + (lane & 3), j);
   }
   __device__ __forceinline__ void chunk(uint32_t at, int c, const float (&bias)[4],
-                                        Residual<T, 4>& r, bool ok) {
+                                        Residual<T, W / 4>& r, bool ok) {
     if (c >= bn || i0 + c >= I) return;  // warp-uniform
-    uint32_t raw[16];
-    if (ok) {
-      tmem_ld16(at + c, raw);
-      tmem_wait_ld(raw);
-    }
-    float v[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
-    transpose16(v, lane);
-    emit<T, 4>(e, I, J, i0 + c + (lane & 3), j, bias, v, r);
-    fetch(r, c + 64);
+    float v[W];
+    accumulator(at + c, ok, v);
+    transpose4(v, lane);
+    emit<T, W / 4>(e, I, J, i0 + c + (lane & 3), j, bias, v, r);
+    fetch(r, c + 2 * kStep);
   }
   __device__ __forceinline__ void run(uint32_t acc, int warp, bool ok) {
     float bias[4];
     bias_at<T>(e, J, j, bias);
     const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-    for (int c = first; c < bn; c += 64) {
+    for (int c = first; c < bn; c += 2 * kStep) {
       chunk(at, c, bias, res[0], ok);
-      chunk(at, c + 32, bias, res[1], ok);
+      chunk(at, c + kStep, bias, res[1], ok);
     }
   }
 };
 
 // The same where rows take no vectors: a lane keeps its column, so a warp's stores
-// and loads are 32 neighbouring elements.
-template <typename T>
+// and loads are 32 neighbouring elements.  Residuals one chunk ahead: registers for
+// two would be spilled.
+template <typename T, int W, int WARPS>
 struct ColumnEpilogue {
+  static constexpr int kStep = WARPS / 4 * W;
   const Epilogue& e;
   int I, J, bn, i0, j, first;
   float bias;
-  ColumnResidual<T, 16> res;
+  ColumnResidual<T, W> res;
 
   __device__ __forceinline__ ColumnEpilogue(const Prod& p, int warp, int lane, int j0, int i0_)
       : e(p.epi), I(p.I), J(p.J), bn(p.bn), i0(i0_), j(j0 + (warp & 3) * 32 + lane),
-        first((warp >> 2) * 16) {
+        first((warp >> 2) * W) {
     bias = e.bias && j < J ? to_f32(static_cast<const T*>(e.bias)[j]) : 0.f;
     fetch(first);
   }
   __device__ __forceinline__ void fetch(int c) {
     if (c < bn) res.fetch(e, I, J, i0 + c, j);
   }
-  __device__ __forceinline__ void chunk(uint32_t at, int c, bool ok) {
-    if (c >= bn || i0 + c >= I) return;  // warp-uniform
-    uint32_t raw[16];
-    if (ok) {
-      tmem_ld16(at + c, raw);
-      tmem_wait_ld(raw);
-    }
-    float v[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = ok ? __uint_as_float(raw[k]) : NAN;
-    emit_column<T, 16>(e, I, J, i0 + c, j, bias, v, res);
-    fetch(c + 32);
-  }
   __device__ __forceinline__ void run(uint32_t acc, int warp, bool ok) {
     const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
-    for (int c = first; c < bn; c += 32) chunk(at, c, ok);
+    for (int c = first; c < bn && i0 + c < I; c += kStep) {
+      float v[W];
+      accumulator(at + c, ok, v);
+      emit_column<T, W>(e, I, J, i0 + c, j, bias, v, res);
+      fetch(c + kStep);
+    }
   }
 };
 
+// Sixteen epilogue warps with 8 columns at a time: an epilogue warp waits for tensor
+// memory, shuffles and conversions in turn, so a short contraction leaves the
+// epilogue as the bound.
+constexpr int kPairEpi = 16, kPairThreads = (kPairEpi + 2) * 32;
 constexpr int kPairStages = 6;
 constexpr int kPairStage = 2 * kBytesA;  // per CTA: 128 rows of A and 128 of B
 constexpr int kPairSmem = kPairStages * kPairStage + 1024;
 
 template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ Launch L) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -164,7 +169,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&acc_full[q], 1);
-      mbar_init(&acc_free[q], 2 * kEpiWarps);
+      mbar_init(&acc_free[q], 2 * kPairEpi);
     }
     mbar_init(&done, 1);
     failed = 0;
@@ -182,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
-  if (warp == kEpiWarps) {
+  if (warp == kPairEpi) {
     {  // TMA producer: this CTA's halves of A and B, counted by the leader
       const bool one = elect_one();
       unsigned g = 0;
@@ -214,7 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (unsigned k = g > kPairStages ? g - kPairStages : 0; k < g; ++k)
           if (!mbar_wait(&full[k % kPairStages], (k / kPairStages) & 1, kSpinLimit)) failed = 1;
     }
-  } else if (warp == kEpiWarps + 1) {
+  } else if (warp == kPairEpi + 1) {
     if (rank == 0) {  // MMA issuer of the pair
       const bool one = elect_one();
       unsigned t = 0;
@@ -262,11 +267,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         fence_after_sync();
       };
       if (p.epi.vec) {
-        TileEpilogue<T> epilogue(p, warp, lane, j0, i0);
+        TileEpilogue<T, 8, kPairEpi> epilogue(p, warp, lane, j0, i0);
         ready();
         epilogue.run(tmem + q * 256, warp, ok);
       } else {
-        ColumnEpilogue<T> epilogue(p, warp, lane, j0, i0);
+        ColumnEpilogue<T, 8, kPairEpi> epilogue(p, warp, lane, j0, i0);
         ready();
         epilogue.run(tmem + q * 256, warp, ok);
       }
@@ -385,11 +390,11 @@ __global__ void __launch_bounds__(kThreads)
       fence_after_sync();
     };
     if (parts == 1 && !p.epi.vec) {
-      ColumnEpilogue<T> epilogue(p, warp, lane, j0, idle ? p.I : i0);
+      ColumnEpilogue<T, 16, kEpiWarps> epilogue(p, warp, lane, j0, idle ? p.I : i0);
       ready();
       epilogue.run(tmem, warp, ok);
     } else if (parts == 1) {
-      TileEpilogue<T> epilogue(p, warp, lane, j0, idle ? p.I : i0);
+      TileEpilogue<T, 16, kEpiWarps> epilogue(p, warp, lane, j0, idle ? p.I : i0);
       ready();
       epilogue.run(tmem, warp, ok);
     } else {
@@ -684,7 +689,7 @@ int launch_tc(Launch& L, const Plan& plan, cudaStream_t st, const char* who) {
     const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), kPairSmem);
     if (rc) return rc;
     const int grid = 2 * std::min(L.units, sm_count() / 2);
-    kernel<<<grid, kThreads, kPairSmem, st>>>(L);
+    kernel<<<grid, kPairThreads, kPairSmem, st>>>(L);
     return check_launch(who);
   }
   const auto kernel = split_kernel<T>;

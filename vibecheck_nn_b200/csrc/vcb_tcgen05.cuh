@@ -183,6 +183,10 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 
 // Completes the loads of this thread; the register operands tie later uses
 // of the loaded values to the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : VCB_RW8(r)::"memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : VCB_RW16(r)::"memory");
 }
