@@ -39,45 +39,59 @@ struct Small {
   void* sum;         // row sums of A (db), or NULL
   Epilogue epi;      // out may be NULL
   int tiles_j, tiles;
+  int parts;         // CTAs per tile, each with a part of the contraction; a power of 2
+  int clusters;
 };
 
 struct SmallPair {
   Small p[2];
-  int split;  // CTAs (a cluster) per tile
+  int size;  // of a cluster: the larger number of parts
 };
 
-// Entries t .. t + 3 of a row: `step` elements apart, `left` of them exist.
+// Entries t .. t + 3 of a row: `step` elements apart, `left` of them exist.  Kept as
+// loaded until they are used: a conversion would wait for them, and loads follow.
 template <typename T>
-__device__ __forceinline__ void quad(const T* p, long long step, bool vec, int left,
-                                     float (&v)[4]) {
-  if (vec && left >= 4) {
-    load4(p, v);
-  } else {
+struct Quad {
+  T e[4];
+  __device__ __forceinline__ void load(const T* p, long long step, bool vec, int left) {
+    using V = decltype(Four<T>::raw);
+    if (vec && left >= 4) {
+      *reinterpret_cast<V*>(e) = *reinterpret_cast<const V*>(p);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = k < left ? to_f32(p[k * step]) : 0.f;
+      for (int k = 0; k < 4; ++k) e[k] = k < left ? p[k * step] : from_f32<T>(0.f);
+    }
   }
-}
+  __device__ __forceinline__ void values(float (&v)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = to_f32(e[k]);
+  }
+};
 
 __device__ __forceinline__ int chunk_at(int row, int chunk) {
   return row * kTT + ((chunk ^ (row & 7)) << 2);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_constant__ SmallPair pair) {
+// CTAS per SM: three have fewer registers and shorter loops each.
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kSmallThreads, CTAS)
+    small_kernel(const __grid_constant__ SmallPair pair) {
   // operands of a step; then the groups' sums; then this CTA's sum of the tile
   __shared__ __align__(16) float buf[(kTI + kTJ) * kTT > kGroups * kTile ? (kTI + kTJ) * kTT
                                                                         : kGroups * kTile];
   __shared__ float row_sum[kTT / 4][kTI], row_mine[kTI];
   float *sa = buf, *sb = buf + kTI * kTT;
-  const int size = pair.split, lg = 31 - __clz(size);
-  const int rank = blockIdx.x & (size - 1), unit = blockIdx.x >> lg;
-  const int second = unit >= pair.p[0].tiles;
+  const int cluster = blockIdx.x / pair.size, rank = blockIdx.x % pair.size;
+  const int second = cluster >= pair.p[0].clusters;
   const Small& s = pair.p[second];
-  const int tile = unit - (second ? pair.p[0].tiles : 0);
+  const int parts = s.parts, lg = 31 - __clz(parts), part = rank & (parts - 1);
+  // a cluster of more CTAs than parts holds several tiles; the last may hold none,
+  // whose rows lie beyond I
+  const int tile = (cluster - (second ? pair.p[0].clusters : 0)) * (pair.size >> lg) + (rank >> lg);
   const int i0 = tile / s.tiles_j * kTI, j0 = tile % s.tiles_j * kTJ;
   const int tid = threadIdx.x, group = tid >> 6, in = tid & 63, ty = in >> 3, tx = in & 7;
   const int steps = (s.T + kTT - 1) / kTT;
-  const int s0 = steps * rank >> lg, s1 = steps * (rank + 1) >> lg;
+  const int s0 = steps * part >> lg, s1 = i0 < s.I ? steps * (part + 1) >> lg : s0;
   // this thread's two quads of A and of B: lanes run along the contiguous index
   const auto row_of = [&](int contiguous_t, int q) {
     return contiguous_t ? (tid >> 4) + 16 * q : tid & 31;
@@ -95,22 +109,19 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
     pa2[q] = static_cast<const T*>(s.a2) + (s.a_t ? ra * s.lda2 : ra) + ca * ta2;
     pb[q] = static_cast<const T*>(s.b) + (s.b_t ? rb * s.ldb : rb) + cb * tb;
   }
-  float fa[2][4], fb[2][4];
+  Quad<T> qa[2], qz[2], qb[2];
   const auto fetch = [&](int step) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int la = i0 + row_of(s.a_t, q) < s.I ? s.T - (step * 16 + chunk_of(s.a_t, q)) * 4 : 0;
-      quad(pa[q], ta, s.va, la, fa[q]);
+      qa[q].load(pa[q], ta, s.va, la);
       pa[q] += kTT * ta;
       if (s.a2) {
-        float z[4];
-        quad(pa2[q], ta2, s.va, la, z);
+        qz[q].load(pa2[q], ta2, s.va, la);
         pa2[q] += kTT * ta2;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) fa[q][k] = act_grad(fa[q][k], z[k], s.act);
       }
-      quad(pb[q], tb, s.vb,
-           j0 + row_of(s.b_t, q) < s.J ? s.T - (step * 16 + chunk_of(s.b_t, q)) * 4 : 0, fb[q]);
+      qb[q].load(pb[q], tb, s.vb,
+                 j0 + row_of(s.b_t, q) < s.J ? s.T - (step * 16 + chunk_of(s.b_t, q)) * 4 : 0);
       pb[q] += kTT * tb;
     }
   };
@@ -121,10 +132,18 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
+      float v[4];
+      qa[q].values(v);
+      if (s.a2) {
+        float z[4];
+        qz[q].values(z);
+        act_grads(v, z, s.act);
+      }
       *reinterpret_cast<float4*>(sa + chunk_at(row_of(s.a_t, q), chunk_of(s.a_t, q))) =
-          make_float4(fa[q][0], fa[q][1], fa[q][2], fa[q][3]);
+          make_float4(v[0], v[1], v[2], v[3]);
+      qb[q].values(v);
       *reinterpret_cast<float4*>(sb + chunk_at(row_of(s.b_t, q), chunk_of(s.b_t, q))) =
-          make_float4(fb[q][0], fb[q][1], fb[q][2], fb[q][3]);
+          make_float4(v[0], v[1], v[2], v[3]);
     }
     __syncthreads();
     if (step + 1 < s1) fetch(step + 1);
@@ -136,7 +155,7 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
         rs += (v.x + v.y) + (v.z + v.w);
       }
     }
-#pragma unroll 2
+#pragma unroll (CTAS == 2 ? 2 : 1)
     for (int c = group * 4; c < group * 4 + 4; ++c) {
       // rows 8 apart share their place in the XOR
       const float* at_a = sa + ty * kTT + ((c ^ ty) << 2);
@@ -185,11 +204,11 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
     emit_column<T, 1>(s.epi, s.I, s.J, i, j,
                       s.epi.bias ? to_f32(static_cast<const T*>(s.epi.bias)[j]) : 0.f, one, res);
   };
-  if (size == 1) {
+  if (parts == 1) {
 #pragma unroll
     for (int k = 0; k < kEntries; ++k) put(tid + k * kSmallThreads, v[k]);
   } else {
-    // the CTAs of the cluster, in order; each finishes its share of the tile
+    // the parts in order; each CTA finishes its share of the tile
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEntries; ++k) buf[tid + k * kSmallThreads] = v[k];
@@ -197,18 +216,20 @@ __global__ void __launch_bounds__(kSmallThreads, 3) small_kernel(const __grid_co
     cluster_sync();
     const int share = kTile >> lg;
     for (int k = tid; k < share; k += kSmallThreads) {
-      const int e = rank * share + k;
+      const int e = part * share + k;
       float sum = 0.f;
-      for (int g = 0; g < size; ++g) sum += peer_f32(map_rank(smem_u32(buf + e), g));
+      for (int g = 0; g < parts; ++g)
+        sum += peer_f32(map_rank(smem_u32(buf + e), rank - part + g));
       put(e, sum);
     }
-    if (sums && rank == 0 && tid < kTI) {
+    if (sums && part == 0 && tid < kTI) {
       db = 0.f;
-      for (int g = 0; g < size; ++g) db += peer_f32(map_rank(smem_u32(row_mine + tid), g));
+      for (int g = 0; g < parts; ++g)
+        db += peer_f32(map_rank(smem_u32(row_mine + tid), rank + g));
     }
     cluster_sync();  // no CTA leaves while its sums are read
   }
-  if (sums && rank == 0 && tid < kTI && i0 + tid < s.I)
+  if (sums && part == 0 && tid < kTI && i0 + tid < s.I)
     static_cast<T*>(s.sum)[i0 + tid] = from_f32<T>(db);
 }
 
@@ -227,29 +248,48 @@ bool vectors(const void* p, long long ld, int type) {
 }
 
 int launch_small(SmallPair& pair, int type, cudaStream_t st, const char* who) {
-  int steps = 1;
   for (Small& s : pair.p) {
     if (s.tiles < 0) return fail(VCB_ERR_UNSUPPORTED, "%s: too many output tiles", who);
     s.va = s.a_t && vectors(s.a, s.lda, type) && (!s.a2 || vectors(s.a2, s.lda2, type));
     s.vb = s.b_t && vectors(s.b, s.ldb, type);
-    if (s.tiles) steps = std::max(steps, (s.T + kTT - 1) / kTT);
+    s.parts = 1;
   }
-  const int tiles = pair.p[0].tiles + pair.p[1].tiles;
-  if (tiles == 0) return VCB_OK;
-  // a cluster per tile while four CTAs per SM hold all of them and each has a step
-  pair.split = 1;
-  while (pair.split < 8 && 2 * pair.split <= steps && 2LL * pair.split * tiles <= 4LL * sm_count())
-    pair.split *= 2;
-  const auto kernel = type == VCB_F32    ? small_kernel<float>
-                      : type == VCB_BF16 ? small_kernel<__nv_bfloat16>
-                                         : small_kernel<__half>;
+  if (pair.p[0].tiles + pair.p[1].tiles == 0) return VCB_OK;
+  // The product whose CTAs have the most steps of the contraction is cut in two, again
+  // and again, while those steps are more than an even share of all steps over the
+  // SMs' two CTAs each: until then the longest CTA is what is waited for.
+  const auto steps = [](const Small& s) {
+    return s.tiles ? (s.T + kTT - 1) / kTT / s.parts : 0;
+  };
+  const long long work = static_cast<long long>(pair.p[0].tiles) * steps(pair.p[0]) +
+                         static_cast<long long>(pair.p[1].tiles) * steps(pair.p[1]);
+  for (;;) {
+    Small& s = pair.p[steps(pair.p[1]) > steps(pair.p[0])];
+    if (s.parts == 8 || steps(s) < 2 || 2LL * sm_count() * steps(s) <= work) break;
+    s.parts *= 2;
+  }
+  pair.size = std::max(pair.p[0].parts, pair.p[1].parts);
+  long long clusters = 0;
+  for (Small& s : pair.p) {
+    const int per = pair.size / s.parts;
+    clusters += s.clusters = (s.tiles + per - 1) / per;
+  }
+  // Three CTAs per SM where that holds all of them at once and two do not (fp32 100 x
+  // 256 x 784 backward 16.4 us against 18.9), two otherwise (bf16 2000 x 64 x 64
+  // backward 20.5 against 22.5).
+  const long long ctas = clusters * pair.size;
+  const bool three = ctas > 2 * sm_count() && ctas <= 3 * sm_count();
+  const auto kernel = type == VCB_F32 ? three ? small_kernel<float, 3> : small_kernel<float, 2>
+                      : type == VCB_BF16
+                          ? three ? small_kernel<__nv_bfloat16, 3> : small_kernel<__nv_bfloat16, 2>
+                          : three ? small_kernel<__half, 3> : small_kernel<__half, 2>;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * pair.split));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSmallThreads);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = pair.split;
+  at[0].val.clusterDim.x = pair.size;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;

@@ -43,6 +43,23 @@ __device__ __forceinline__ float act_grad(float dy, float z, int act) {
   return dy * act_slope(z, act);
 }
 
+// The same for many values, the choice of act outside of their loop.
+template <int ACT, int N>
+__device__ __forceinline__ void act_grad_all(float (&dy)[N], const float (&z)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) dy[k] = act_grad(dy[k], z[k], ACT);
+}
+
+template <int N>
+__device__ __forceinline__ void act_grads(float (&dy)[N], const float (&z)[N], int act) {
+  switch (act) {
+    case VCB_ACT_RELU: act_grad_all<VCB_ACT_RELU>(dy, z); break;
+    case VCB_ACT_GELU: act_grad_all<VCB_ACT_GELU>(dy, z); break;
+    case VCB_ACT_SILU: act_grad_all<VCB_ACT_SILU>(dy, z); break;
+    default: break;
+  }
+}
+
 // Where a product's rows go and what is done to them on the way.
 struct Epilogue {
   void *out, *z;

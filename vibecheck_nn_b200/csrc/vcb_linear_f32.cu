@@ -175,13 +175,24 @@ struct ColJobs {
 
 constexpr int kStripThreads = 256, kStripWarps = kStripThreads / 32;
 
-__device__ __forceinline__ void job4(const ColJob& q, long long r, int c, float (&v)[4]) {
-  row4(q.src + r * q.ld, c, q.cols, q.vec, v);
-  if (q.act == VCB_ACT_NONE) return;
-  float t[4];
-  row4(q.z + r * q.ldz, c, q.cols, q.vec, t);
+// Entries of N rows from r, `step` rows apart; 0 from row `end` on.  All loads come
+// before the first use.
+template <int N>
+__device__ __forceinline__ void job_rows(const ColJob& q, long long r, long long step,
+                                         long long end, int c, float (&v)[N][4]) {
+  float t[N][4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = act_grad(v[k], t[k], q.act);
+  for (int u = 0; u < N; ++u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[u][k] = t[u][k] = 0.f;
+    if (r + u * step >= end) continue;
+    row4(q.src + (r + u * step) * q.ld, c, q.cols, q.vec, v[u]);
+    if (q.act != VCB_ACT_NONE) row4(q.z + (r + u * step) * q.ldz, c, q.cols, q.vec, t[u]);
+  }
+  if (q.act != VCB_ACT_NONE) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) act_grads(v[u], t[u], q.act);
+  }
 }
 
 // The job and strip (of `width` columns) of strip s of a launch.
@@ -214,13 +225,7 @@ __global__ void __launch_bounds__(kStripThreads, 4)
   constexpr int U = 4, W = kStripWarps * 4;  // rows in flight per lane, rows of a CTA's step
   for (long long base = r0 + warp * 4; base < r1; base += U * W) {
     float v[U][4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long r = base + u * W + (lane >> 3);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
-      if (r < r1) job4(q, r, c, v[u]);
-    }
+    job_rows<U>(q, base + (lane >> 3), W, r1, c, v);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long r = base + u * W + (lane >> 3);
@@ -288,16 +293,20 @@ __global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < 4; ++i) scale[i] = c + i < q.cols ? exp2i(-scale_exp(q.col_most[c + i])) : 0.f;
   const long long end = min(q.rows, (blockIdx.y + 1LL) * kHalvesRows);
-#pragma unroll 2
-  for (long long r = static_cast<long long>(blockIdx.y) * kHalvesRows + warp; r < end;
-       r += kStripWarps) {
-    float v[4];
-    job4(q, r, c, v);
-    if (q.by_row) put_halves(q.by_row + r * q.ldh + c, q.plane, v, exp2i(-scale_exp(q.row_most[r])));
+  constexpr int U = kHalvesRows / kStripWarps;  // rows of a warp
+  const long long r0 = static_cast<long long>(blockIdx.y) * kHalvesRows + warp;
+  float v[U][4];
+  job_rows<U>(q, r0, kStripWarps, end, c, v);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long r = r0 + u * kStripWarps;
+    if (r >= end) break;
+    if (q.by_row)
+      put_halves(q.by_row + r * q.ldh + c, q.plane, v[u], exp2i(-scale_exp(q.row_most[r])));
     if (q.by_col) {
       __half h[4], l[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) halves(v[i], scale[i], h[i], l[i]);
+      for (int i = 0; i < 4; ++i) halves(v[u][i], scale[i], h[i], l[i]);
       __half* at = q.by_col + r * q.ldh + c;
       *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(h);
       *reinterpret_cast<uint2*>(at + q.plane) = *reinterpret_cast<const uint2*>(l);
@@ -623,8 +632,9 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
 // ---- host ----
 // M N K from which the tensor cores are used.  Forward: 64 x 1024 x 1024 (2^26) 12.6
 // us against 15.4 on the FP32 units, 64 x 512 x 512 9.9 against 5.8.  Backward, with
-// two more launches: 512^3 (2^27) 38 against 46, 256 x 512 x 512 39 against 23.
-constexpr long long kTcLeast = 1LL << 26, kTcLeastBackward = 1LL << 27;
+// two more launches: 146 x 800 x 810 (2^26.5) 40 against 48, 300 x 300 x 1000 28
+// against 36, 512 x 512 x 256 (2^26) 28 against 26, 128 x 512 x 512 30 against 20.
+constexpr long long kTcLeast = 1LL << 26;
 
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -800,11 +810,11 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
 }
 
 bool f32_backward_fits(const Bwd& b) {
-  return b.type == VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K, kTcLeastBackward);
+  return b.type == VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K, kTcLeast);
 }
 
 size_t f32_backward_bytes(int M, int N, int K) {
-  if (!fits(M, N, K, kTcLeastBackward)) return 0;
+  if (!fits(M, N, K, kTcLeast)) return 0;
   return 2 * halves_bytes(M, N) + halves_bytes(N, K) + halves_bytes(M, K) + up256(M * 4LL) +
          up256(N * 4LL) + 2 * up256(K * 4LL) + 256;
 }

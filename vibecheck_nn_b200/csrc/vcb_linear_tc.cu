@@ -465,21 +465,36 @@ struct Prep {
 constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
 constexpr int kStrip = 32;  // columns
 
-// Four elements at p, `align` bytes aligned (8, 4 or 2); 0 from `left` on.
+// Four elements of a row as loaded: two words, or an element in each.  They are
+// unpacked where they are used: more loads follow these.
+struct Loaded {
+  uint32_t w[4];
+};
+
+// From p, `align` bytes aligned (8, 4 or 2); 0 from `left` on.
 template <typename T>
-__device__ __forceinline__ void four_at(const T* p, int align, int left, float (&v)[4]) {
-  T e[4];
+__device__ __forceinline__ void four_at(const T* p, int align, int left, Loaded& e) {
   if (align == 8 && left >= 4) {
-    *reinterpret_cast<uint2*>(e) = __ldcs(reinterpret_cast<const uint2*>(p));
+    const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
+    e.w[0] = t.x, e.w[1] = t.y;
   } else if (align >= 4 && left >= 4) {
-    reinterpret_cast<uint32_t*>(e)[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
-    reinterpret_cast<uint32_t*>(e)[1] = __ldcs(reinterpret_cast<const uint32_t*>(p) + 1);
+    e.w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    e.w[1] = __ldcs(reinterpret_cast<const uint32_t*>(p) + 1);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = i < left ? p[i] : from_f32<T>(0.f);
+    for (int i = 0; i < 4; ++i)
+      e.w[i] = i < left ? __ldcs(reinterpret_cast<const uint16_t*>(p) + i) : 0;
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void values(const Loaded& e, bool packed, float (&v)[4]) {
+  const uint32_t w[2] = {packed ? e.w[0] : e.w[0] | e.w[1] << 16,
+                         packed ? e.w[1] : e.w[2] | e.w[3] << 16};
+  T t[4];
+  *reinterpret_cast<uint2*>(t) = make_uint2(w[0], w[1]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
+  for (int i = 0; i < 4; ++i) v[i] = to_f32(t[i]);
 }
 
 // Alignment of all rows of a 16-bit matrix at columns that are multiples of 4.
@@ -526,12 +541,10 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
     float sum[4] = {};
     constexpr int U = 2, W = kPrepWarps * 4;  // rows in flight, rows of a CTA's step
     for (long long r = r0 + warp * 4 + (lane >> 3); r < r1; r += U * W) {
-      float g[U][4], t[U][4];
+      Loaded g[U], t[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const long long row = r + k * W;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) g[k][i] = t[k][i] = 0.f;
         if (row >= r1) continue;
         four_at(dy + row * a.lddy, ay, left, g[k]);
         if (a.act != VCB_ACT_NONE) four_at(z + row * a.ldz, az, left, t[k]);
@@ -540,13 +553,16 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
       for (int k = 0; k < U; ++k) {
         const long long row = r + k * W;
         if (row >= r1) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[k][i] = act_grad(g[k][i], t[k][i], a.act);
-          sum[i] += g[k][i];
+        float v[4], w[4];
+        values<T>(g[k], ay >= 4 && left >= 4, v);
+        if (a.act != VCB_ACT_NONE) {
+          values<T>(t[k], az >= 4 && left >= 4, w);
+          act_grads(v, w, a.act);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += v[i];
         // lddz is a multiple of 8, so a vector that crosses N stays in its row
-        if (a.dz && left > 0) store4(static_cast<T*>(a.dz) + row * a.lddz + c, g[k]);
+        if (a.dz && left > 0) store4(static_cast<T*>(a.dz) + row * a.lddz + c, v);
       }
     }
     if (a.db) {
@@ -729,9 +745,12 @@ int launch_type(Launch& L, const Plan& plan, int type, cudaStream_t st, const ch
 
 namespace {
 
-// M N K from which the tensor cores are used: bf16 64 x 256 x 256 (2^22) 4.9 us
-// against 5.4 on the FP32 units, 8 x 1024 x 1024 backward 10 against 45.
-constexpr long long kTcLeast = 1LL << 20;
+// M N K from which the tensor cores are used.  As the operands lie: bf16 64 x 256 x
+// 256 (2^22) 4.9 us against 5.4 on the FP32 units, 100 x 200 x 200 9.2 against 11.3,
+// 8 x 1024 x 1024 backward 10 against 45.  With a launch that prepares them: 128 x
+// 128 x 128 backward (2^21, GELU) 17 against 13, 2000 x 63 x 63 (2^23) 15 against
+// 11, 64 x 300 x 301 backward (2^22.5) 17 and 17.
+constexpr long long kTcLeast = 1LL << 20, kTcLeastPrepared = 1LL << 23;
 
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 size_t matrix_bytes(long long rows, long long cols) {
@@ -743,9 +762,9 @@ bool tma_rows(const void* p, long long ld) {
 }
 
 // Sizes that 32-bit tile and TMA coordinates describe.
-bool fits(long long M, long long N, long long K) {
+bool fits(long long M, long long N, long long K, bool prepared) {
   const long long most = 1LL << 30;
-  return M * N * K >= kTcLeast && M < most && N < most && K < most &&
+  return M * N * K >= (prepared ? kTcLeastPrepared : kTcLeast) && M < most && N < most && K < most &&
          ((M + 15) / 16) * ((N + 127) / 128) < most && ((N + 15) / 16) * ((K + 127) / 128) < most &&
          ((M + 15) / 16) * ((K + 127) / 128) < most;
 }
@@ -797,10 +816,13 @@ int launch_prep(Prep& a, int type, cudaStream_t st, const char* who) {
 
 }  // namespace
 
-bool tc_forward_fits(const Fwd& f) { return f.type != VCB_F32 && fits(f.M, f.N, f.K); }
+bool tc_forward_fits(const Fwd& f) {
+  return f.type != VCB_F32 &&
+         fits(f.M, f.N, f.K, !tma_rows(f.x, f.ldx) || !tma_rows(f.w, f.ldw));
+}
 
 size_t tc_forward_bytes(int M, int N, int K) {
-  return fits(M, N, K) ? matrix_bytes(M, K) + matrix_bytes(N, K) + 256 : 0;
+  return fits(M, N, K, true) ? matrix_bytes(M, K) + matrix_bytes(N, K) + 256 : 0;
 }
 
 int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
@@ -823,11 +845,13 @@ int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
 }
 
 bool tc_backward_fits(const Bwd& b) {
-  return b.type != VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K);
+  const bool prepared = b.act != VCB_ACT_NONE || b.db || !tma_rows(b.dy, b.lddy) ||
+                        !tma_rows(b.x, b.ldx) || !tma_rows(b.w, b.ldw);
+  return b.type != VCB_F32 && (b.dx || b.dw) && fits(b.M, b.N, b.K, prepared);
 }
 
 size_t tc_backward_bytes(int M, int N, int K, int act, bool rows16) {
-  if (!fits(M, N, K) || (rows16 && act == VCB_ACT_NONE)) return 0;
+  if ((rows16 && act == VCB_ACT_NONE) || !fits(M, N, K, true)) return 0;
   return matrix_bytes(M, N) + (rows16 ? 0 : matrix_bytes(N, K) + matrix_bytes(M, K)) + 256;
 }
 
