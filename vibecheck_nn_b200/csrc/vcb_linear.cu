@@ -335,22 +335,25 @@ namespace {
 bool misaligned(const void* p, int type) {
   return reinterpret_cast<uintptr_t>(p) % dtype_bytes(type) != 0;
 }
-// Which calls take the kernels for few rows (vcb_linear_rows.cu).  Forward in us,
-// others against them: fp32 1 x 4096 x 4096 62 against 7.7, 8 x 4096 x 4096 37
-// against 26, 16 x 1024 x 1024 7.7 against 5.4 but 16 x 4096 x 4096 37 against 48;
-// bf16 8 x 1024 x 1024 5.9 against 4.5, 1 x 4096 x 4096 equal, 4 x 4096 x 4096 8.8
-// against 25.  Backward: fp32 16 x 1024 x 1024 36 against 14, 16 x 256 x 256 6.7
-// against 8.8; bf16 4 x 4096 x 4096 44 against 27, 16 x 1024 x 1024 10 against 17.
+// Which calls take the kernels for few rows (vcb_linear_rows.cu).  Times in us with
+// cold inputs, theirs first.  Forward: fp32 8 x 4096 x 4096 33 against 50, 16 x 1024 x
+// 1024 11 against 14, 16 x 2048 x 2048 20 against 35, but 16 x 4096 x 4096 51 against
+// 48; bf16 1 x 4096 x 4096 16
+// against 18, x 4097 18 against 34, 2 x 4096 x 4097 23 against 35, 4 x 1024 x 1024 8
+// against 12, but 4 x 4096 x 4096 22 against 18.  Backward: fp32 16 x 1024 x 1024 25
+// against 31, 16 x 2048 x 2048 32 against 80, but 4 x 60 x 60 13 against 9; bf16 4 x
+// 4096 x 4096 39 against 52, 6 x 1024 x 1024 20 against 35, but 8 x 1024 x 1024 22
+// against 20.
 bool few_rows_forward(long long M, long long N, long long K, int type) {
   if (M <= 0 || N <= 0 || K <= 0) return false;
-  if (type == VCB_F32) return M <= 8 || (M <= lin::kFewRows && N * K <= (1 << 20));
-  return M <= 8 && M * N * K <= (1 << 23);
+  if (type == VCB_F32) return M <= 8 || (M <= lin::kFewRows && N * K <= (1 << 23));
+  return M <= 2 || (M <= 8 && M * N * K <= (1 << 23));
 }
 
 bool few_rows_backward(long long M, long long N, long long K, int type) {
   if (M <= 0 || N <= 0 || K <= 0) return false;
-  if (M <= 4) return true;
-  return type == VCB_F32 && M <= lin::kFewRows && N * K >= (1 << 18);
+  if (N * K < (1 << 18)) return M <= 2;
+  return M <= 4 || (type == VCB_F32 ? M <= lin::kFewRows : M <= 8 && M * N * K < (1 << 23));
 }
 }  // namespace
 }  // namespace vcb

@@ -22,30 +22,67 @@ namespace {
 
 constexpr int kRowThreads = 256, kRowWarps = 8, kOut = 4;
 
-// N elements of a row from c on (lane-wise): a vector, or elements 32 apart.
-template <typename T, int N>
-__device__ __forceinline__ void row_part(const T* row, int base, int lane, int cols, bool vec,
-                                         float (&v)[N]) {
-  if (vec) {
-    const int c = base + lane * N;
-    if (c + N <= cols) {
-      const uint4 q = *reinterpret_cast<const uint4*>(row + c);
-      T e[N];
-      *reinterpret_cast<uint4*>(e) = q;
+// V neighbouring elements as loaded.  They are unpacked where they are used: a use
+// would wait for them, and more loads follow.
+template <typename T, int V>
+struct Raw {
+  static constexpr int W = V * sizeof(T) / 4;
+  uint32_t w[W + 1];
+  bool odd;  // words of the elements from the second on, then the first and the last element
+
+  // At p; 0 from `left` on.  vec: p is aligned to all V elements.
+  __device__ __forceinline__ void load(const T* p, int left, bool vec) {
+    odd = false;
+    if (left < V) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = to_f32(e[i]);
+      for (int i = 0; i < W; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          w[i] = i < left ? reinterpret_cast<const uint32_t*>(p)[i] : 0;
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+          w[i] = (2 * i < left ? h[0] : 0u) | (2 * i + 1 < left ? h[1] : 0u) << 16;
+        }
+      }
+    } else if (vec) {
+      struct alignas(4 * W) Pack {
+        uint32_t w[W];
+      };
+      const Pack q = *reinterpret_cast<const Pack*>(p);
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = q.w[i];
     } else {
+      odd = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(p) % 4 != 0;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p + odd);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = base + i * 32 + lane;
-      v[i] = c < cols ? to_f32(row[c]) : 0.f;
+      for (int i = 0; i < W - 1; ++i) w[i] = q[i];
+      if (odd) {
+        w[W - 1] = *reinterpret_cast<const uint16_t*>(p);
+        w[W] = *reinterpret_cast<const uint16_t*>(p + V - 1);
+      } else {
+        w[W - 1] = q[W - 1];
+      }
     }
   }
-}
+  __device__ __forceinline__ void values(float (&v)[V]) const {
+    uint32_t o[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint32_t low = i ? w[i - 1] >> 16 : w[W - 1], high = i < W - 1 ? w[i] : w[W];
+      o[i] = odd ? low | high << 16 : w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      T e;
+      if constexpr (sizeof(T) == 4) {
+        e = __uint_as_float(o[i]);
+      } else {
+        const uint16_t h = static_cast<uint16_t>(i % 2 ? o[i / 2] >> 16 : o[i / 2]);
+        e = *reinterpret_cast<const T*>(&h);
+      }
+      v[i] = to_f32(e);
+    }
+  }
+};
 
 // Sums of N values over the warp; lane l < N gets value l (N a power of two).
 template <int N>
@@ -83,14 +120,19 @@ __global__ void __launch_bounds__(kRowThreads) rows_forward_kernel(const __grid_
   float acc[NV] = {};
 #pragma unroll 2
   for (int base = warp * 32 * V; base < f.K; base += kRowWarps * 32 * V) {
+    const int c = base + lane * V, left = f.K - c;
+    Raw<T, V> wr[kOut], xr[MR];
+#pragma unroll
+    for (int r = 0; r < kOut; ++r) wr[r].load(w + min(n0 + r, f.N - 1) * f.ldw + c, left, a.vec);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) xr[m].load(x + min(m0 + m, f.M - 1) * f.ldx + c, left, a.vec);
     float wv[kOut][V];
 #pragma unroll
-    for (int r = 0; r < kOut; ++r)
-      row_part<T, V>(w + min(n0 + r, f.N - 1) * f.ldw, base, lane, f.K, a.vec, wv[r]);
+    for (int r = 0; r < kOut; ++r) wr[r].values(wv[r]);
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
       float xv[V];
-      row_part<T, V>(x + min(m0 + m, f.M - 1) * f.ldx, base, lane, f.K, a.vec, xv);
+      xr[m].values(xv);
 #pragma unroll
       for (int r = 0; r < kOut; ++r) {
 #pragma unroll
@@ -120,22 +162,6 @@ struct RowsBwd {
 };
 
 constexpr int kSpan = 512;  // rows n whose dz are in shared memory at a time
-
-// V neighbouring elements of a row, 0 from `left` on.
-template <typename T, int V>
-__device__ __forceinline__ void some(const T* p, int left, bool vec, float (&v)[V]) {
-  struct alignas(sizeof(T) * V) Pack {
-    T e[V];
-  };
-  if (vec && left >= V) {
-    const Pack q = *reinterpret_cast<const Pack*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_f32(q.e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
-  }
-}
 
 template <typename T, int V>
 __device__ __forceinline__ void put_some(T* p, int left, bool vec, const float (&v)[V]) {
@@ -173,12 +199,9 @@ __global__ void __launch_bounds__(kRowThreads) rows_backward_kernel(const __grid
   if (b.dw) {
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
-      if (m < b.M) {
-        some<T, V>(static_cast<const T*>(b.x) + m * b.ldx + c, left, a.vec_x, x[m]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[m][i] = 0.f;
-      }
+      Raw<T, V> r;
+      r.load(static_cast<const T*>(b.x) + min(m, b.M - 1) * b.ldx + c, m < b.M ? left : 0, a.vec_x);
+      r.values(x[m]);
     }
   }
   for (int n0 = n_begin; n0 < n_end; n0 += kSpan) {
@@ -199,29 +222,42 @@ __global__ void __launch_bounds__(kRowThreads) rows_backward_kernel(const __grid
       if (b.db && strip == 0) static_cast<T*>(b.db)[n] = from_f32<T>(sum);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int t = warp; t < rows; t += kRowWarps) {
-      const long long n = n0 + t;
-      float dz[MR];
-#pragma unroll
-      for (int m = 0; m < MR; ++m) dz[m] = buf[t * MR + m];
+    constexpr int U = 4;  // rows of W in flight; the stores of dW between them would end that
+    for (int t0 = warp; t0 < rows; t0 += U * kRowWarps) {
+      Raw<T, V> wr[U];
       if (b.dx) {
-        float v[V];
-        some<T, V>(w + n * b.ldw, left, a.vec_w, v);
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[m][i] = fmaf(dz[m], v[i], acc[m][i]);
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + u * kRowWarps;
+          if (t < rows) wr[u].load(w + (long long)(n0 + t) * b.ldw, left, a.vec_w);
         }
       }
-      if (b.dw) {
-        float v[V] = {};
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kRowWarps;
+        if (t >= rows) break;
+        const long long n = n0 + t;
+        float dz[MR];
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] = fmaf(dz[m], x[m][i], v[i]);
+        for (int m = 0; m < MR; ++m) dz[m] = buf[t * MR + m];
+        if (b.dx) {
+          float v[V];
+          wr[u].values(v);
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[m][i] = fmaf(dz[m], v[i], acc[m][i]);
+          }
         }
-        put_some<T, V>(dw + n * b.lddw, left, a.vec_dw, v);
+        if (b.dw) {
+          float v[V] = {};
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = fmaf(dz[m], x[m][i], v[i]);
+          }
+          put_some<T, V>(dw + n * b.lddw, left, a.vec_dw, v);
+        }
       }
     }
   }
