@@ -8,7 +8,7 @@
 //
 // Small products are bound by latency, so a product of few tiles is spread as wide
 // as it goes: a 32 x 32 tile per CTA of 256 threads, four groups of 64 threads each
-// taking a quarter of every 64-deep step of the contraction, and the contraction cut
+// taking every fourth chunk of every 64-deep step of the contraction, and the contraction cut
 // over up to 8 CTAs of a cluster when there are few tiles.  Groups are joined through
 // shared memory and CTAs through distributed shared memory, in order.  Operands lie
 // in shared memory by row, four entries of the contraction to a 16-byte chunk, chunks
@@ -159,8 +159,9 @@ __global__ void __launch_bounds__(kSmallThreads, CTAS)
         rs += (v.x + v.y) + (v.z + v.w);
       }
     }
+    const int chunks = min(kTT / 4, (s.T - step * kTT + 3) / 4);  // the others are 0
 #pragma unroll (CTAS == 2 ? 2 : 1)
-    for (int c = group * 4; c < group * 4 + 4; ++c) {
+    for (int c = group; c < chunks; c += kGroups) {
       // rows 8 apart share their place in the XOR
       const float* at_a = sa + ty * kTT + ((c ^ ty) << 2);
       const float* at_b = sb + tx * kTT + ((c ^ tx) << 2);
