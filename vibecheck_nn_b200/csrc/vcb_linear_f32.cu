@@ -111,6 +111,7 @@ template <int TPR>  // threads per row
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJobs a) {
   constexpr int kKeep = 4;  // vectors of a row that stay in registers
   __shared__ uint32_t warp_most[8];
+  let_next_start();
   long long r = static_cast<long long>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const bool second = r >= a.j[0].rows;
@@ -218,6 +219,7 @@ __global__ void __launch_bounds__(kStripThreads, 4)
     scales_kernel(const __grid_constant__ ColJobs a) {
   __shared__ float part[kStripWarps][32], sum_mine[32];
   __shared__ uint32_t most_part[kStripWarps][32], most_mine[32];
+  let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int size = a.cluster, rank = blockIdx.x % size;
   int strip = blockIdx.x / size;
@@ -288,6 +290,8 @@ __global__ void __launch_bounds__(kStripThreads, 4)
 constexpr int kHalvesRows = 32;  // rows of a CTA
 
 __global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_constant__ ColJobs a) {
+  after_previous();
+  let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int strip = blockIdx.x;
   const ColJob& q = strip_of(a, strip, 128);
@@ -430,6 +434,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
   __syncthreads();
   if (PAIR) cluster_sync();  // barriers of both CTAs are ready
   fence_after_sync();
+  after_previous();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   // the part of a contraction of nk stages
   const auto begin = [&](int nk) { return PAIR ? 0 : static_cast<int>((long long)nk * rank / size); };
@@ -736,32 +741,22 @@ int set_prod(Prod32& r, int I, int J, int T, const Halves& a, const Halves& b, c
 }
 
 template <int BN, bool PAIR>
-int launch(const Launch32& L, cudaStream_t st, const char* who) {
+int launch(const Launch32& L, bool chained, cudaStream_t st, const char* who) {
   using C = Cfg<BN, PAIR>;
   g_launched = true;
   const auto kernel = f32_kernel<BN, PAIR>;
   const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
   if (rc) return rc;
   const int size = PAIR ? 2 : L.split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units));
-  cfg.blockDim = dim3(kF32Threads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = size;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  return check_launch(who);
+  return launch_clusters(kernel, L, size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units),
+                         kF32Threads, C::kSmem, size, chained, st, who);
 }
 
-int launch_plan(const Launch32& L, const Plan32& plan, cudaStream_t st, const char* who) {
-  if (plan.pair) return launch<256, true>(L, st, who);
-  return plan.bn == 64 ? launch<64, false>(L, st, who) : launch<128, false>(L, st, who);
+int launch_plan(const Launch32& L, const Plan32& plan, bool chained, cudaStream_t st,
+                const char* who) {
+  if (plan.pair) return launch<256, true>(L, chained, st, who);
+  return plan.bn == 64 ? launch<64, false>(L, chained, st, who)
+                       : launch<128, false>(L, chained, st, who);
 }
 
 bool vec16(const void* p, long long ld) {
@@ -810,7 +805,7 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
   if (rc) return rc;
   L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
   L.split = plan.split;
-  return launch_plan(L, plan, st, who);
+  return launch_plan(L, plan, true, st, who);
 }
 
 bool f32_backward_fits(const Bwd& b) {
@@ -858,24 +853,12 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_fail(e, who);
   jobs.cluster = 1;  // a CTA's step is 128 rows
   while (jobs.cluster < 8 && tall > 128 * jobs.cluster) jobs.cluster *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(strips * jobs.cluster));
-  cfg.blockDim = dim3(kStripThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = jobs.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, scales_kernel, jobs);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  int rc = check_launch(who);
+  int rc = launch_clusters(scales_kernel, jobs, static_cast<unsigned>(strips * jobs.cluster),
+                           kStripThreads, 0, jobs.cluster, false, st, who);
   if (rc) return rc;
-  halves_kernel<<<dim3(static_cast<unsigned>(wide),
-                       static_cast<unsigned>((tall + kHalvesRows - 1) / kHalvesRows)),
-                  kStripThreads, 0, st>>>(jobs);
-  rc = check_launch(who);
+  const auto blocks = static_cast<unsigned>((tall + kHalvesRows - 1) / kHalvesRows);
+  rc = launch_clusters(halves_kernel, jobs, dim3(static_cast<unsigned>(wide), blocks),
+                       kStripThreads, 0, 1, true, st, who);
   if (rc) return rc;
   const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
   const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
@@ -893,7 +876,7 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
     L.split = px.split;
     if (!together) {
-      rc = launch_plan(L, px, st, who);
+      rc = launch_plan(L, px, true, st, who);
       if (rc || !b.dw) return rc;
       L.units0 = L.units = 0;
     }
@@ -904,7 +887,7 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   L.units += p.tiles_i * p.tiles_j;
   if (!together) L.units0 = L.units;
   L.split = pw.split;
-  return launch_plan(L, pw, st, who);
+  return launch_plan(L, pw, together || !b.dx, st, who);
 }
 
 int f32_fault_take(cudaStream_t st, int* was_set) {

@@ -155,7 +155,7 @@ constexpr int kPairStage = 2 * kBytesA;  // per CTA: 128 rows of A and 128 of B
 constexpr int kPairSmem = kPairStages * kPairStage + 1024;
 
 template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ Launch L) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -190,6 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncthreads();
   cluster_sync();  // barriers of both CTAs are ready
   fence_after_sync();
+  after_previous();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
   if (warp == kPairEpi) {
@@ -338,6 +339,7 @@ __global__ void __launch_bounds__(kThreads)
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
+  after_previous();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   const int j0 = tj * kTileJ, i0 = ti * p.bn;
   bool ok = true;
@@ -535,6 +537,7 @@ template <typename T>
 __global__ void __launch_bounds__(kPrepThreads, 5)
     prep_kernel(const __grid_constant__ Prep a) {
   __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
+  let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int size = a.cluster, strip = blockIdx.x / size;
   if (strip < a.strips) {
@@ -703,15 +706,14 @@ int set_prod(Prod& r, int type, int I, int J, int T, const Operand& a, const Ope
 }
 
 template <typename T>
-int launch_tc(Launch& L, const Plan& plan, cudaStream_t st, const char* who) {
+int launch_tc(Launch& L, const Plan& plan, bool chained, cudaStream_t st, const char* who) {
   g_launched = true;
   if (plan.pair) {
     const auto kernel = pair_kernel<T>;
     const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), kPairSmem);
     if (rc) return rc;
     const int grid = 2 * std::min(L.units, sm_count() / 2);
-    kernel<<<grid, kPairThreads, kPairSmem, st>>>(L);
-    return check_launch(who);
+    return launch_clusters(kernel, L, grid, kPairThreads, kPairSmem, 2, chained, st, who);
   }
   const auto kernel = split_kernel<T>;
   const int bn = std::max(L.units0 ? L.p[0].bn : 0, L.units > L.units0 ? L.p[1].bn : 0);
@@ -727,25 +729,14 @@ int launch_tc(Launch& L, const Plan& plan, cudaStream_t st, const char* who) {
   const int smem = std::max(L.stages * stage, plan.split > 1 ? bn * kTileJ * 4 : 0) + 1024;
   const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - 1024);
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * plan.split));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = plan.split;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  return check_launch(who);
+  return launch_clusters(kernel, L, static_cast<unsigned>(clusters * plan.split), kThreads, smem,
+                         plan.split, chained, st, who);
 }
 
-int launch_type(Launch& L, const Plan& plan, int type, cudaStream_t st, const char* who) {
-  return type == VCB_BF16 ? launch_tc<__nv_bfloat16>(L, plan, st, who)
-                          : launch_tc<__half>(L, plan, st, who);
+int launch_type(Launch& L, const Plan& plan, int type, bool chained, cudaStream_t st,
+                const char* who) {
+  return type == VCB_BF16 ? launch_tc<__nv_bfloat16>(L, plan, chained, st, who)
+                          : launch_tc<__half>(L, plan, chained, st, who);
 }
 
 namespace {
@@ -803,20 +794,8 @@ int launch_prep(Prep& a, int type, cudaStream_t st, const char* who) {
   while (a.strips && a.cluster < 8 && a.M > 64 * a.cluster) a.cluster *= 2;
   const long long grid = (a.strips + (ctas + a.cluster - 1) / a.cluster) * (long long)a.cluster;
   if (grid == 0) return VCB_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kPrepThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = a.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const auto kernel = type == VCB_BF16 ? prep_kernel<__nv_bfloat16> : prep_kernel<__half>;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  return check_launch(who);
+  return launch_clusters(type == VCB_BF16 ? prep_kernel<__nv_bfloat16> : prep_kernel<__half>, a,
+                         static_cast<unsigned>(grid), kPrepThreads, 0, a.cluster, false, st, who);
 }
 
 }  // namespace
@@ -846,7 +825,7 @@ int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
   p.epi = {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
   p.epi.vec = vector_rows(p.epi, 2);
   L.units0 = L.units = p.tiles_i * p.tiles_j;
-  return launch_type(L, plan, f.type, st, who);
+  return launch_type(L, plan, f.type, prep.copies > 0, st, who);
 }
 
 bool tc_backward_fits(const Bwd& b) {
@@ -878,6 +857,7 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (b.dw) x = readable(b.x, b.ldx, b.M, b.K, true, prep, arena);
   int rc = launch_prep(prep, b.type, st, who);
   if (rc) return rc;
+  const bool prepared = prep.strips || prep.copies;
   // dX and dW share a launch when both are pairs or both are not; the contraction of
   // dW, the rows, is then not cut
   const Plan px = plan_of(b.M, b.K, b.N, true, false), pw = plan_of(b.N, b.K, b.M, true, true);
@@ -893,7 +873,7 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
   }
   if (b.dx && !together) {
-    rc = launch_type(L, px, b.type, st, who);
+    rc = launch_type(L, px, b.type, prepared, st, who);
     if (rc) return rc;
     L.units0 = L.units = 0;
   }
@@ -910,7 +890,7 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
       L.p[0] = L.p[1];
       L.units0 = L.units;
     }
-    rc = launch_type(L, plan, b.type, st, who);
+    rc = launch_type(L, plan, b.type, prepared && (together || !b.dx), st, who);
   }
   return rc;
 }

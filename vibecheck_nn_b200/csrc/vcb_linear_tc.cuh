@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t ctarank() {
   return r;
 }
 
+// A kernel that prepares operands lets the product's CTAs take their places, barriers
+// and tensor memory as its own run out; each thread of the product waits for all that
+// was prepared before it touches anything else.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile(
       "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
@@ -197,6 +208,28 @@ __device__ __forceinline__ void tile_at(int tiles_i, int tiles_j, int u, int& ti
   const int rows = min(G, tiles_i - g * G);
   ti = g * G + in % rows;
   tj = in / rows;
+}
+
+// Launches in clusters of `size`; with `chained` as the kernel before it runs out.
+template <typename Args>
+int launch_clusters(void (*kernel)(Args), const Args& args, dim3 grid, int threads, int smem,
+                    int size, bool chained, cudaStream_t st, const char* who) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return check_launch(who);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
