@@ -460,7 +460,8 @@ struct Copy {
 };
 
 struct Prep {
-  int M, N, act, strips;  // strips of 32 columns of dy, 0 for none
+  int M, N, act, strips;  // strips of 4 lanes columns of dy, 0 for none
+  int lanes;              // of a row in a strip: 8 or 4
   const void *dy, *z;
   void *dz, *db;          // either may be NULL
   long long lddy, ldz, lddz;
@@ -470,7 +471,7 @@ struct Prep {
 };
 
 constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
-constexpr int kStrip = 32;  // columns
+constexpr int kStrip = 32;  // columns at most
 
 // Four elements of a row as loaded: two words, or an element in each.  They are
 // unpacked where they are used: more loads follow these.
@@ -529,11 +530,11 @@ __device__ __forceinline__ uint4 eight_at(const uint16_t* p, int left) {
   return make_uint4(a0 | w0 << 16, w0 >> 16 | w1 << 16, w1 >> 16 | w2 << 16, w2 >> 16 | a7 << 16);
 }
 
-// A cluster of up to 8 CTAs per strip of 32 columns: each sums its part of the rows
-// (8 lanes per row, 4 columns per lane), rank 0 adds the sums in order.  Bound by
+// A cluster of up to 8 CTAs per strip of 32 or 16 columns: each sums its part of the
+// rows (4 columns per lane), rank 0 adds the sums in order.  Bound by
 // HBM: dy and z are read and dz is written once; strips are narrow so that a matrix
 // of 2,000 columns keeps every SM reading.  The remaining CTAs copy.
-template <typename T>
+template <typename T, int LANES>  // of a row in a strip
 __global__ void __launch_bounds__(kPrepThreads, 5)
     prep_kernel(const __grid_constant__ Prep a) {
   __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
@@ -541,14 +542,15 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int size = a.cluster, strip = blockIdx.x / size;
   if (strip < a.strips) {
-    const int rank = blockIdx.x % size, c = strip * kStrip + (lane & 7) * 4;
+    constexpr int lanes = LANES, rows = 32 / lanes;  // rows of a warp
+    const int rank = blockIdx.x % size, c = (strip * lanes + lane % lanes) * 4;
     const long long r0 = static_cast<long long>(a.M) * rank / size;
     const long long r1 = static_cast<long long>(a.M) * (rank + 1) / size;
     const T *dy = static_cast<const T*>(a.dy) + c, *z = static_cast<const T*>(a.z) + c;
     const int ay = rows_align(a.dy, a.lddy), az = rows_align(a.z, a.ldz), left = a.N - c;
     float sum[4] = {};
-    constexpr int U = 2, W = kPrepWarps * 4;  // rows in flight, rows of a CTA's step
-    for (long long r = r0 + warp * 4 + (lane >> 3); r < r1; r += U * W) {
+    constexpr int U = 2, W = kPrepWarps * rows;  // rows in flight, rows of a CTA's step
+    for (long long r = r0 + warp * rows + lane / lanes; r < r1; r += U * W) {
       Loaded g[U], t[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
@@ -576,20 +578,20 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
     if (a.db) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
-        if (lane < 8) part[warp][lane * 4 + i] = sum[i];
+#pragma unroll
+        for (int k = lanes; k < 32; k *= 2) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
+        if (lane < lanes) part[warp][lane * 4 + i] = sum[i];
       }
       __syncthreads();
-      if (threadIdx.x < kStrip) {
+      if (threadIdx.x < lanes * 4) {
         float v = 0.f;
         for (int w = 0; w < kPrepWarps; ++w) v += part[w][threadIdx.x];
         mine[threadIdx.x] = v;
       }
     }
     cluster_sync();
-    if (a.db && rank == 0 && threadIdx.x < kStrip) {
-      const int col = strip * kStrip + threadIdx.x;
+    if (a.db && rank == 0 && threadIdx.x < lanes * 4) {
+      const int col = strip * lanes * 4 + threadIdx.x;
       float v = 0.f;
       for (int k = 0; k < size; ++k) v += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
       if (col < a.N) static_cast<T*>(a.db)[col] = from_f32<T>(v);
@@ -790,12 +792,15 @@ int launch_prep(Prep& a, int type, cudaStream_t st, const char* who) {
     vectors = std::max(vectors, a.copy[k].rows * ((a.copy[k].cols + 7LL) / 8));
   const long long ctas =
       std::min<long long>((vectors + kPrepThreads - 1) / kPrepThreads, 4LL * sm_count());
-  a.cluster = 1;  // a CTA's step is 64 rows
+  a.cluster = 1;  // a CTA's step is 64 rows or more
   while (a.strips && a.cluster < 8 && a.M > 64 * a.cluster) a.cluster *= 2;
   const long long grid = (a.strips + (ctas + a.cluster - 1) / a.cluster) * (long long)a.cluster;
   if (grid == 0) return VCB_OK;
-  return launch_clusters(type == VCB_BF16 ? prep_kernel<__nv_bfloat16> : prep_kernel<__half>, a,
-                         static_cast<unsigned>(grid), kPrepThreads, 0, a.cluster, false, st, who);
+  const auto kernel = type == VCB_BF16
+                          ? a.lanes == 4 ? prep_kernel<__nv_bfloat16, 4> : prep_kernel<__nv_bfloat16, 8>
+                          : a.lanes == 4 ? prep_kernel<__half, 4> : prep_kernel<__half, 8>;
+  return launch_clusters(kernel, a, static_cast<unsigned>(grid), kPrepThreads, 0, a.cluster, false,
+                         st, who);
 }
 
 }  // namespace
@@ -851,7 +856,12 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
     prep.dz = arena.take(matrix_bytes(b.M, b.N));
     dz = {prep.dz, prep.lddz, false};
   }
-  if (prep.dz || prep.db) prep.strips = (b.N + kStrip - 1) / kStrip;
+  if (prep.dz || prep.db) {
+    // narrower strips where those of 32 columns would leave a third of the SMs' places
+    // empty: bf16 4096 x 1024 x 1024 (GELU) 58 -> 54 us, 5273 x 444 x 131 50 -> 44 us
+    prep.lanes = ((b.N + 31) / 32) * 8 < 3 * sm_count() ? 4 : 8;
+    prep.strips = (b.N + 4 * prep.lanes - 1) / (4 * prep.lanes);
+  }
   Operand w{}, x{};
   if (b.dx) w = readable(b.w, b.ldw, b.N, b.K, true, prep, arena);
   if (b.dw) x = readable(b.x, b.ldx, b.M, b.K, true, prep, arena);
