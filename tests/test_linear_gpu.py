@@ -246,3 +246,63 @@ def test_refusals():
                                   0, None) == _lib.VCB_ERR_INVALID
     assert lib.vcb_linear_backward(2, 3, 4, 0, p, 3, p, 4, p, 4, None, 0, 1, p, 4, p, 4, p, None, 0,
                                    None) == _lib.VCB_ERR_INVALID
+
+
+# Rows of every kernel: few rows, small products cut unevenly, copies of unaligned operands,
+# pairs with a short contraction, narrow gradients.
+VIEW_SIZES = [(1, 300, 1001), (2, 1025, 515), (4, 520, 2050), (6, 1001, 515), (8, 130, 100),
+              (16, 600, 500), (50, 33, 5), (900, 40, 70), (2314, 5, 10), (1500, 131, 300),
+              (700, 1200, 40)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,N,K', VIEW_SIZES)
+@pytest.mark.parametrize('first,pad', [(1, 0), (1, 3), (3, 8)])
+def test_rows_that_start_anywhere(M, N, K, first, pad, dtype):
+    """Operands are columns first.. of wider matrices, so that rows start on odd elements; the
+    neighbours are NaN and may not be read into any result."""
+    gen = torch.Generator(DEV).manual_seed(M + 7 * N + 31 * K + first)
+
+    def view(rows, cols, scale=1.0):
+        t = torch.full((rows, first + cols + pad), float('nan'), dtype=dtype, device=DEV)
+        t[:, first:first + cols] = rand(gen, rows, cols, dtype=dtype, scale=scale)
+        return t[:, first:first + cols]
+
+    x, w, r = view(M, K), view(N, K, K ** -0.5), view(M, N)
+    b = rand(gen, N + 1, dtype=dtype)[1:]
+    z = x.double() @ w.double().t() + b.double()
+    got, gz = linear.linear_forward(x, w, b, 'silu', r, keep=True)
+    close(got, act64(z, 'silu') + r.double(), dtype)
+    close(gz, z, dtype)
+    dy, zz = view(M, N), view(M, N)
+    dz = dy.double() * slope64(zz.double(), 'gelu')
+    dx, dw, db = linear.linear_backward(dy, x, w, zz, 'gelu')
+    close(dx, dz @ w.double(), dtype, 2)
+    close(dw, dz.t() @ x.double(), dtype, 2)
+    close(db, dz.sum(0), dtype, 2)
+    _lib.fault_check()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_calls_in_a_row_share_the_workspace(dtype):
+    """Each call prepares its operands in the memory that the call before it used: the product of
+    one has to be over before the preparation of the next, and after its own."""
+    gen = torch.Generator(DEV).manual_seed(11)
+    M, N, K = 520, 515, 513
+    xs = [rand(gen, M, K, dtype=dtype) for _ in range(4)]
+    w, dy = rand(gen, N, K, dtype=dtype, scale=K ** -0.5), rand(gen, M, N, dtype=dtype)
+    alone = []
+    for x in xs:
+        y, z = linear.linear_forward(x, w, None, 'gelu', keep=True)
+        alone.append((y, z, *linear.linear_backward(dy, x, w, z, 'gelu')))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        together = []
+        for x in xs:
+            y, z = linear.linear_forward(x, w, None, 'gelu', keep=True)
+            together.append((y, z, *linear.linear_backward(dy, x, w, z, 'gelu')))
+        torch.cuda.synchronize()
+        for got, want in zip(together, alone):
+            for g, t in zip(got, want):
+                assert torch.equal(g, t)
+    _lib.fault_check()
