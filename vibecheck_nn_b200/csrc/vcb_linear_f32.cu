@@ -29,6 +29,7 @@
 // f32_kernel<256, true> in CTA pairs for large ones, f32_kernel<64 / 128, false>
 // with the contraction cut over a cluster for the rest.
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <initializer_list>
 
@@ -700,6 +701,18 @@ struct Shape {
   int I, J, T;
 };
 
+// CTAs at a time in clusters of 1, 2, 4 and 8.
+int slots_of(int size) {
+  static const std::array<int, 4> slots = [] {
+    using C = Cfg<128, false>;
+    std::array<int, 4> n;
+    for (int k = 0; k < 4; ++k)
+      n[k] = cluster_slots(f32_kernel<128, false>, kF32Threads, C::kSmem, 1 << k);
+    return n;
+  }();
+  return slots[size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
+}
+
 Plan32 plan_of(std::initializer_list<Shape> products) {
   const int sms = sm_count();
   const auto ceil = [](long long a, long long b) { return (a + b - 1) / b; };
@@ -714,7 +727,7 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
     for (const Shape& s : products) tiles += ceil(s.I, bn) * ceil(s.J, kTileJ);
     for (int split : {1, 2, 4, 8}) {
       if (split > nk) break;
-      const double t = static_cast<double>(ceil(tiles * split, sms)) *
+      const double t = static_cast<double>(ceil(tiles * split, slots_of(split))) *
                            (ceil(nk, split) * (bn == 64 ? 800 : 1000) + 4000 + 20.0 * bn) +
                        (split > 1 ? 1500 + 8.0 * bn : 0);
       if (t < best.cycles) best = {false, bn, split, t};

@@ -34,6 +34,7 @@
 // word (vcb_fault_check), writes NaN to the tiles it has not finished, waits
 // for its copies and MMAs in flight, frees its tensor memory and returns.
 #include <algorithm>
+#include <array>
 #include <atomic>
 
 #include "vcb_linear_tc.cuh"
@@ -654,7 +655,18 @@ struct Plan {
   int bn, split;
 };
 
-// Cycles of a launch: rounds of tiles over the SMs times the longer of the MMAs
+// CTAs at a time in clusters of 1, 2, 4 and 8 (most of an SM's shared memory each).
+int slots_of(int size) {
+  static const std::array<int, 4> slots = [] {
+    std::array<int, 4> n;
+    for (int k = 0; k < 4; ++k)
+      n[k] = cluster_slots(split_kernel<__half>, kThreads, 200 << 10, 1 << k);
+    return n;
+  }();
+  return slots[size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
+}
+
+// Cycles of a launch: rounds of tiles over those places times the longer of the MMAs
 // (128 rows take 64 cycles per 16 of the contraction up to 128 columns, then
 // half a cycle a column; a pair's 256 x 256 takes 128) and the operands'
 // way from L2 (about 60 B per cycle and SM), plus a start and an epilogue.
@@ -670,7 +682,7 @@ Plan plan_of(int I, int J, int T, bool pair_possible, bool by64) {
     for (int split : {1, 2, 4, 8}) {
       if (split > nk) break;
       const double stage = std::max(4.0 * std::max(64, bn / 2), (kTileJ + bn) * 128 / 60.0);
-      const double rounds = static_cast<double>(ceil(tiles * split, sms));
+      const double rounds = static_cast<double>(ceil(tiles * split, slots_of(split)));
       const double t = rounds * (ceil(nk, split) * stage + 2500 + 12.0 * bn) +
                        (split > 1 ? 1500 + 6.0 * bn : 0);
       if (t < least) least = t, best = {false, bn, split};
@@ -725,7 +737,7 @@ int launch_tc(Launch& L, const Plan& plan, bool chained, cudaStream_t st, const 
   const long long clusters =
       L.units0 + (L.units - L.units0 + plan.split - 1LL) / plan.split;
   // two CTAs per SM overlap one's epilogue with the other's loads
-  const int room = clusters * plan.split > sm_count() ? 100 << 10 : 200 << 10;
+  const int room = clusters * plan.split > slots_of(plan.split) ? 100 << 10 : 200 << 10;
   L.stages = std::max(2, std::min({kMostStages, nk, room / stage}));
   L.split = plan.split;
   const int smem = std::max(L.stages * stage, plan.split > 1 ? bn * kTileJ * 4 : 0) + 1024;

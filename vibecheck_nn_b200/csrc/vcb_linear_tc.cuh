@@ -232,6 +232,30 @@ int launch_clusters(void (*kernel)(Args), const Args& args, dim3 grid, int threa
   return check_launch(who);
 }
 
+// CTAs of a kernel with one CTA per SM that run at the same time in clusters of `size`:
+// a cluster lies in one group of SMs, and the groups of a B200 hold 15 clusters of 8
+// rather than 148 / 8.  A sixteenth would run alone after them.
+template <typename Args>
+int cluster_slots(void (*kernel)(Args), int threads, int smem, int size) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (ensure_smem(reinterpret_cast<const void*>(kernel), smem) != VCB_OK ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+    cudaGetLastError();
+    clusters = sm_count() / size;
+  }
+  return clusters * size;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
