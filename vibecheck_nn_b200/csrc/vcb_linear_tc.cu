@@ -28,7 +28,7 @@
 // Measured: bf16 8192 x 8192 x 4096 with GELU, residual and pre-activation 350 us in
 // short bursts (1,570 TFLOP/s, 93 % of the library's measured rate), 465 us back to back
 // under the power cap (1,180); 4096^3 105 us; 2048 x 8192 x 1024 with the same epilogue
-// 64 us (epilogue-bound: 20 us of MMAs); both gradients at 2047 x 2050 x 1999 58 us, 25
+// 64 us (epilogue-bound: 20 us of MMAs); both gradients at 2047 x 2050 x 1999 57 us, 20
 // of them the preparation.
 // Every mbarrier wait is bounded: when one runs out the CTA raises the fault
 // word (vcb_fault_check), writes NaN to the tiles it has not finished, waits
