@@ -339,8 +339,10 @@ int backward(const Bwd& b, cudaStream_t st) {
   if (b.M == 1) return backward<T, 1, 4>(b, st);
   if (b.M == 2) return backward<T, 2, 4>(b, st);
   if (b.M <= 4) return backward<T, 4, 4>(b, st);
-  if (b.M <= 8) return backward<T, 8, 4>(b, st);
-  return backward<T, 16, 2>(b, st);
+  if constexpr (sizeof(T) == 4) {  // 16-bit types take the tensor cores from 9 rows on
+    if (b.M > 8) return backward<T, 16, 2>(b, st);
+  }
+  return backward<T, 8, 4>(b, st);
 }
 
 }  // namespace

@@ -452,7 +452,9 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // What a backward pass needs first: dz = dy act'(z) in rows that TMA can read,
-// db, and copies of operands whose rows TMA cannot read (not 16-byte aligned).
+// db, and copies of operands whose rows TMA cannot read (not 16-byte aligned).  dz is
+// rounded to the operands' type, which a tensor-core operand has to have; db sums the
+// values before that.
 struct Copy {
   const void* src;
   void* dst;
