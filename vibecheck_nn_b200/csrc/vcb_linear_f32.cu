@@ -57,31 +57,31 @@ __device__ __forceinline__ float scaled(float v, int e) {
   return v * exp2i(h) * exp2i(e - h);
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float x) {
-  return __float_as_uint(x) & 0x7FFFFFFFu;
-}
+// Larger |entry|, NaN left aside: it needs no scale.
+__device__ __forceinline__ float more(float m, float x) { return fmaxf(m, fabsf(x)); }
 
-// Larger |entry| as bits, NaN left aside: it needs no scale.
-__device__ __forceinline__ uint32_t more(uint32_t m, float x) {
-  const uint32_t b = abs_bits(x);
-  return b > 0x7F800000u ? m : max(m, b);
-}
-
-__device__ __forceinline__ void halves(float x, float scale, __half& h, __half& l) {
-  const float t = x * scale;
-  h = __float2half_rn(t);
-  const float back = __half2float(h);
-  // an infinite h has no remainder
-  l = isinf(back) ? __float2half_rn(0.f) : __float2half_rn(t - back);
+__device__ __forceinline__ void halves4(const float (&x)[4], const float (&scale)[4], uint2& high,
+                                        uint2& low) {
+  __half2 h[2], l[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float a = x[2 * k] * scale[2 * k], b = x[2 * k + 1] * scale[2 * k + 1];
+    h[k] = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(h[k]);
+    // an infinite h has no remainder
+    l[k] = __floats2half2_rn(isinf(back.x) ? 0.f : a - back.x, isinf(back.y) ? 0.f : b - back.y);
+  }
+  high = *reinterpret_cast<const uint2*>(h);
+  low = *reinterpret_cast<const uint2*>(l);
 }
 
 __device__ __forceinline__ void put_halves(__half* h, long long plane, const float (&v)[4],
                                            float scale) {
-  __half a[4], b[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) halves(v[k], scale, a[k], b[k]);
-  *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(a);
-  *reinterpret_cast<uint2*>(h + plane) = *reinterpret_cast<const uint2*>(b);
+  const float all[4] = {scale, scale, scale, scale};
+  uint2 high, low;
+  halves4(v, all, high, low);
+  *reinterpret_cast<uint2*>(h) = high;
+  *reinterpret_cast<uint2*>(h + plane) = low;
 }
 
 // Four entries of a row from column c; 0 beyond the last.
@@ -108,9 +108,9 @@ struct RowJobs {
   RowJob j[2];
 };
 
-template <int TPR>  // threads per row
+// TPR threads per row, of which KEEP vectors per thread stay in registers.
+template <int TPR, int KEEP>
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJobs a) {
-  constexpr int kKeep = 4;  // vectors of a row that stay in registers
   __shared__ uint32_t warp_most[8];
   let_next_start();
   long long r = static_cast<long long>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
@@ -120,40 +120,40 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJo
   if (second) r -= a.j[0].rows;
   const bool row = r < q.rows;  // uniform over the threads of a row
   const float* src = q.src + r * q.ld;
-  float v[kKeep][4];
-  uint32_t m = 0;
+  float v[KEEP][4];
+  float most = 0.f;
   if (row) {
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-      const int c = (k * TPR + t) * 4;
-      row4(src, c, q.cols, q.vec, v[k]);
+    for (int k = 0; k < KEEP; ++k) row4(src, (k * TPR + t) * 4, q.cols, q.vec, v[k]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = more(m, v[k][i]);
+    for (int k = 0; k < KEEP; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = more(most, v[k][i]);
     }
-    for (int c = (kKeep * TPR + t) * 4; c < q.cols; c += TPR * 4) {
+    for (int c = (KEEP * TPR + t) * 4; c < q.cols; c += TPR * 4) {
       float w[4];
       row4(src, c, q.cols, q.vec, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = more(m, w[i]);
+      for (int i = 0; i < 4; ++i) most = more(most, w[i]);
     }
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
   if (TPR > 32) {
     if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, warp_most[w]);
+    for (int w = 0; w < TPR / 32; ++w) m = max(m, warp_most[threadIdx.x / TPR * (TPR / 32) + w]);
   }
   if (!row) return;
   if (t == 0) q.most[r] = m;
   const float scale = exp2i(-scale_exp(m));
   __half* h = q.h + r * q.ldh;
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k) {
+  for (int k = 0; k < KEEP; ++k) {
     const int c = (k * TPR + t) * 4;
     if (c < q.cols) put_halves(h + c, q.plane, v[k], scale);
   }
-  for (int c = (kKeep * TPR + t) * 4; c < q.cols; c += TPR * 4) {
+  for (int c = (KEEP * TPR + t) * 4; c < q.cols; c += TPR * 4) {
     float w[4];
     row4(src, c, q.cols, q.vec, w);
     put_halves(h + c, q.plane, w, scale);
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kStripThreads, 4)
   const int c = strip * 32 + (lane & 7) * 4;
   const long long r0 = q.rows * rank / size, r1 = q.rows * (rank + 1) / size;
   float sum[4] = {};
-  uint32_t most[4] = {};
+  float most[4] = {};
   constexpr int U = 4, W = kStripWarps * 4;  // rows in flight per lane, rows of a CTA's step
   for (long long base = r0 + warp * 4; base < r1; base += U * W) {
     float v[U][4];
@@ -236,14 +236,15 @@ __global__ void __launch_bounds__(kStripThreads, 4)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long r = base + u * W + (lane >> 3);
-      uint32_t m = 0;
+      float top = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         most[i] = more(most[i], v[u][i]);
         sum[i] += v[u][i];
-        m = more(m, v[u][i]);
+        top = more(top, v[u][i]);
       }
       if (q.row_most) {
+        uint32_t m = __float_as_uint(top);
 #pragma unroll
         for (int k = 4; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
         if ((lane & 7) == 0 && r < r1) atomicMax(q.row_most + r, m);
@@ -255,11 +256,11 @@ __global__ void __launch_bounds__(kStripThreads, 4)
 #pragma unroll
     for (int k = 8; k < 32; k *= 2) {
       sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
-      most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], k));
+      most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], k));
     }
     if (lane < 8) {
       part[warp][lane * 4 + i] = sum[i];
-      most_part[warp][lane * 4 + i] = most[i];
+      most_part[warp][lane * 4 + i] = __float_as_uint(most[i]);
     }
   }
   __syncthreads();
@@ -313,12 +314,11 @@ __global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_cons
     if (q.by_row)
       put_halves(q.by_row + r * q.ldh + c, q.plane, v[u], exp2i(-scale_exp(q.row_most[r])));
     if (q.by_col) {
-      __half h[4], l[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) halves(v[u][i], scale[i], h[i], l[i]);
+      uint2 high, low;
+      halves4(v[u], scale, high, low);
       __half* at = q.by_col + r * q.ldh + c;
-      *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(h);
-      *reinterpret_cast<uint2*>(at + q.plane) = *reinterpret_cast<const uint2*>(l);
+      *reinterpret_cast<uint2*>(at) = high;
+      *reinterpret_cast<uint2*>(at + q.plane) = low;
     }
   }
 }
@@ -804,11 +804,17 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
   jobs.j[0] = job(f.w, f.ldw, w);
   jobs.j[1] = job(f.x, f.ldx, x);
   const long long rows = static_cast<long long>(f.N) + f.M;
-  // a warp per row while that keeps a row in registers, else a CTA
+  // a warp per row while that keeps a row in registers: what a thread does once is spread
+  // over more entries (1000^3 27.6 -> 25.6 us against a CTA per row)
+  const auto launch_rows = [&](void (*kernel)(RowJobs), int per) {
+    kernel<<<static_cast<unsigned>((rows + per - 1) / per), 256, 0, st>>>(jobs);
+  };
   if (f.K <= 512)
-    rows_kernel<32><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(jobs);
+    launch_rows(rows_kernel<32, 4>, 8);
+  else if (f.K <= 2048)
+    launch_rows(rows_kernel<32, 16>, 8);
   else
-    rows_kernel<256><<<static_cast<unsigned>(rows), 256, 0, st>>>(jobs);
+    launch_rows(rows_kernel<256, 4>, 1);
   int rc = check_launch(who);
   if (rc) return rc;
   const Plan32 plan = plan_of({{f.M, f.N, f.K}});
