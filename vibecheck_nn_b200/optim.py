@@ -13,7 +13,10 @@ finite makes its block of 256 moments NaN.
 
 Weights are updated in place, in float32 arithmetic, rounded once to their own
 type (float32, bfloat16, float16: in 16 bits a step below half a unit in the
-last place is lost); gradients have the weights' type or float32.
+last place is lost); gradients have the weights' type or float32.  A parameter
+keeps the type, shape, device and contiguous layout that it had when the optimiser
+was built; a step refuses (``ValueError``) one that a conversion of its module
+has changed.
 """
 from __future__ import annotations
 
@@ -47,6 +50,7 @@ class AdamW:
         self._types = [type_of(p, f'parameter {i}') for i, p in enumerate(self.params)]
         self._one_type = len(set(self._types)) == 1
         self._shapes = [p.shape for p in self.params]
+        self._dtypes = [p.dtype for p in self.params]
         self._sizes, self.offsets, total = [], [], 0
         for i, p in enumerate(self.params):
             if p.device != self.device or not p.is_contiguous():
@@ -79,6 +83,7 @@ class AdamW:
         grads = [p.grad for p in ps] if grads is None else list(grads)
         if len(grads) != len(ps):
             raise ValueError(f'{len(grads)} gradients for {len(ps)} parameters')
+        self._check_params()
         groups = self._groups(grads)
         self.t += 1
         opts = self._opts()
@@ -101,13 +106,30 @@ class AdamW:
                 _lib.check(rc, 'vcb_adamw')
         torch.autograd.graph.increment_version(ps)
 
+    def _check_params(self):
+        """A parameter keeps its identity when a module is converted or moved
+        (its ``data`` is replaced): what the state was laid out for must still
+        hold before a pointer is taken."""
+        here = self.device.index
+        if [p.dtype for p in self.params] == self._dtypes \
+                and [p.shape for p in self.params] == self._shapes \
+                and all([p.get_device() == here and p.is_contiguous() for p in self.params]):
+            return
+        for i, p in enumerate(self.params):
+            if p.dtype != self._dtypes[i] or p.shape != self._shapes[i] \
+                    or p.get_device() != here or not p.is_contiguous():
+                raise ValueError(f'parameter {i}: {p.dtype} {tuple(p.shape)} strides {p.stride()} on '
+                                 f'{p.device}, contiguous {self._dtypes[i]} '
+                                 f'{tuple(self._shapes[i])} on {self.device} when this optimiser '
+                                 'was built')
+
     def _groups(self, grads):
         """[(weights' type, gradients' type, indices, gradient pointers)], one
         entry per launch."""
         here = self.device.index
         if not any([g is None for g in grads]):  # usually one type, and nothing to copy
             first = grads[0].dtype
-            if self._one_type and (first == torch.float32 or first == self.params[0].dtype) \
+            if self._one_type and (first == torch.float32 or first == self._dtypes[0]) \
                     and [g.shape for g in grads] == self._shapes \
                     and all([g.dtype is first and g.get_device() == here and g.is_contiguous()
                              for g in grads]):
@@ -125,7 +147,7 @@ class AdamW:
             key = (self._types[i], g.dtype)
             group = groups.get(key)
             if group is None:
-                if g.dtype != torch.float32 and g.dtype != self.params[i].dtype:
+                if g.dtype != torch.float32 and g.dtype != self._dtypes[i]:
                     raise _lib.UnsupportedInput(f'vibecheck_nn_b200: gradient {i} of type '
                                                 f'{g.dtype}; the weight\'s or float32')
                 group = groups[key] = (key[0], TYPES[g.dtype], [], [])
