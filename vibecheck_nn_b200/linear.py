@@ -5,7 +5,7 @@ that is trained here and bounded by the rest of the package.
   ``keep`` also the pre-activation ``z = x W^T + b`` for the backward pass;
 * ``linear_backward`` -- ``dz = dy * act'(z)``, ``dx = dz W``, ``dW = dz^T x``
   and ``db``;
-* ``linear`` -- the same as a differentiable function.
+* ``linear`` -- the same for autograd, differentiable once.
 
 ``x`` is (..., K), ``weight`` (N, K) as in a ``gg`` dict's fc layer.  float32,
 bfloat16 and float16, one type per call; sums are held in float32 and each
@@ -163,6 +163,29 @@ def _p(t):
     return 0 if t is None else t.data_ptr()
 
 
+class _Refuse(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, anchor, what, *outs):
+        ctx.what = what
+        return outs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f'vibecheck_nn_b200: {ctx.what} is differentiable once (its gradients '
+                           'come from kernels that autograd does not see)')
+
+
+def first_order(what, outs):
+    """Gradients ``outs`` (tensors or None) of ``what``: where a graph of the
+    backward pass is asked for, a second derivative through them raises instead of
+    missing its terms."""
+    if not torch.is_grad_enabled():
+        return outs
+    anchor = torch.zeros((), requires_grad=True)
+    made = iter(_Refuse.apply(anchor, what, *[t for t in outs if t is not None]))
+    return tuple(None if t is None else next(made) for t in outs)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
@@ -179,11 +202,13 @@ class _Linear(torch.autograd.Function):
         gx, gw, gb = ctx.needs_input_grad[:3]
         dx = dw = db = None
         if gx or gw or gb:
-            dx, dw, db = linear_backward(dy, x, weight, z, ctx.act, gb, (gx, gw))
+            with torch.no_grad():
+                outs = linear_backward(dy, x, weight, z, ctx.act, gb, (gx, gw))
+            dx, dw, db = first_order('linear', outs)
         return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None
 
 
 def linear(x, weight, bias=None, act='none', residual=None):
-    """Differentiable ``linear_forward`` (gradients of x, weight, bias and
-    residual)."""
+    """``linear_forward``, differentiable once (gradients of x, weight, bias and
+    residual; a second derivative through them raises ``RuntimeError``)."""
     return _Linear.apply(x, weight, bias, act, residual)

@@ -1,7 +1,7 @@
 """Softmax cross-entropy with its gradient in one pass over the logits.
 
 * ``cross_entropy_grad`` -- (loss, dlogits) of the mean over labelled rows;
-* ``cross_entropy`` -- the same loss as a differentiable function.
+* ``cross_entropy`` -- the same loss for autograd, differentiable once.
 
 Logits (..., C) in float32, bfloat16 or float16, int64 labels (...).  Rows
 labelled ``ignore_index`` count for nothing and get gradient 0; with no
@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _lib
-from .linear import _p, _workspace_bytes, rows_of, type_of
+from .linear import _p, _workspace_bytes, first_order, rows_of, type_of
 
 _ARGS = struct.Struct('13q').pack
 
@@ -58,9 +58,12 @@ class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         grad, = ctx.saved_tensors
-        return (grad * g).to(grad.dtype), None, None
+        with torch.no_grad():
+            out = (grad * g).to(grad.dtype)
+        return (*first_order('cross_entropy', (out,)), None, None)
 
 
 def cross_entropy(logits, labels, ignore_index=-100):
-    """Differentiable mean cross-entropy over the labelled rows."""
+    """Mean cross-entropy over the labelled rows, differentiable once (a second
+    derivative through its gradient raises ``RuntimeError``)."""
     return _CrossEntropy.apply(logits, labels, ignore_index)
