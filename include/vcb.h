@@ -718,7 +718,8 @@ size_t vcb_cross_entropy_workspace(int32_t R, int32_t C);
 
 /* vcb_linear_forward, vcb_linear_backward and vcb_cross_entropy with their
  * arguments, in order, as consecutive 64-bit integers (sizes, pointers, the
- * stream): for bindings that pay for every argument they convert. */
+ * stream): for bindings that pay for every argument they convert.  A size that
+ * 32 bits do not hold is refused (VCB_ERR_UNSUPPORTED). */
 int vcb_linear_forward_packed(const int64_t* args);
 int vcb_linear_backward_packed(const int64_t* args);
 int vcb_cross_entropy_packed(const int64_t* args);

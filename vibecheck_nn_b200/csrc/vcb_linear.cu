@@ -20,6 +20,7 @@
 // db, 16 us (its bytes take 0.4 us: what is left are the launch, two trips to memory
 // in turn and the cluster's join), bf16 2000 x 63 x 63 forward 11 us.
 #include <algorithm>
+#include <initializer_list>
 
 #include "vcb_linear_tc.cuh"
 
@@ -449,8 +450,20 @@ static T* at(int64_t v) {
   return reinterpret_cast<T*>(static_cast<uintptr_t>(v));
 }
 
+// Those of the arguments `which` that the entry points take in 32 bits do fit.
+static bool in_32_bits(const int64_t* a, std::initializer_list<int> which) {
+  for (const int k : which)
+    if (a[k] != static_cast<int32_t>(a[k])) return false;
+  return true;
+}
+
+static int too_large(const char* who) {
+  return fail(VCB_ERR_UNSUPPORTED, "%s: a size or code that 32 bits do not hold", who);
+}
+
 extern "C" int vcb_linear_forward_packed(const int64_t* a) {
   if (!a) return fail(VCB_ERR_INVALID, "vcb_linear_forward_packed: NULL");
+  if (!in_32_bits(a, {0, 1, 2, 3, 9})) return too_large("vcb_linear_forward_packed");
   const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
   return vcb_linear_forward(i(0), i(1), i(2), i(3), at(a[4]), a[5], at(a[6]), a[7], at(a[8]), i(9),
                             at(a[10]), a[11], at(a[12]), a[13], at(a[14]), a[15], at(a[16]),
@@ -459,6 +472,7 @@ extern "C" int vcb_linear_forward_packed(const int64_t* a) {
 
 extern "C" int vcb_linear_backward_packed(const int64_t* a) {
   if (!a) return fail(VCB_ERR_INVALID, "vcb_linear_backward_packed: NULL");
+  if (!in_32_bits(a, {0, 1, 2, 3, 12})) return too_large("vcb_linear_backward_packed");
   const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
   return vcb_linear_backward(i(0), i(1), i(2), i(3), at(a[4]), a[5], at(a[6]), a[7], at(a[8]), a[9],
                              at(a[10]), a[11], i(12), at(a[13]), a[14], at(a[15]), a[16],
@@ -467,6 +481,7 @@ extern "C" int vcb_linear_backward_packed(const int64_t* a) {
 
 extern "C" int vcb_cross_entropy_packed(const int64_t* a) {
   if (!a) return fail(VCB_ERR_INVALID, "vcb_cross_entropy_packed: NULL");
+  if (!in_32_bits(a, {0, 1, 2})) return too_large("vcb_cross_entropy_packed");
   const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
   return vcb_cross_entropy(i(0), i(1), i(2), at(a[3]), a[4], at<const int64_t>(a[5]), a[6],
                            at<float>(a[7]), at(a[8]), a[9], at(a[10]), static_cast<size_t>(a[11]),

@@ -49,6 +49,9 @@ def rows_of(t, cols, like, name):
     dim = t.dim()
     if dim < 1 or t.shape[-1] != cols:
         raise ValueError(f'{name}: shape {tuple(t.shape)}, expected (..., {cols})')
+    if ((t.shape[0] if dim == 2 else t.shape[:-1].numel()) | cols) >> 31:
+        raise _lib.UnsupportedInput(f'vibecheck_nn_b200: {name} {tuple(t.shape)}: rows and columns '
+                                    'are counted in 32 bits')
     if dim == 2 and t.is_contiguous():
         return t, cols
     if dim != 2:
