@@ -177,6 +177,7 @@ struct ColJobs {
   ColJob j[3];
   int count;
   int cluster;  // CTAs per strip of scales_kernel
+  int wide;     // strips of halves_kernel, for each block of rows
 };
 
 constexpr int kStripThreads = 256, kStripWarps = kStripThreads / 32;
@@ -295,16 +296,17 @@ __global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_cons
   after_previous();
   let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int strip = blockIdx.x;
+  const int block = blockIdx.x / a.wide;
+  int strip = blockIdx.x % a.wide;
   const ColJob& q = strip_of(a, strip, 128);
   const int c = strip * 128 + lane * 4;
   if (c >= q.cols) return;
   float scale[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) scale[i] = c + i < q.cols ? exp2i(-scale_exp(q.col_most[c + i])) : 0.f;
-  const long long end = min(q.rows, (blockIdx.y + 1LL) * kHalvesRows);
+  const long long end = min(q.rows, (block + 1LL) * kHalvesRows);
   constexpr int U = kHalvesRows / kStripWarps;  // rows of a warp
-  const long long r0 = static_cast<long long>(blockIdx.y) * kHalvesRows + warp;
+  const long long r0 = static_cast<long long>(block) * kHalvesRows + warp;
   float v[U][4];
   job_rows<U>(q, r0, kStripWarps, end, c, v);
 #pragma unroll
@@ -865,7 +867,8 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (!b.dw) dz.by_col = nullptr;
   if (b.dx) add(b.w, b.ldw, w);
   if (b.dw) add(b.x, b.ldx, x);
-  if (strips * 8 > 0x7fffffffLL || (tall + kHalvesRows - 1) / kHalvesRows > 65535)
+  const long long blocks = (tall + kHalvesRows - 1) / kHalvesRows;
+  if (strips * 8 > 0x7fffffffLL || wide * blocks > 0x7fffffffLL)
     return fail(VCB_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d", who, b.M, b.N, b.K);
   cudaError_t e = cudaSuccess;
   if (b.dx) e = cudaMemsetAsync(row_most, 0, b.M * 4LL, st);
@@ -875,9 +878,9 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   int rc = launch_clusters(scales_kernel, jobs, static_cast<unsigned>(strips * jobs.cluster),
                            kStripThreads, 0, jobs.cluster, false, st, who);
   if (rc) return rc;
-  const auto blocks = static_cast<unsigned>((tall + kHalvesRows - 1) / kHalvesRows);
-  rc = launch_clusters(halves_kernel, jobs, dim3(static_cast<unsigned>(wide), blocks),
-                       kStripThreads, 0, 1, true, st, who);
+  jobs.wide = static_cast<int>(wide);
+  rc = launch_clusters(halves_kernel, jobs, static_cast<unsigned>(wide * blocks), kStripThreads, 0,
+                       1, true, st, who);
   if (rc) return rc;
   const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
   const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
