@@ -1,33 +1,35 @@
 // The linear layer's float32 products on the tensor cores.
 //
-// A float32 operand row is scaled by a power of two, so that its largest entry
-// lies in [2^14, 2^15), and split in two half-precision numbers,
-//   x 2^-e = h + l + d,  h = fp16(x 2^-e),  l = fp16(x 2^-e - h),
-// |d| <= 2^-22 |x| 2^-e (and 2^-40 of the row's largest where l is subnormal).
-// The tensor cores form  h h' + h l' + l h'  with exact products and fp32
-// accumulators; l l' is below 2^-22 of the product and left out.  That is the
-// precision of three TF32 products at twice their rate: fp16 multiplies twice as
-// fast as TF32 and has as many significant bits, and the row scales supply the
-// exponents that it lacks.  A scale belongs to a row along which nothing is
-// summed (a row of the output, or a column of it), so it leaves the product as a
-// factor 2^(e + e').  An infinite or NaN entry makes the outputs of its row
-// infinite or NaN.
+// A float32 number is the sum of three bfloat16 numbers,
+//   b1 = bf16(x),  b2 = bf16(x - b1),  b3 = x - b1 - b2,
+// exactly (24 bits in three times 8) while |x| >= 2^-110; below that b3, then b2,
+// end at bfloat16's smallest step, 2^-133.  Each has float32's exponents, so
+// entries of any size share a row.  The tensor cores form
+//   b1 b1' + (b1 b2' + b2 b1') + (b2 b2' + b1 b3' + b3 b1')
+// with exact products and fp32 accumulators.  b2 b3' + b3 b2' + b3 b3' are left out:
+// below 2^-24 |x x'|, what rounding one product to float32 may lose.  So an output's
+// error is bounded by its own sum of |x x'|, as that of a float32 sum is, whatever
+// else lies in the rows.  (Two fp16 halves under one scale per row took three products
+// instead of six, but their error went by the row's largest entry: a column at 2^30
+// that met zero weights cost the other columns three digits.)  An infinite or NaN
+// entry makes the outputs that it meets infinite or NaN: its products with b2' and
+// b3', which may be 0, are formed too.
 //
 // The tensor cores drop low-order bits in every accumulation.  So an accumulator
-// in tensor memory takes one 64-deep stage (12 MMAs) only, and the epilogue warps
-// add the stages' sums in registers, rounding to nearest, while the next stage
-// fills the other accumulator.
+// in tensor memory takes one 64-deep stage (24 MMAs) only, the smaller products
+// first, and the epilogue warps add the stages' sums in registers, rounding to
+// nearest, while the next stage fills the other accumulator.
 //
-// Measured: 4096^3 forward 355 us in short bursts (387 TFLOP/s of fp32 products, 1,160
-// of fp16), 424 us back to back under the power cap, both gradients 750 us; largest
-// error 3e-7 of the largest output, against 1.1e-6 of an fp32 sum.
+// Measured: 4096^3 forward 605 us in short bursts (227 TFLOP/s of fp32 products, 1,360
+// of bfloat16), 680 us back to back under the power cap, both gradients 1,065 us;
+// largest error 1.7e-7 of the largest output, against 1.1e-6 of an fp32 sum.
 //
-// Preparation is bound by HBM: forward, one launch reads each row once, finds its
-// scale and writes both halves.  Backward, dz needs row scales for dX and column
-// scales for dW, so a first launch finds all scales (and db, and never stores
-// dz), a second writes the halves.  Then products as in vcb_linear_tc.cu:
-// f32_kernel<256, true> in CTA pairs for large ones, f32_kernel<64 / 128, false>
-// with the contraction cut over a cluster for the rest.
+// Preparation is bound by HBM: one launch reads each operand once and writes its
+// three parts (backward: dz = dy act'(z) and db in strips of columns, W and X flat
+// beside them).  The parts of dz serve both products, read along either index.
+// Then products as in vcb_linear_tc.cu: f32_kernel<256, true> in CTA pairs for
+// large ones, f32_kernel<64 / 128, false> with the contraction cut over a cluster
+// for the rest.
 #include <algorithm>
 #include <array>
 #include <atomic>
@@ -42,46 +44,34 @@ namespace {
 __device__ int g_f32_fault;
 std::atomic<bool> g_launched{false};
 
-// Exponent e of the scale 2^-e for a row whose largest |entry| has these bits.
-__device__ __forceinline__ int scale_exp(uint32_t bits) {
-  const int b = static_cast<int>(bits >> 23);
-  if (bits == 0 || b >= 255) return 0;  // all zero, or not finite
-  return max(b - 127 - 14, -126);
-}
+constexpr int kParts = 3;
+constexpr uint32_t kLargest16 = 0x7F7F0000u;  // of bfloat16, as a float's bits
 
-__device__ __forceinline__ float exp2i(int k) { return __int_as_float((k + 127) << 23); }
-
-// v 2^e for the sum e of two scale_exp(): in two steps, each in range.
-__device__ __forceinline__ float scaled(float v, int e) {
-  const int h = e >> 1;
-  return v * exp2i(h) * exp2i(e - h);
-}
-
-// Larger |entry|, NaN left aside: it needs no scale.
-__device__ __forceinline__ float more(float m, float x) { return fmaxf(m, fabsf(x)); }
-
-__device__ __forceinline__ void halves4(const float (&x)[4], const float (&scale)[4], uint2& high,
-                                        uint2& low) {
-  __half2 h[2], l[2];
+// The parts of four entries.  What would round up to infinity is cut instead; an
+// infinite entry has no remainder.
+__device__ __forceinline__ void split4(const float (&x)[4], uint2 (&part)[kParts]) {
+  uint32_t w[kParts][2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float a = x[2 * k] * scale[2 * k], b = x[2 * k + 1] * scale[2 * k + 1];
-    h[k] = __floats2half2_rn(a, b);
-    const float2 back = __half22float2(h[k]);
-    // an infinite h has no remainder
-    l[k] = __floats2half2_rn(isinf(back.x) ? 0.f : a - back.x, isinf(back.y) ? 0.f : b - back.y);
+    float r[2] = {x[2 * k], x[2 * k + 1]}, top[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t bits = __float_as_uint(r[i]), size = bits & 0x7FFFFFFFu;
+      top[i] = size > kLargest16 && size < 0x7F800000u
+                   ? __uint_as_float(kLargest16 | (bits & 0x80000000u)) : r[i];
+    }
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const __nv_bfloat162 h =
+          p ? __floats2bfloat162_rn(r[0], r[1]) : __floats2bfloat162_rn(top[0], top[1]);
+      const uint32_t u = w[p][k] = *reinterpret_cast<const uint32_t*>(&h);
+      const float back[2] = {__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) r[i] = isinf(back[i]) ? 0.f : r[i] - back[i];
+    }
   }
-  high = *reinterpret_cast<const uint2*>(h);
-  low = *reinterpret_cast<const uint2*>(l);
-}
-
-__device__ __forceinline__ void put_halves(__half* h, long long plane, const float (&v)[4],
-                                           float scale) {
-  const float all[4] = {scale, scale, scale, scale};
-  uint2 high, low;
-  halves4(v, all, high, low);
-  *reinterpret_cast<uint2*>(h) = high;
-  *reinterpret_cast<uint2*>(h + plane) = low;
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) part[p] = make_uint2(w[p][0], w[p][1]);
 }
 
 // Four entries of a row from column c; 0 beyond the last.
@@ -94,243 +84,135 @@ __device__ __forceinline__ void row4(const float* row, int c, int cols, bool vec
   }
 }
 
-// ---- preparation, forward: halves of the rows of two matrices ----
-struct RowJob {
+// ---- preparation ----
+// A row-major matrix and its parts: `plane` elements apart, rows of ldp (a multiple of
+// 8) elements.
+struct Matrix {
   const float* src;
   long long ld, rows;
   int cols, vec;
-  __half* h;        // rows x ldh, the second halves `plane` elements further
-  long long ldh, plane;
-  uint32_t* most;   // bits of the largest |entry| of each row
+  __nv_bfloat16* parts;
+  long long ldp, plane;
 };
 
-struct RowJobs {
-  RowJob j[2];
+struct Prep32 {
+  Matrix dz;              // in strips of columns (backward); its src is dy
+  const float* z;
+  float* sum;             // column sums of dz (db), or NULL
+  long long ldz;
+  int act, strips;        // strips of 32 columns, 0 for none
+  int cluster;            // CTAs per strip
+  Matrix flat[2];
+  int flats;
 };
 
-// TPR threads per row, of which KEEP vectors per thread stay in registers.
-template <int TPR, int KEEP>
-__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowJobs a) {
-  __shared__ uint32_t warp_most[8];
+constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32, kStrip = 32;
+
+// Strips: a cluster of up to 8 CTAs each, a part of the rows per CTA, 8 lanes per
+// row; column sums in the order of the ranks.  The remaining CTAs: 8 entries per
+// thread, neighbouring threads on neighbouring entries of all rows.
+__global__ void __launch_bounds__(kPrepThreads, 4) parts_kernel(const __grid_constant__ Prep32 a) {
+  __shared__ float part[kPrepWarps][kStrip], mine[kStrip];
   let_next_start();
-  long long r = static_cast<long long>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
-  const int t = threadIdx.x % TPR;
-  const bool second = r >= a.j[0].rows;
-  const RowJob& q = a.j[second];
-  if (second) r -= a.j[0].rows;
-  const bool row = r < q.rows;  // uniform over the threads of a row
-  const float* src = q.src + r * q.ld;
-  float v[KEEP][4];
-  float most = 0.f;
-  if (row) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int size = a.cluster, strip = blockIdx.x / size;
+  if (strip < a.strips) {
+    const Matrix& q = a.dz;
+    const int rank = blockIdx.x % size, c = strip * kStrip + (lane & 7) * 4;
+    const long long r0 = q.rows * rank / size, r1 = q.rows * (rank + 1) / size;
+    float sum[4] = {};
+    constexpr int U = 4, W = kPrepWarps * 4;  // rows in flight per lane, rows of a CTA's step
+    for (long long base = r0 + warp * 4 + (lane >> 3); base < r1; base += U * W) {
+      float v[U][4], t[U][4];
 #pragma unroll
-    for (int k = 0; k < KEEP; ++k) row4(src, (k * TPR + t) * 4, q.cols, q.vec, v[k]);
+      for (int u = 0; u < U; ++u) {
+        const long long r = base + u * W;
+        if (r >= r1) continue;
+        row4(q.src + r * q.ld, c, q.cols, q.vec, v[u]);
+        if (a.act != VCB_ACT_NONE) row4(a.z + r * a.ldz, c, q.cols, q.vec, t[u]);
+      }
 #pragma unroll
-    for (int k = 0; k < KEEP; ++k) {
+      for (int u = 0; u < U; ++u) {
+        const long long r = base + u * W;
+        if (r >= r1) continue;
+        if (a.act != VCB_ACT_NONE) act_grads(v[u], t[u], a.act);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most = more(most, v[k][i]);
+        for (int i = 0; i < 4; ++i) sum[i] += v[u][i];
+        if (c < q.cols) {
+          uint2 p[kParts];
+          split4(v[u], p);
+          __nv_bfloat16* at = q.parts + r * q.ldp + c;
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) *reinterpret_cast<uint2*>(at + k * q.plane) = p[k];
+        }
+      }
     }
-    for (int c = (KEEP * TPR + t) * 4; c < q.cols; c += TPR * 4) {
-      float w[4];
-      row4(src, c, q.cols, q.vec, w);
+    if (!a.sum) return;  // the same for all CTAs
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most = more(most, w[i]);
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int k = 8; k < 32; k *= 2) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
+      if (lane < 8) part[warp][lane * 4 + i] = sum[i];
     }
-  }
-  uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-  if (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) m = max(m, warp_most[threadIdx.x / TPR * (TPR / 32) + w]);
+    if (threadIdx.x < kStrip) {
+      float s = 0.f;
+      for (int w = 0; w < kPrepWarps; ++w) s += part[w][threadIdx.x];
+      mine[threadIdx.x] = s;
+    }
+    cluster_sync();
+    const int col = strip * kStrip + threadIdx.x;
+    if (rank == 0 && threadIdx.x < kStrip && col < q.cols) {
+      float s = 0.f;
+      for (int k = 0; k < size; ++k) s += peer_f32(map_rank(smem_u32(mine + threadIdx.x), k));
+      a.sum[col] = s;
+    }
+    cluster_sync();  // no CTA leaves while its sums are read
+    return;
   }
-  if (!row) return;
-  if (t == 0) q.most[r] = m;
-  const float scale = exp2i(-scale_exp(m));
-  __half* h = q.h + r * q.ldh;
+  const long long first = (long long)(blockIdx.x - a.strips * size) * kPrepThreads + threadIdx.x;
+  const long long step = (long long)(gridDim.x - a.strips * size) * kPrepThreads;
+  for (int m = 0; m < a.flats; ++m) {
+    const Matrix& q = a.flat[m];
+    const int nv = (q.cols + 7) / 8;
+    long long row = first / nv;
+    int v = static_cast<int>(first - row * nv);
+    const long long down = step / nv;
+    const int right = static_cast<int>(step - down * nv);
+    constexpr int U = 2;  // vectors of 8 in flight
+    while (row < q.rows) {
+      float x[U][2][4];
+      __nv_bfloat16* out[U];
 #pragma unroll
-  for (int k = 0; k < KEEP; ++k) {
-    const int c = (k * TPR + t) * 4;
-    if (c < q.cols) put_halves(h + c, q.plane, v[k], scale);
-  }
-  for (int c = (KEEP * TPR + t) * 4; c < q.cols; c += TPR * 4) {
-    float w[4];
-    row4(src, c, q.cols, q.vec, w);
-    put_halves(h + c, q.plane, w, scale);
-  }
-}
-
-// ---- preparation, backward ----
-// A matrix in strips of columns, 4 columns per lane; with z the entries are dz = dy
-// act'(z).
-struct ColJob {
-  const float *src, *z;
-  long long ld, ldz, rows;
-  int cols, vec, act;
-  uint32_t *col_most, *row_most;  // row_most may be NULL; zero on entry
-  float* sum;                     // column sums, or NULL
-  __half *by_col, *by_row;        // halves with column scales; with row scales, or NULL
-  long long ldh, plane;
-};
-
-struct ColJobs {
-  ColJob j[3];
-  int count;
-  int cluster;  // CTAs per strip of scales_kernel
-  int wide;     // strips of halves_kernel, for each block of rows
-};
-
-constexpr int kStripThreads = 256, kStripWarps = kStripThreads / 32;
-
-// Entries of N rows from r, `step` rows apart; 0 from row `end` on.  All loads come
-// before the first use.
-template <int N>
-__device__ __forceinline__ void job_rows(const ColJob& q, long long r, long long step,
-                                         long long end, int c, float (&v)[N][4]) {
-  float t[N][4];
-#pragma unroll
-  for (int u = 0; u < N; ++u) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[u][k] = t[u][k] = 0.f;
-    if (r + u * step >= end) continue;
-    row4(q.src + (r + u * step) * q.ld, c, q.cols, q.vec, v[u]);
-    if (q.act != VCB_ACT_NONE) row4(q.z + (r + u * step) * q.ldz, c, q.cols, q.vec, t[u]);
-  }
-  if (q.act != VCB_ACT_NONE) {
-#pragma unroll
-    for (int u = 0; u < N; ++u) act_grads(v[u], t[u], q.act);
-  }
-}
-
-// The job and strip (of `width` columns) of strip s of a launch.
-__device__ __forceinline__ const ColJob& strip_of(const ColJobs& a, int& s, int width = 32) {
-  int k = 0;
-  while (k + 1 < a.count) {
-    const int strips = (a.j[k].cols + width - 1) / width;
-    if (s < strips) break;
-    s -= strips;
-    ++k;
-  }
-  return a.j[k];
-}
-
-// Largest entries of every column (a cluster of up to 8 CTAs per strip of 32 columns,
-// a part of the rows each, 8 lanes per row) and of every row (atomic maxima: any
-// order gives the same), column sums in the order of the ranks.
-__global__ void __launch_bounds__(kStripThreads, 4)
-    scales_kernel(const __grid_constant__ ColJobs a) {
-  __shared__ float part[kStripWarps][32], sum_mine[32];
-  __shared__ uint32_t most_part[kStripWarps][32], most_mine[32];
-  let_next_start();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int size = a.cluster, rank = blockIdx.x % size;
-  int strip = blockIdx.x / size;
-  const ColJob& q = strip_of(a, strip);
-  const int c = strip * 32 + (lane & 7) * 4;
-  const long long r0 = q.rows * rank / size, r1 = q.rows * (rank + 1) / size;
-  float sum[4] = {};
-  float most[4] = {};
-  constexpr int U = 4, W = kStripWarps * 4;  // rows in flight per lane, rows of a CTA's step
-  for (long long base = r0 + warp * 4; base < r1; base += U * W) {
-    float v[U][4];
-    job_rows<U>(q, base + (lane >> 3), W, r1, c, v);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long r = base + u * W + (lane >> 3);
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        most[i] = more(most[i], v[u][i]);
-        sum[i] += v[u][i];
-        top = more(top, v[u][i]);
+      for (int u = 0; u < U; ++u) {
+        out[u] = row < q.rows ? q.parts + row * q.ldp + v * 8 : nullptr;
+        if (out[u]) {
+          row4(q.src + row * q.ld, v * 8, q.cols, q.vec, x[u][0]);
+          row4(q.src + row * q.ld, v * 8 + 4, q.cols, q.vec, x[u][1]);
+        }
+        row += down, v += right;
+        if (v >= nv) v -= nv, ++row;
       }
-      if (q.row_most) {
-        uint32_t m = __float_as_uint(top);
 #pragma unroll
-        for (int k = 4; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
-        if ((lane & 7) == 0 && r < r1) atomicMax(q.row_most + r, m);
+      for (int u = 0; u < U; ++u) {
+        if (!out[u]) continue;
+        uint2 lo[kParts], hi[kParts];
+        split4(x[u][0], lo);
+        split4(x[u][1], hi);
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+          *reinterpret_cast<uint4*>(out[u] + k * q.plane) =
+              make_uint4(lo[k].x, lo[k].y, hi[k].x, hi[k].y);
       }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int k = 8; k < 32; k *= 2) {
-      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], k);
-      most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], k));
-    }
-    if (lane < 8) {
-      part[warp][lane * 4 + i] = sum[i];
-      most_part[warp][lane * 4 + i] = __float_as_uint(most[i]);
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    float s = 0.f;
-    uint32_t m = 0;
-    for (int w = 0; w < kStripWarps; ++w) {
-      s += part[w][threadIdx.x];
-      m = max(m, most_part[w][threadIdx.x]);
-    }
-    sum_mine[threadIdx.x] = s;
-    most_mine[threadIdx.x] = m;
-  }
-  cluster_sync();
-  const int col = strip * 32 + threadIdx.x;
-  if (rank == 0 && threadIdx.x < 32 && col < q.cols) {
-    float s = 0.f;
-    uint32_t m = 0;
-    for (int k = 0; k < size; ++k) {
-      s += peer_f32(map_rank(smem_u32(sum_mine + threadIdx.x), k));
-      m = max(m, __float_as_uint(peer_f32(map_rank(smem_u32(most_mine + threadIdx.x), k))));
-    }
-    if (q.sum) q.sum[col] = s;
-    q.col_most[col] = m;
-  }
-  cluster_sync();  // no CTA leaves while its figures are read
-}
-
-constexpr int kHalvesRows = 32;  // rows of a CTA
-
-__global__ void __launch_bounds__(kStripThreads) halves_kernel(const __grid_constant__ ColJobs a) {
-  after_previous();
-  let_next_start();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int block = blockIdx.x / a.wide;
-  int strip = blockIdx.x % a.wide;
-  const ColJob& q = strip_of(a, strip, 128);
-  const int c = strip * 128 + lane * 4;
-  if (c >= q.cols) return;
-  float scale[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) scale[i] = c + i < q.cols ? exp2i(-scale_exp(q.col_most[c + i])) : 0.f;
-  const long long end = min(q.rows, (block + 1LL) * kHalvesRows);
-  constexpr int U = kHalvesRows / kStripWarps;  // rows of a warp
-  const long long r0 = static_cast<long long>(block) * kHalvesRows + warp;
-  float v[U][4];
-  job_rows<U>(q, r0, kStripWarps, end, c, v);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long r = r0 + u * kStripWarps;
-    if (r >= end) break;
-    if (q.by_row)
-      put_halves(q.by_row + r * q.ldh + c, q.plane, v[u], exp2i(-scale_exp(q.row_most[r])));
-    if (q.by_col) {
-      uint2 high, low;
-      halves4(v[u], scale, high, low);
-      __half* at = q.by_col + r * q.ldh + c;
-      *reinterpret_cast<uint2*>(at) = high;
-      *reinterpret_cast<uint2*>(at + q.plane) = low;
     }
   }
 }
 
 // ---- products ----
 struct alignas(64) Prod32 {
-  CUtensorMap a, b;  // (64, rows, 2 halves) boxes
+  CUtensorMap a, b;  // (64, rows, parts) boxes
   int J, I, a_mn, b_mn, tiles_j, tiles_i, nk;
   uint32_t idesc;
-  const uint32_t *most_a, *most_b;  // scales of the rows of A (j) and of B (i)
   Epilogue epi;
 };
 
@@ -339,7 +221,7 @@ struct Launch32 {
   int units0, units, split;
 };
 
-// Sixteen epilogue warps: what they do at a tile's end (scales, activation, stores)
+// Sixteen epilogue warps: what they do at a tile's end (activation, stores)
 // runs beside two stages of the next tile's MMAs only, so it is spread as wide as
 // registers allow.
 constexpr int kEpi = 16, kF32Threads = (kEpi + 2) * 32;
@@ -347,9 +229,9 @@ constexpr int kEpi = 16, kF32Threads = (kEpi + 2) * 32;
 template <int BN, bool PAIR>
 struct Cfg {
   static constexpr int kRowsB = PAIR ? BN / 2 : BN;
-  static constexpr int kBytesB = 2 * kRowsB * 128;
-  static constexpr int kStage = 2 * kBytesA + kBytesB;
-  static constexpr int kStages = 196608 / kStage;
+  static constexpr int kBytesB = kParts * kRowsB * 128;
+  static constexpr int kStage = kParts * kBytesA + kBytesB;
+  static constexpr int kStages = 221184 / kStage;
   static constexpr int kSmem = kStages * kStage + 1024;
   static constexpr int kBufs = BN == 256 ? 2 : 4;
   static constexpr int kColumns = kBufs * BN;  // of tensor memory
@@ -375,17 +257,18 @@ __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Both halves of an operand's rows.  K-major: all h rows, then all l rows.
-// MN-major: per 64 rows, 8 KB of h and 8 KB of l.
+// The parts of an operand's rows.  K-major: all rows of b1, then of b2 and b3.
+// MN-major: per 64 rows, 8 KB of each.
+constexpr uint32_t kBoxMn = kParts * 8192;
 template <bool PAIR>
-__device__ __forceinline__ void load_halves(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+__device__ __forceinline__ void load_parts(uint32_t dst, const CUtensorMap* map, uint32_t bar,
                                             int mn, int row, int rows, int t) {
   if (!mn) {
     if (PAIR) tma_3d_pair(dst, map, bar, t, row); else tma_3d(dst, map, bar, t, row);
   } else {
     for (int q = 0; q < rows; q += 64) {
-      if (PAIR) tma_3d_pair(dst + q * 256, map, bar, row + q, t);
-      else tma_3d(dst + q * 256, map, bar, row + q, t);
+      if (PAIR) tma_3d_pair(dst + q / 64 * kBoxMn, map, bar, row + q, t);
+      else tma_3d(dst + q / 64 * kBoxMn, map, bar, row + q, t);
     }
   }
 }
@@ -467,8 +350,8 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
         if (one) {
           if (!PAIR || rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * C::kStage);
           const uint32_t bar = full0 + s * 8, st = smem + s * C::kStage;
-          load_halves<PAIR>(st, &p.a, bar, a_mn, ja, kTileJ, kb * kBK);
-          load_halves<PAIR>(st + 2 * kBytesA, &p.b, bar, b_mn, ib, C::kRowsB, kb * kBK);
+          load_parts<PAIR>(st, &p.a, bar, a_mn, ja, kTileJ, kb * kBK);
+          load_parts<PAIR>(st + kParts * kBytesA, &p.b, bar, b_mn, ib, C::kRowsB, kb * kBK);
         }
       }
     }
@@ -485,9 +368,11 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
       for (int u = first; ok && u < L.units; u += step) {
         const Prod32& p = L.p[u >= L.units0];
         const int a_mn = p.a_mn, b_mn = p.b_mn, k1 = end(p.nk);
-        const Desc da = operand(smem, a_mn, C::kStage, 16384);
-        const Desc db = operand(smem + 2 * kBytesA, b_mn, C::kStage, 16384);
-        const uint32_t la = (a_mn ? 8192 : kBytesA) >> 4, lb = (b_mn ? 8192 : C::kBytesB / 2) >> 4;
+        const Desc da = operand(smem, a_mn, C::kStage, kBoxMn);
+        const Desc db = operand(smem + kParts * kBytesA, b_mn, C::kStage, kBoxMn);
+        // from a part to the next
+        const uint32_t pa = (a_mn ? 8192 : kBytesA) >> 4;
+        const uint32_t pb = (b_mn ? 8192 : C::kBytesB / kParts) >> 4;
         const uint32_t idesc = p.idesc;
         for (int kb = begin(p.nk); kb < k1;
              ++kb, ++chunks, ring.next(C::kStages), buf.next(C::kBufs)) {
@@ -501,12 +386,16 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
           if (one) {
             const uint32_t d = tmem + buf.s * BN;
             const uint64_t a0 = da.base + ring.s * da.stage, b0 = db.base + ring.s * db.stage;
+            // the smallest products first: what their sums lose is of their size
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) {
-              const uint64_t ah = a0 + k * da.k, bh = b0 + k * db.k;
-              mma_f16<PAIR>(d, ah + la, bh, idesc, k == 0 ? 0u : 1u);
-              mma_f16<PAIR>(d, ah, bh + lb, idesc, 1u);
-              mma_f16<PAIR>(d, ah, bh, idesc, 1u);
+            for (int sum = kParts - 1; sum >= 0; --sum) {
+#pragma unroll
+              for (int p = 0; p <= sum; ++p) {
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k)
+                  mma_f16<PAIR>(d, a0 + p * pa + k * da.k, b0 + (sum - p) * pb + k * db.k, idesc,
+                                sum == kParts - 1 && p == 0 && k == 0 ? 0u : 1u);
+              }
             }
             if (PAIR) {
               commit_pair(&empty[ring.s]);
@@ -576,20 +465,16 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
         break;
       }
       const int I = p.I, J = p.J, j = j0 + (lane & ~3);
-      const int ea = j0 + lane < J ? scale_exp(__ldg(p.most_a + j0 + lane)) : 0;
       float bias[4];
       bias_at<float>(p.epi, J, j, bias);
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
         if (i0 + c < I) {  // warp-uniform
-          const int eb = i0 + c + (lane & 15) < I
-                             ? scale_exp(__ldg(p.most_b + i0 + c + (lane & 15))) : 0;
           Residual<float, 4> res;
           res.fetch(p.epi, I, J, i0 + c + (lane & 3), j);
           float v[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            v[k] = scaled(acc[c + k], ea + __shfl_sync(0xffffffffu, eb, k));
+          for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
           transpose4(v, lane);
           emit<float, 4>(p.epi, I, J, i0 + c + (lane & 3), j, bias, v, res);
         }
@@ -609,10 +494,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
       const int i0 = ti * BN, j = tj * kTileJ + lane * 4;
       const int columns = min(BN, p.I - i0);
       float bias[4];
-      int ea[4];
       bias_at<float>(e, p.J, j, bias);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ea[k] = j + k < p.J ? scale_exp(__ldg(p.most_a + j + k)) : 0;
       for (int c = rank * kEpi + warp; c < columns; c += size * kEpi) {
         const uint32_t at = smem + (c * kTileJ + lane * 4) * 4;
         float v[4] = {};
@@ -620,9 +502,6 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
           const float4 t = peer_f32x4(map_rank(at, k));
           v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
         }
-        const int eb = scale_exp(__ldg(p.most_b + i0 + c));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = scaled(v[k], ea[k] + eb);
         Residual<float, 1> res;
         res.fetch(e, p.I, p.J, i0 + c, j);
         emit<float, 1>(e, p.I, p.J, i0 + c, j, bias, v, res);
@@ -642,24 +521,18 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
 }
 
 // ---- host ----
-// M N K from which the tensor cores are used.  Forward: 64 x 1024 x 1024 (2^26) 12.6
-// us against 15.4 on the FP32 units, 64 x 512 x 512 9.9 against 5.8.  Backward, with
-// two more launches: 146 x 800 x 810 (2^26.5) 40 against 48, 300 x 300 x 1000 28
-// against 36, 512 x 512 x 256 (2^26) 28 against 26, 128 x 512 x 512 30 against 20.
+// M N K from which the tensor cores are used.  Forward: 64 x 1024 x 1024 (2^26) 17 us
+// against 21 on the FP32 units, 512 x 512 x 256 (2^26) 15 against 22, but 64 x 512 x 512
+// 15 against 12 and 128 x 512 x 512 (2^25) 17 against 16.  Both gradients: 146 x 800 x
+// 810 (2^26.5) 26 against 41, 512 x 512 x 256 20 against 32, 128 x 512 x 512 19 against
+// 21, 20000 x 50 x 50 (2^25.6) 106 against 90.
 constexpr long long kTcLeast = 1LL << 26;
 
 long long pad8(long long n) { return (n + 7) / 8 * 8; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-size_t halves_bytes(long long rows, long long cols) { return up256(rows * pad8(cols) * 4); }
-
-// Both halves of a row-major (rows x cols) operand: planes of rows x ld.
-struct Halves {
-  __half* p;
-  int rows, cols;
-  long long ld, plane;
-  uint32_t* most;  // of the rows (or columns) that the product does not sum over
-  bool mn;
-};
+size_t parts_bytes(long long rows, long long cols) {
+  return up256(rows * pad8(cols) * 2 * kParts);
+}
 
 struct Arena {
   uint8_t* at;
@@ -671,19 +544,19 @@ struct Arena {
   }
 };
 
-Halves make_halves(Arena& ws, int rows, int cols, bool mn, uint32_t* most) {
-  Halves h{ws.take<__half>(halves_bytes(rows, cols)), rows, cols, pad8(cols), 0, most, mn};
-  h.plane = h.rows * h.ld;
-  return h;
+Matrix matrix(Arena& ws, const void* p, long long ld, int rows, int cols) {
+  const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0;
+  return {static_cast<const float*>(p), ld, rows, cols, vec,
+          ws.take<__nv_bfloat16>(parts_bytes(rows, cols)), pad8(cols), rows * pad8(cols)};
 }
 
-int make_map(CUtensorMap* map, const Halves& h, int box_rows, const char* who) {
+int make_map(CUtensorMap* map, const Matrix& h, int box_rows, const char* who) {
   const auto fn = encode_fn();
   if (!fn) return fail(VCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
-  const cuuint64_t dims[3] = {(cuuint64_t)h.cols, (cuuint64_t)h.rows, 2};
-  const cuuint64_t strides[2] = {(cuuint64_t)h.ld * 2, (cuuint64_t)h.plane * 2};
-  const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, 2}, estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, h.p, dims, strides, box, estr,
+  const cuuint64_t dims[3] = {(cuuint64_t)h.cols, (cuuint64_t)h.rows, kParts};
+  const cuuint64_t strides[2] = {(cuuint64_t)h.ldp * 2, (cuuint64_t)h.plane * 2};
+  const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, kParts}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, h.parts, dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(VCB_ERR_CUDA, "%s: tensor map encode failed (%d)", who, (int)r);
@@ -697,8 +570,9 @@ struct Plan32 {
 };
 
 // As the 16-bit products' plan: rounds of tiles over the SMs times the stages'
-// cycles (12 MMAs: 1,536 for a pair's tile, 768 for 64 or 128 columns), plus start
-// and epilogue.
+// cycles, plus start and epilogue.  The cycles are measured (24 MMAs alone: 3,072 for a
+// pair's tile, 1,536 for 64 or 128 columns; the operands' way from L2 and the clock
+// under load add the rest).
 struct Shape {
   int I, J, T;
 };
@@ -723,14 +597,14 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
     nk = std::max(nk, ceil(s.T, kBK));
     pairs += ceil(s.I, 256) * ceil(s.J, 256);
   }
-  Plan32 best{true, 256, 1, static_cast<double>(ceil(pairs, sms / 2)) * (nk * 1540 + 4000) + 4000};
+  Plan32 best{true, 256, 1, static_cast<double>(ceil(pairs, sms / 2)) * (nk * 4200 + 4000) + 4000};
   for (int bn : {64, 128}) {
     long long tiles = 0;
     for (const Shape& s : products) tiles += ceil(s.I, bn) * ceil(s.J, kTileJ);
     for (int split : {1, 2, 4, 8}) {
       if (split > nk) break;
       const double t = static_cast<double>(ceil(tiles * split, slots_of(split))) *
-                           (ceil(nk, split) * (bn == 64 ? 800 : 1000) + 4000 + 20.0 * bn) +
+                           (ceil(nk, split) * (bn == 64 ? 1950 : 2700) + 4000 + 20.0 * bn) +
                        (split > 1 ? 1500 + 8.0 * bn : 0);
       if (t < best.cycles) best = {false, bn, split, t};
     }
@@ -738,20 +612,20 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
   return best;
 }
 
-int set_prod(Prod32& r, int I, int J, int T, const Halves& a, const Halves& b, const Plan32& plan,
-             const Epilogue& epi, const char* who) {
+// mn: the operand is contiguous along its row index, not along the contraction.
+int set_prod(Prod32& r, int I, int J, int T, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn,
+             const Plan32& plan, const Epilogue& epi, const char* who) {
   r.I = I, r.J = J;
-  r.a_mn = a.mn, r.b_mn = b.mn;
+  r.a_mn = a_mn, r.b_mn = b_mn;
   const int tj = plan.pair ? 256 : kTileJ;
   r.tiles_j = (J + tj - 1) / tj;
   r.tiles_i = (I + plan.bn - 1) / plan.bn;
   r.nk = std::max(1, (T + kBK - 1) / kBK);
-  r.idesc = idesc_16(VCB_F16, tj, plan.bn, a.mn, b.mn);
-  r.most_a = a.most, r.most_b = b.most;
+  r.idesc = idesc_16(VCB_BF16, tj, plan.bn, a_mn, b_mn);
   r.epi = epi;
   r.epi.vec = vector_rows(epi, 4);
-  int rc = make_map(&r.a, a, a.mn ? kBK : kTileJ, who);
-  if (!rc) rc = make_map(&r.b, b, b.mn ? kBK : plan.pair ? kTileJ : plan.bn, who);
+  int rc = make_map(&r.a, a, a_mn ? kBK : kTileJ, who);
+  if (!rc) rc = make_map(&r.b, b, b_mn ? kBK : plan.pair ? kTileJ : plan.bn, who);
   return rc;
 }
 
@@ -774,8 +648,17 @@ int launch_plan(const Launch32& L, const Plan32& plan, bool chained, cudaStream_
                        : launch<128, false>(L, chained, st, who);
 }
 
-bool vec16(const void* p, long long ld) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0;
+int launch_prep(Prep32& a, cudaStream_t st, const char* who) {
+  long long vectors = 0;
+  for (int k = 0; k < a.flats; ++k)
+    vectors = std::max(vectors, a.flat[k].rows * ((a.flat[k].cols + 7LL) / 8));
+  const long long ctas =
+      std::min<long long>((vectors + kPrepThreads - 1) / kPrepThreads, 4LL * sm_count());
+  a.cluster = 1;  // a CTA's step is 128 rows
+  while (a.strips && a.cluster < 8 && a.dz.rows > 128 * a.cluster) a.cluster *= 2;
+  const long long grid = (a.strips + (ctas + a.cluster - 1) / a.cluster) * a.cluster;
+  return launch_clusters(parts_kernel, a, static_cast<unsigned>(grid), kPrepThreads, 0, a.cluster,
+                         false, st, who);
 }
 
 bool fits(long long M, long long N, long long K, long long least) {
@@ -789,39 +672,20 @@ bool fits(long long M, long long N, long long K, long long least) {
 bool f32_forward_fits(const Fwd& f) { return f.type == VCB_F32 && fits(f.M, f.N, f.K, kTcLeast); }
 
 size_t f32_forward_bytes(int M, int N, int K) {
-  if (!fits(M, N, K, kTcLeast)) return 0;
-  return halves_bytes(M, K) + halves_bytes(N, K) + up256(M * 4LL) + up256(N * 4LL) + 256;
+  return fits(M, N, K, kTcLeast) ? parts_bytes(M, K) + parts_bytes(N, K) + 256 : 0;
 }
 
 int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
   const char* who = "vcb_linear_forward";
   Arena arena{reinterpret_cast<uint8_t*>(up256(reinterpret_cast<size_t>(ws)))};
-  const Halves w = make_halves(arena, f.N, f.K, false, arena.take<uint32_t>(f.N * 4LL));
-  const Halves x = make_halves(arena, f.M, f.K, false, arena.take<uint32_t>(f.M * 4LL));
-  RowJobs jobs{};
-  const auto job = [](const void* p, long long ld, const Halves& h) {
-    return RowJob{static_cast<const float*>(p), ld, h.rows, h.cols, vec16(p, ld), h.p, h.ld,
-                  h.plane, h.most};
-  };
-  jobs.j[0] = job(f.w, f.ldw, w);
-  jobs.j[1] = job(f.x, f.ldx, x);
-  const long long rows = static_cast<long long>(f.N) + f.M;
-  // a warp per row while that keeps a row in registers: what a thread does once is spread
-  // over more entries (1000^3 27.6 -> 25.6 us against a CTA per row)
-  const auto launch_rows = [&](void (*kernel)(RowJobs), int per) {
-    kernel<<<static_cast<unsigned>((rows + per - 1) / per), 256, 0, st>>>(jobs);
-  };
-  if (f.K <= 512)
-    launch_rows(rows_kernel<32, 4>, 8);
-  else if (f.K <= 2048)
-    launch_rows(rows_kernel<32, 16>, 8);
-  else
-    launch_rows(rows_kernel<256, 4>, 1);
-  int rc = check_launch(who);
+  Prep32 prep{};
+  const Matrix w = matrix(arena, f.w, f.ldw, f.N, f.K), x = matrix(arena, f.x, f.ldx, f.M, f.K);
+  prep.flat[0] = w, prep.flat[1] = x, prep.flats = 2;
+  int rc = launch_prep(prep, st, who);
   if (rc) return rc;
   const Plan32 plan = plan_of({{f.M, f.N, f.K}});
   Launch32 L{};
-  rc = set_prod(L.p[0], f.M, f.N, f.K, w, x, plan,
+  rc = set_prod(L.p[0], f.M, f.N, f.K, w, false, x, false, plan,
                 {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0}, who);
   if (rc) return rc;
   L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
@@ -835,52 +699,23 @@ bool f32_backward_fits(const Bwd& b) {
 
 size_t f32_backward_bytes(int M, int N, int K) {
   if (!fits(M, N, K, kTcLeast)) return 0;
-  return 2 * halves_bytes(M, N) + halves_bytes(N, K) + halves_bytes(M, K) + up256(M * 4LL) +
-         up256(N * 4LL) + 2 * up256(K * 4LL) + 256;
+  return parts_bytes(M, N) + parts_bytes(N, K) + parts_bytes(M, K) + 256;
 }
 
 int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   const char* who = "vcb_linear_backward";
   Arena arena{reinterpret_cast<uint8_t*>(up256(reinterpret_cast<size_t>(ws)))};
-  uint32_t* row_most = arena.take<uint32_t>(b.M * 4LL);
-  const Halves dzr = make_halves(arena, b.M, b.N, false, row_most);
-  const Halves dzc = make_halves(arena, b.M, b.N, true, arena.take<uint32_t>(b.N * 4LL));
-  const Halves w = make_halves(arena, b.N, b.K, true, arena.take<uint32_t>(b.K * 4LL));
-  const Halves x = make_halves(arena, b.M, b.K, true, arena.take<uint32_t>(b.K * 4LL));
-  ColJobs jobs{};
-  long long strips = 0, wide = 0, tall = 0;
-  const auto add = [&](const void* p, long long ld, const Halves& h) -> ColJob& {
-    ColJob& q = jobs.j[jobs.count++];
-    q.src = static_cast<const float*>(p);
-    q.ld = ld, q.rows = h.rows, q.cols = h.cols, q.vec = vec16(p, ld);
-    q.col_most = h.most, q.by_col = h.p, q.ldh = h.ld, q.plane = h.plane;
-    strips += (h.cols + 31) / 32;
-    wide += (h.cols + 127) / 128;
-    tall = std::max(tall, q.rows);
-    return q;
-  };
-  ColJob& dz = add(b.dy, b.lddy, dzc);
-  dz.act = b.act, dz.z = static_cast<const float*>(b.z), dz.ldz = b.ldz;
-  if (b.act != VCB_ACT_NONE) dz.vec = dz.vec && vec16(b.z, b.ldz);
-  dz.sum = static_cast<float*>(b.db);
-  if (b.dx) dz.by_row = dzr.p, dz.row_most = row_most;
-  if (!b.dw) dz.by_col = nullptr;
-  if (b.dx) add(b.w, b.ldw, w);
-  if (b.dw) add(b.x, b.ldx, x);
-  const long long blocks = (tall + kHalvesRows - 1) / kHalvesRows;
-  if (strips * 8 > 0x7fffffffLL || wide * blocks > 0x7fffffffLL)
-    return fail(VCB_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d", who, b.M, b.N, b.K);
-  cudaError_t e = cudaSuccess;
-  if (b.dx) e = cudaMemsetAsync(row_most, 0, b.M * 4LL, st);
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  jobs.cluster = 1;  // a CTA's step is 128 rows
-  while (jobs.cluster < 8 && tall > 128 * jobs.cluster) jobs.cluster *= 2;
-  int rc = launch_clusters(scales_kernel, jobs, static_cast<unsigned>(strips * jobs.cluster),
-                           kStripThreads, 0, jobs.cluster, false, st, who);
-  if (rc) return rc;
-  jobs.wide = static_cast<int>(wide);
-  rc = launch_clusters(halves_kernel, jobs, static_cast<unsigned>(wide * blocks), kStripThreads, 0,
-                       1, true, st, who);
+  Prep32 prep{};
+  const Matrix dz = prep.dz = matrix(arena, b.dy, b.lddy, b.M, b.N);
+  const Matrix w = matrix(arena, b.w, b.ldw, b.N, b.K), x = matrix(arena, b.x, b.ldx, b.M, b.K);
+  prep.z = static_cast<const float*>(b.z), prep.ldz = b.ldz, prep.act = b.act;
+  if (b.act != VCB_ACT_NONE)
+    prep.dz.vec = dz.vec && reinterpret_cast<uintptr_t>(b.z) % 16 == 0 && b.ldz % 4 == 0;
+  prep.sum = static_cast<float*>(b.db);
+  prep.strips = (b.N + kStrip - 1) / kStrip;
+  if (b.dx) prep.flat[prep.flats++] = w;
+  if (b.dw) prep.flat[prep.flats++] = x;
+  int rc = launch_prep(prep, st, who);
   if (rc) return rc;
   const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
   const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
@@ -889,11 +724,11 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   const Plan32 both = plan_of({shape_x, shape_w});
   // One launch for both products unless their shapes want different cuts by more than
   // a launch costs.
-  const bool together = b.dx && b.dw && both.cycles < px.cycles + pw.cycles + 4000;
+  const bool together = b.dx && b.dw && both.cycles < px.cycles + pw.cycles + 9000;
   if (together) px = pw = both;
   Launch32 L{};
   if (b.dx) {
-    rc = set_prod(L.p[0], b.M, b.K, b.N, w, dzr, px, ex, who);
+    rc = set_prod(L.p[0], b.M, b.K, b.N, w, true, dz, false, px, ex, who);
     if (rc) return rc;
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
     L.split = px.split;
@@ -904,7 +739,7 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
     }
   }
   Prod32& p = L.p[together ? 1 : 0];
-  rc = set_prod(p, b.N, b.K, b.M, x, dzc, pw, ew, who);
+  rc = set_prod(p, b.N, b.K, b.M, x, true, dz, true, pw, ew, who);
   if (rc) return rc;
   L.units += p.tiles_i * p.tiles_j;
   if (!together) L.units0 = L.units;

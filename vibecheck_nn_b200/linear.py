@@ -9,8 +9,11 @@ that is trained here and bounded by the rest of the package.
 
 ``x`` is (..., K), ``weight`` (N, K) as in a ``gg`` dict's fc layer.  float32,
 bfloat16 and float16, one type per call; sums are held in float32 and each
-output is rounded once.  In float32 a product keeps float32 accuracy (operands
-are split, not rounded, for the tensor cores).  ``act`` is one of 'none',
+output is rounded once.  In float32 a product keeps float32 accuracy: entries are
+split into three bfloat16 parts, not rounded, for the tensor cores, and an output's
+error goes by its own sum of |x w|, whatever else lies in the rows (entries below
+2^-110 are held to 2^-134).  An entry that is not finite makes the outputs that it
+meets infinite or NaN.  ``act`` is one of 'none',
 'relu', 'gelu' (with erf) and 'silu'; a ReLU's slope at 0 is 0.  Work runs on
 the current stream of ``x``'s device; like the tensor-core bounds, a caller
 can ask ``_lib.fault_check`` whether a bounded device wait ran out.
