@@ -709,20 +709,29 @@ size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t ty
  * ignore_index of logsumexp(x_r) - x_r,label, 0 when there is none; ignored
  * rows get gradient 0.  A row whose logits are all -inf has loss +inf and
  * gradient 0; a row whose label is outside [0, C) becomes NaN, and so does the
- * loss.  workspace: vcb_cross_entropy_workspace bytes, 16-byte aligned (NULL when
- * that is 0). */
+ * loss.  grad and logits may not overlap.  workspace: vcb_cross_entropy_workspace
+ * bytes, 16-byte aligned (NULL when that is 0). */
 int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
                       const int64_t* labels, int64_t ignore_index, float* loss, void* grad,
                       int64_t ldg, void* workspace, size_t workspace_bytes, void* stream);
 size_t vcb_cross_entropy_workspace(int32_t R, int32_t C);
 
-/* vcb_linear_forward, vcb_linear_backward and vcb_cross_entropy with their
+/* The same with the gradient times scale[0] (on the device; NULL: 1), multiplied
+ * before the gradient is rounded to the logits' type, and with loss or grad NULL
+ * where only the other is wanted. */
+int vcb_cross_entropy_scaled(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
+                             const int64_t* labels, int64_t ignore_index, const float* scale,
+                             float* loss, void* grad, int64_t ldg, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* vcb_linear_forward, vcb_linear_backward and vcb_cross_entropy(_scaled) with their
  * arguments, in order, as consecutive 64-bit integers (sizes, pointers, the
  * stream): for bindings that pay for every argument they convert.  A size that
  * 32 bits do not hold is refused (VCB_ERR_UNSUPPORTED). */
 int vcb_linear_forward_packed(const int64_t* args);
 int vcb_linear_backward_packed(const int64_t* args);
 int vcb_cross_entropy_packed(const int64_t* args);
+int vcb_cross_entropy_scaled_packed(const int64_t* args);
 
 /* One AdamW step over `count` tensors: tensor i has n[i] weights at p[i] and
  * gradients at g[i], and its moments are the elements [off[i], off[i] + n[i]) of

@@ -17,15 +17,15 @@ def on_the_host(monkeypatch):
         dy, x, w = dy.detach(), x.detach(), w.detach()
         return dy @ w, dy.t() @ x, dy.sum(0) if bias else None
 
-    def value_and_gradient(x, y, ignore_index=-100):
+    def value_and_gradient(x, y, ignore_index, scale=None, want_loss=True, want_grad=True):
         x = x.detach()
         p = torch.softmax(x, 1)
         p[torch.arange(len(y)), y] -= 1
-        return torch.nn.functional.cross_entropy(x, y), p / len(y)
+        return torch.nn.functional.cross_entropy(x, y), p / len(y) * (1 if scale is None else scale)
 
     monkeypatch.setattr(linear, 'linear_forward', forward)
     monkeypatch.setattr(linear, 'linear_backward', backward)
-    monkeypatch.setattr(loss, 'cross_entropy_grad', value_and_gradient)
+    monkeypatch.setattr(loss, '_run', value_and_gradient)
 
 
 def penalties():

@@ -140,10 +140,13 @@ SIGNATURES = {
                             _P, _P, ctypes.c_size_t, _P],
     'vcb_linear_backward_workspace': [_I, _I, _I, _I, _I, _I],
     'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
+    'vcb_cross_entropy_scaled': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _L, _P, ctypes.c_size_t,
+                                 _P],
     'vcb_cross_entropy_workspace': [_I, _I],
     'vcb_linear_forward_packed': [ctypes.c_char_p],
     'vcb_linear_backward_packed': [ctypes.c_char_p],
     'vcb_cross_entropy_packed': [ctypes.c_char_p],
+    'vcb_cross_entropy_scaled_packed': [ctypes.c_char_p],
     'vcb_adamw': [_I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.POINTER(VcbAdamwOpts),
                   _P],
     'vcb_adamw_values': [_L, _P, _P, _P, _P, _P, _P, _P],

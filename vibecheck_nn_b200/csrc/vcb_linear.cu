@@ -487,3 +487,12 @@ extern "C" int vcb_cross_entropy_packed(const int64_t* a) {
                            at<float>(a[7]), at(a[8]), a[9], at(a[10]), static_cast<size_t>(a[11]),
                            at(a[12]));
 }
+
+extern "C" int vcb_cross_entropy_scaled_packed(const int64_t* a) {
+  if (!a) return fail(VCB_ERR_INVALID, "vcb_cross_entropy_scaled_packed: NULL");
+  if (!in_32_bits(a, {0, 1, 2})) return too_large("vcb_cross_entropy_scaled_packed");
+  const auto i = [&](int k) { return static_cast<int32_t>(a[k]); };
+  return vcb_cross_entropy_scaled(i(0), i(1), i(2), at(a[3]), a[4], at<const int64_t>(a[5]), a[6],
+                                  at<const float>(a[7]), at<float>(a[8]), at(a[9]), a[10],
+                                  at(a[11]), static_cast<size_t>(a[12]), at(a[13]));
+}

@@ -50,7 +50,8 @@ struct CeArgs {
   int* tickets;       // one per group
   double* part;       // one partial loss per CTA (per cluster)
   int parts;
-  float* loss;
+  float* loss;         // may be NULL, as g
+  const float* scale;  // factor of the gradient, on the device, or NULL
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -93,6 +94,13 @@ __device__ __forceinline__ float inv_count(const CeArgs& a) {
   return 1.f / static_cast<float>(max(n, 1));
 }
 
+// What a softmax entry of the gradient is multiplied with: the factor comes before the
+// rounding to the logits' type, or loss scaling would multiply what float16 has
+// already lost.
+__device__ __forceinline__ float gradient_scale(const CeArgs& a, float inv) {
+  return a.scale ? inv * *a.scale : inv;
+}
+
 // Loss of a row from its maximum, sum and label's logit.
 __device__ __forceinline__ float row_loss(float m, float s, float xy) {
   return s == 0.f ? INFINITY : logf(s) - (xy - m);
@@ -104,7 +112,7 @@ __device__ void finish(const CeArgs& a, int part, double value, float inv) {
   __shared__ int last;
   __shared__ double sums[32];
   if (a.counts == 0) {
-    if (threadIdx.x == 0) *a.loss = static_cast<float>(value * inv);
+    if (threadIdx.x == 0 && a.loss) *a.loss = static_cast<float>(value * inv);
     return;
   }
   if (threadIdx.x == 0) {
@@ -129,7 +137,7 @@ __device__ void finish(const CeArgs& a, int part, double value, float inv) {
   if (threadIdx.x == 0) {
     t = 0.0;
     for (unsigned w = 0; w < blockDim.x / 32; ++w) t += sums[w];
-    *a.loss = static_cast<float>(t * inv);
+    if (a.loss) *a.loss = static_cast<float>(t * inv);
   }
 }
 
@@ -138,7 +146,7 @@ template <typename T, int G, int PER>
 __global__ void __launch_bounds__(256) ce_small_kernel(const CeArgs a) {
   constexpr int kRows = 256 / G;  // rows of a CTA per step
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  const float inv = inv_count(a);
+  const float inv = inv_count(a), scale = gradient_scale(a, inv);
   double total = 0.0;
   for (long long r0 = static_cast<long long>(blockIdx.x) * kRows; r0 < a.R;
        r0 += static_cast<long long>(gridDim.x) * kRows) {
@@ -168,9 +176,9 @@ __global__ void __launch_bounds__(256) ce_small_kernel(const CeArgs a) {
     }
 #pragma unroll
     for (int k = G / 2; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    if (row) {
-      const float f = bad ? NAN : live && s != 0.f ? inv / s : 0.f;
-      const float one = live && s != 0.f ? inv : 0.f;
+    if (row && a.g) {
+      const float f = bad ? NAN : live && s != 0.f ? scale / s : 0.f;
+      const float one = live && s != 0.f ? scale : 0.f;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int c = lane + G * i;
@@ -326,7 +334,7 @@ __global__ void __launch_bounds__(256) ce_warp_kernel(const CeArgs a) {
   int r = blockIdx.x * 8 + warp;
   long long label = r < a.R ? a.y[r] : a.ignore;
   double total = 0.0;
-  float inv = 0.f;
+  float inv = 0.f, scale = 0.f;
   while (r < a.R) {
     const bool more = r < a.R - step;
     const long long next = more ? a.y[r + step] : a.ignore;
@@ -378,13 +386,14 @@ __global__ void __launch_bounds__(256) ce_warp_kernel(const CeArgs a) {
       // the count of labelled rows (and zeroed tickets) come from the launch before
       asm volatile("griddepcontrol.wait;" ::: "memory");
       inv = inv_count(a);
+      scale = gradient_scale(a, inv);
     }
-    const float f = s != 0.f ? inv / s : 0.f, one = s != 0.f ? inv : 0.f;
+    const float f = s != 0.f ? scale / s : 0.f, one = s != 0.f ? scale : 0.f;
     const int at = static_cast<int>(label) - head, label_vec = read && at >= 0 ? at / VE : -1;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k = lane + 32 * i;
-      if (k < vecs) {
+      if (k < vecs && a.g) {
         float v[VE];
         if (read) {
           unpack<T>(q[i], v);
@@ -411,7 +420,7 @@ __global__ void __launch_bounds__(256) ce_warp_kernel(const CeArgs a) {
         }
       }
     }
-    if (edge >= 0)
+    if (edge >= 0 && a.g)
       g[edge] = from_f32<T>(read ? ex2((xe - m) * kLog2e) * f - (edge == label ? one : 0.f)
                                  : bad ? NAN : 0.f);
     if (live && lane == 0) total += bad ? NAN : row_loss(m, s, xy);
@@ -479,8 +488,10 @@ __global__ void __launch_bounds__(512, 3) ce_row_kernel(const CeArgs a) {
     float v[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) v[i] = fill;
-    for (int b = v0 + tid; b < v1; b += nt) put(b, v);
-    if (edge >= 0) g[edge] = from_f32<T>(fill);
+    if (a.g) {
+      for (int b = v0 + tid; b < v1; b += nt) put(b, v);
+      if (edge >= 0) g[edge] = from_f32<T>(fill);
+    }
     if (label != a.ignore) value = NAN;
     inv = count();
   } else {
@@ -524,10 +535,11 @@ __global__ void __launch_bounds__(512, 3) ce_row_kernel(const CeArgs a) {
       join_lanes<8>(m, s);
     }
     inv = count();
-    const float f = s != 0.f ? inv / s : 0.f, one = s != 0.f ? inv : 0.f;
+    const float scale = gradient_scale(a, inv);
+    const float f = s != 0.f ? scale / s : 0.f, one = s != 0.f ? scale : 0.f;
     const int at = static_cast<int>(label) - head;  // label's place among the vectors' elements
     const int label_vec = at >= 0 ? at / VE : -1;
-    for (int b = v0 + tid; b < v1; b += nt) {
+    for (int b = a.g ? v0 + tid : v1; b < v1; b += nt) {
       float v[VE];
       unpack<T>(STAGED ? slice[b - v0] : xv[b], v);
 #pragma unroll
@@ -543,7 +555,8 @@ __global__ void __launch_bounds__(512, 3) ce_row_kernel(const CeArgs a) {
       }
       put(b, v);
     }
-    if (edge >= 0) g[edge] = from_f32<T>(ex2((xe - m) * kLog2e) * f - (edge == label ? one : 0.f));
+    if (edge >= 0 && a.g)
+      g[edge] = from_f32<T>(ex2((xe - m) * kLog2e) * f - (edge == label ? one : 0.f));
     if (tid == 0) value = row_loss(m, s, to_f32(x[label]));
     if (size > 1) cluster_barrier();  // no CTA leaves while another reads its pair
   }
@@ -649,17 +662,18 @@ extern "C" size_t vcb_cross_entropy_workspace(int32_t R, int32_t C) {
   return kHeader * 4 + (rows / kGroup + 2) / 2 * 8 + rows * sizeof(double);
 }
 
-extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
-                                 const int64_t* labels, int64_t ignore_index, float* loss,
-                                 void* grad, int64_t ldg, void* workspace, size_t workspace_bytes,
-                                 void* stream) {
-  if (R < 0 || C <= 0 || !valid_dtype(type) || ld < C || ldg < C || !loss)
+extern "C" int vcb_cross_entropy_scaled(int32_t R, int32_t C, int32_t type, const void* logits,
+                                        int64_t ld, const int64_t* labels, int64_t ignore_index,
+                                        const float* scale, float* loss, void* grad, int64_t ldg,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (R < 0 || C <= 0 || !valid_dtype(type) || ld < C || (grad && ldg < C))
     return fail(VCB_ERR_INVALID, "vcb_cross_entropy: R=%d C=%d type=%d ld=%lld ldg=%lld", R, C,
                 type, (long long)ld, (long long)ldg);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (R == 0) return cuda_fail(cudaMemsetAsync(loss, 0, sizeof(float), st), "vcb_cross_entropy");
+  if (R == 0)
+    return loss ? cuda_fail(cudaMemsetAsync(loss, 0, sizeof(float), st), "vcb_cross_entropy") : VCB_OK;
   const int eb = dtype_bytes(type);
-  if (!logits || !labels || !grad || reinterpret_cast<uintptr_t>(logits) % eb ||
+  if (!logits || !labels || reinterpret_cast<uintptr_t>(logits) % eb ||
       reinterpret_cast<uintptr_t>(grad) % eb || reinterpret_cast<uintptr_t>(labels) % 8)
     return fail(VCB_ERR_INVALID, "vcb_cross_entropy: NULL or misaligned pointer");
   const size_t need = vcb_cross_entropy_workspace(R, C);
@@ -667,7 +681,7 @@ extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void*
     return fail(VCB_ERR_INVALID, "vcb_cross_entropy: workspace of %zu bytes", workspace_bytes);
   CeArgs a{};
   a.R = R, a.C = C, a.ld = ld, a.ldg = ldg, a.ignore = ignore_index;
-  a.x = logits, a.g = grad, a.loss = loss;
+  a.x = logits, a.g = grad, a.loss = loss, a.scale = scale;
   a.y = reinterpret_cast<const long long*>(labels);
   if (need) {
     a.header = static_cast<int*>(workspace);
@@ -677,4 +691,15 @@ extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void*
   if (type == VCB_F32) return launch<float>(a, st);
   if (type == VCB_BF16) return launch<__nv_bfloat16>(a, st);
   return launch<__half>(a, st);
+}
+
+extern "C" int vcb_cross_entropy(int32_t R, int32_t C, int32_t type, const void* logits, int64_t ld,
+                                 const int64_t* labels, int64_t ignore_index, float* loss,
+                                 void* grad, int64_t ldg, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  if (!loss || (R > 0 && !grad) || ldg < C)
+    return fail(VCB_ERR_INVALID, "vcb_cross_entropy: loss=%p grad=%p ldg=%lld", loss, grad,
+                (long long)ldg);
+  return vcb_cross_entropy_scaled(R, C, type, logits, ld, labels, ignore_index, nullptr, loss, grad,
+                                  ldg, workspace, workspace_bytes, stream);
 }

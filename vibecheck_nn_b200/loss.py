@@ -8,6 +8,10 @@ labelled ``ignore_index`` count for nothing and get gradient 0; with no
 labelled row the loss is 0.  A row whose logits are all ``-inf`` has loss
 ``inf`` and gradient 0.  Labels are not read back to the host: one outside
 [0, C) makes its row's gradient and the loss NaN.
+
+``cross_entropy`` reads the logits once for the loss; its backward pass makes
+the gradient from them, times the upstream factor, before the one rounding to
+their type: a loss scale reaches entries that float16 alone would lose.
 """
 from __future__ import annotations
 
@@ -18,12 +22,11 @@ import torch
 from . import _lib
 from .linear import _p, _workspace_bytes, first_order, rows_of, type_of
 
-_ARGS = struct.Struct('13q').pack
+_ARGS = struct.Struct('14q').pack
 
 
-def cross_entropy_grad(logits, labels, ignore_index=-100):
-    """(loss, d loss / d logits): loss a float32 scalar on the device, the
-    gradient in the logits' type and shape."""
+def _run(logits, labels, ignore_index, scale=None, want_loss=True, want_grad=True):
+    """(loss or None, gradient times ``scale`` (a device scalar) or None)."""
     ty = type_of(logits, 'logits')
     shape = logits.shape
     if not shape or shape[-1] == 0:
@@ -36,31 +39,37 @@ def cross_entropy_grad(logits, labels, ignore_index=-100):
     x2, ld = rows_of(logits, C, logits, 'logits')
     labels = labels.contiguous()
     R = x2.shape[0]
-    grad = logits.new_empty((R, C))
-    loss = logits.new_empty((), dtype=torch.float32)
+    grad = logits.new_empty((R, C)) if want_grad else None
+    loss = logits.new_empty((), dtype=torch.float32) if want_loss else None
     nbytes = _workspace_bytes('vcb_cross_entropy_workspace', R, C)
     ws = _lib.workspace(nbytes, logits.device)
-    rc = _lib.launch_packed(dev, _lib.lib().vcb_cross_entropy_packed, _ARGS, R, C, ty,
-                            x2.data_ptr(), ld, labels.data_ptr(), int(ignore_index),
-                            loss.data_ptr(), grad.data_ptr(), C, _p(ws), nbytes)
+    rc = _lib.launch_packed(dev, _lib.lib().vcb_cross_entropy_scaled_packed, _ARGS, R, C, ty,
+                            x2.data_ptr(), ld, labels.data_ptr(), int(ignore_index), _p(scale),
+                            _p(loss), _p(grad), C, _p(ws), nbytes)
     if rc:
         _lib.check(rc, 'vcb_cross_entropy')
-    return loss, grad if len(shape) == 2 else grad.view(shape)
+    return loss, grad if grad is None or len(shape) == 2 else grad.view(shape)
+
+
+def cross_entropy_grad(logits, labels, ignore_index=-100):
+    """(loss, d loss / d logits): loss a float32 scalar on the device, the
+    gradient in the logits' type and shape."""
+    return _run(logits, labels, ignore_index)
 
 
 class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ignore_index):
-        loss, grad = cross_entropy_grad(logits, labels, ignore_index)
-        ctx.save_for_backward(grad)
-        return loss
+        ctx.ignore_index = ignore_index
+        ctx.save_for_backward(logits, labels)
+        return _run(logits, labels, ignore_index, want_grad=False)[0]
 
     @staticmethod
     def backward(ctx, g):
-        grad, = ctx.saved_tensors
+        logits, labels = ctx.saved_tensors
         with torch.no_grad():
-            out = (grad * g).to(grad.dtype)
-        return (*first_order('cross_entropy', (out,)), None, None)
+            out = _run(logits, labels, ctx.ignore_index, g.float(), want_loss=False)[1:]
+        return (*first_order('cross_entropy', out), None, None)
 
 
 def cross_entropy(logits, labels, ignore_index=-100):
