@@ -226,8 +226,7 @@ def fault_check(device=None):
     """Synchronise ``device``'s current stream and raise ``TimeoutError`` if a
     kernel of the library gave up a bounded wait since the last check (its
     outputs for the unfinished boxes or tiles are NaN).  The drivers call it where
-    they synchronise anyway (each BaB iteration's counter read, the end of a
-    verdict); a caller of the raw operators calls it at its own sync points."""
+    they synchronise anyway (the end of a verdict); a caller of the raw operators calls it at its own sync points."""
     stream = stream_of(device if device is not None else torch.device('cuda'))
     check(lib().vcb_fault_check(stream), 'vcb_fault_check')
 

@@ -4,8 +4,6 @@
 #include <unordered_map>
 
 #include "vcb_common.cuh"
-#include "vcb_crown_tc.cuh"
-#include "vcb_linear.cuh"
 
 namespace vcb {
 
@@ -72,22 +70,18 @@ int ensure_smem(const void* kernel, int bytes) {
 extern "C" int vcb_version(void) { return 101; }
 
 extern "C" int vcb_fault_check(void* stream) {
-  int set = 0;
-  const int rc = vcb::crown_tc_fault_take(static_cast<cudaStream_t>(stream), &set);
-  if (rc) return rc;
-  if (set)
-    return vcb::fail(VCB_ERR_TIMEOUT,
-                     "crown_tc_kernel: a bounded device-side wait expired; the bounds of the "
-                     "boxes it had not finished are NaN");
-  for (const auto take : {vcb::lin::tc_fault_take, vcb::lin::f32_fault_take}) {
-    const int status = take(static_cast<cudaStream_t>(stream), &set);
-    if (status) return status;
-    if (set)
-      return vcb::fail(VCB_ERR_TIMEOUT,
-                       "linear layer: a bounded device-side wait expired; the outputs it had not "
-                       "finished are NaN");
-  }
-  return VCB_OK;
+  int bits = 0;
+  const int rc = vcb::fault_take(static_cast<cudaStream_t>(stream), &bits);
+  if (rc || !bits) return rc;
+  return vcb::fail(VCB_ERR_TIMEOUT, "%s%s",
+                   bits & vcb::kFaultCrown
+                       ? "crown_tc_kernel: a bounded device-side wait expired; the bounds of the "
+                         "boxes it had not finished are NaN. "
+                       : "",
+                   bits & vcb::kFaultLinear
+                       ? "linear layer: a bounded device-side wait expired; the outputs it had not "
+                         "finished are NaN"
+                       : "");
 }
 
 extern "C" const char* vcb_last_error(void) {

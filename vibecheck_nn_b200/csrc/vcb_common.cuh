@@ -27,6 +27,14 @@ int sm_count();
 // Raises a kernel's dynamic shared-memory limit once per (kernel, size).
 int ensure_smem(const void* kernel, int bytes);
 
+// The current device's fault word: kernels with bounded waits set their bit when
+// one runs out (atomicOr).
+constexpr int kFaultCrown = 1, kFaultLinear = 2;
+int fault_word(int** word);
+
+// Its bits after synchronising st; clears them.
+int fault_take(cudaStream_t st, int* bits);
+
 __host__ __device__ inline int pad4(int n) { return (n + 3) & ~3; }
 
 // Smallest multiple of 4 that is >= n and whose quotient by 4 is odd: a row

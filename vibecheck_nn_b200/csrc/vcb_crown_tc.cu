@@ -50,7 +50,9 @@
 // bound proves nothing -- and sets the workspace error word.
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <type_traits>
+#include <unordered_map>
 
 #include "vcb_common.cuh"
 #include "vcb_crown_tc.cuh"
@@ -63,7 +65,8 @@ namespace {
 using namespace tc5;
 
 // Set by crown_tc_kernel when a bounded wait expired (its unfinished boxes
-// got NaN bounds); read and cleared by vcb_fault_check.
+// got NaN bounds) or of the linear layer's (fault bits in vcb_common.cuh); read and
+// cleared by vcb_fault_check.
 __device__ int g_tc_fault;
 
 constexpr int kTB = 128;                   // boxes per tile (MMA rows)
@@ -794,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) crown_tc_kernel(const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   if (threadIdx.x == 0 && failed) {
     atomicExch(p.err, 1);
-    atomicExch(&g_tc_fault, 1);
+    atomicOr(&g_tc_fault, kFaultCrown);
   }
 }
 
@@ -887,7 +890,7 @@ __global__ void __launch_bounds__(64 * kTieBoxes, 1)
   if (kNetSmem) {
     if (tid == 0 && !mbar_wait(bar, 0, kSpin)) {
       failed = 1;
-      atomicExch(&g_tc_fault, 1);
+      atomicOr(&g_tc_fault, kFaultCrown);
       mbar_wait(bar, 0, kSpin);  // let the copy land before the CTA exits
     }
     __syncthreads();
@@ -1287,7 +1290,20 @@ int crown_tc_launch(const vcb_mlp* net, int32_t B, const float* xl, const float*
   return check_launch(who);
 }
 
-int crown_tc_fault_take(cudaStream_t st, int* was_set) {
+int fault_word(int** word) {
+  static std::mutex mu;
+  static std::unordered_map<int, int*> cache;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "fault word");
+  std::lock_guard<std::mutex> lk(mu);
+  int*& at = cache[dev];
+  if (!at) e = cudaGetSymbolAddress(reinterpret_cast<void**>(&at), g_tc_fault);
+  *word = at;
+  return cuda_fail(e, "fault word");
+}
+
+int fault_take(cudaStream_t st, int* bits) {
   int h = 0;
   cudaError_t e = cudaMemcpyFromSymbolAsync(&h, g_tc_fault, sizeof(int), 0,
                                             cudaMemcpyDeviceToHost, st);
@@ -1297,7 +1313,7 @@ int crown_tc_fault_take(cudaStream_t st, int* was_set) {
     e = cudaMemcpyToSymbolAsync(g_tc_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   }
-  *was_set = h;
+  *bits = h;
   return cuda_fail(e, "vcb_fault_check");
 }
 

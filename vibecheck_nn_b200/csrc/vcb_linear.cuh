@@ -260,11 +260,6 @@ bool f32_backward_fits(const Bwd& b);
 size_t f32_backward_bytes(int M, int N, int K);
 int f32_backward(const Bwd& b, void* ws, cudaStream_t st);
 
-// Reads and clears the fault word of the 16-bit / float32 tensor-core kernels
-// after synchronising st; *was_set = 1 when a bounded wait had run out.
-int tc_fault_take(cudaStream_t st, int* was_set);
-int f32_fault_take(cudaStream_t st, int* was_set);
-
 }  // namespace lin
 
 }  // namespace vcb

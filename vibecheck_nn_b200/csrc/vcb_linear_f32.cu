@@ -32,7 +32,6 @@
 // for the rest.
 #include <algorithm>
 #include <array>
-#include <atomic>
 #include <initializer_list>
 
 #include "vcb_linear_tc.cuh"
@@ -40,9 +39,6 @@
 namespace vcb {
 namespace lin {
 namespace {
-
-__device__ int g_f32_fault;
-std::atomic<bool> g_launched{false};
 
 constexpr int kParts = 3;
 constexpr uint32_t kLargest16 = 0x7F7F0000u;  // of bfloat16, as a float's bits
@@ -219,6 +215,7 @@ struct alignas(64) Prod32 {
 struct Launch32 {
   Prod32 p[2];
   int units0, units, split;
+  int* fault;
 };
 
 // Sixteen epilogue warps: what they do at a tile's end (activation, stores)
@@ -517,7 +514,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_consta
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                    "r"(C::kColumns));
   }
-  if (threadIdx.x == 0 && failed) atomicExch(&g_f32_fault, 1);
+  if (threadIdx.x == 0 && failed) atomicOr(L.fault, kFaultLinear);
 }
 
 // ---- host ----
@@ -630,18 +627,18 @@ int set_prod(Prod32& r, int I, int J, int T, const Matrix& a, bool a_mn, const M
 }
 
 template <int BN, bool PAIR>
-int launch(const Launch32& L, bool chained, cudaStream_t st, const char* who) {
+int launch(Launch32& L, bool chained, cudaStream_t st, const char* who) {
   using C = Cfg<BN, PAIR>;
-  g_launched = true;
   const auto kernel = f32_kernel<BN, PAIR>;
-  const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
+  int rc = fault_word(&L.fault);
+  if (!rc) rc = ensure_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
   if (rc) return rc;
   const int size = PAIR ? 2 : L.split;
   return launch_clusters(kernel, L, size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units),
                          kF32Threads, C::kSmem, size, chained, st, who);
 }
 
-int launch_plan(const Launch32& L, const Plan32& plan, bool chained, cudaStream_t st,
+int launch_plan(Launch32& L, const Plan32& plan, bool chained, cudaStream_t st,
                 const char* who) {
   if (plan.pair) return launch<256, true>(L, chained, st, who);
   return plan.bn == 64 ? launch<64, false>(L, chained, st, who)
@@ -745,22 +742,6 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (!together) L.units0 = L.units;
   L.split = pw.split;
   return launch_plan(L, pw, together || !b.dx, st, who);
-}
-
-int f32_fault_take(cudaStream_t st, int* was_set) {
-  *was_set = 0;
-  if (!g_launched) return VCB_OK;
-  int h = 0;
-  cudaError_t e =
-      cudaMemcpyFromSymbolAsync(&h, g_f32_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && h) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbolAsync(g_f32_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
-  *was_set = h;
-  return cuda_fail(e, "vcb_fault_check");
 }
 
 }  // namespace lin

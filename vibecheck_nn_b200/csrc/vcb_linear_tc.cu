@@ -35,16 +35,12 @@
 // for its copies and MMAs in flight, frees its tensor memory and returns.
 #include <algorithm>
 #include <array>
-#include <atomic>
 
 #include "vcb_linear_tc.cuh"
 
 namespace vcb {
 namespace lin {
 namespace {
-
-__device__ int g_tc16_fault;
-std::atomic<bool> g_launched{false};
 
 struct alignas(64) Prod {
   CUtensorMap a, b;
@@ -62,6 +58,7 @@ struct Launch {
   int units0, units;  // tiles of the first product, of both
   int split;          // split_kernel: CTAs per tile of the first product (cluster size)
   int stages;
+  int* fault;
 };
 
 // W columns of the accumulator, NaN if !ok.
@@ -294,7 +291,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   cluster_sync();
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-  if (threadIdx.x == 0 && failed) atomicExch(&g_tc16_fault, 1);
+  if (threadIdx.x == 0 && failed) atomicOr(L.fault, kFaultLinear);
 }
 
 // One tile per CTA; the tiles of the first product are shared by the
@@ -427,7 +424,7 @@ __global__ void __launch_bounds__(kThreads)
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(columns));
-  if (threadIdx.x == 0 && failed) atomicExch(&g_tc16_fault, 1);
+  if (threadIdx.x == 0 && failed) atomicOr(L.fault, kFaultLinear);
   if (size == 1) return;
   cluster_sync();
   if (parts > 1 && warp < kEpiWarps) {
@@ -723,10 +720,11 @@ int set_prod(Prod& r, int type, int I, int J, int T, const Operand& a, const Ope
 
 template <typename T>
 int launch_tc(Launch& L, const Plan& plan, bool chained, cudaStream_t st, const char* who) {
-  g_launched = true;
+  int rc = fault_word(&L.fault);
+  if (rc) return rc;
   if (plan.pair) {
     const auto kernel = pair_kernel<T>;
-    const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), kPairSmem);
+    rc = ensure_smem(reinterpret_cast<const void*>(kernel), kPairSmem);
     if (rc) return rc;
     const int grid = 2 * std::min(L.units, sm_count() / 2);
     return launch_clusters(kernel, L, grid, kPairThreads, kPairSmem, 2, chained, st, who);
@@ -743,7 +741,7 @@ int launch_tc(Launch& L, const Plan& plan, bool chained, cudaStream_t st, const 
   L.stages = std::max(2, std::min({kMostStages, nk, room / stage}));
   L.split = plan.split;
   const int smem = std::max(L.stages * stage, plan.split > 1 ? bn * kTileJ * 4 : 0) + 1024;
-  const int rc = ensure_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - 1024);
+  rc = ensure_smem(reinterpret_cast<const void*>(kernel), 227 * 1024 - 1024);
   if (rc) return rc;
   return launch_clusters(kernel, L, static_cast<unsigned>(clusters * plan.split), kThreads, smem,
                          plan.split, chained, st, who);
@@ -917,22 +915,6 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
     rc = launch_type(L, plan, b.type, prepared && (together || !b.dx), st, who);
   }
   return rc;
-}
-
-int tc_fault_take(cudaStream_t st, int* was_set) {
-  *was_set = 0;
-  if (!g_launched) return VCB_OK;
-  int h = 0;
-  cudaError_t e =
-      cudaMemcpyFromSymbolAsync(&h, g_tc16_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && h) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbolAsync(g_tc16_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
-  *was_set = h;
-  return cuda_fail(e, "vcb_fault_check");
 }
 
 }  // namespace lin
