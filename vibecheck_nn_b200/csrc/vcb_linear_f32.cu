@@ -27,14 +27,14 @@
 // Preparation is bound by HBM: one launch reads each operand once and writes its
 // three parts (backward: dz = dy act'(z) and db in strips of columns, W and X flat
 // beside them).  The parts of dz serve both products, read along either index.
-// Then products as in vcb_linear_tc.cu: f32_kernel<256, true> in CTA pairs for
-// large ones, f32_kernel<64 / 128, false> with the contraction cut over a cluster
+// Then products as in vcb_linear_tc.cu: sum_kernel<float, 3, 256, true> in CTA pairs for
+// large ones, sum_kernel<float, 3, 64 / 128, false> with the contraction cut over a cluster
 // for the rest.
 #include <algorithm>
 #include <array>
 #include <initializer_list>
 
-#include "vcb_linear_tc.cuh"
+#include "vcb_linear_sum.cuh"
 
 namespace vcb {
 namespace lin {
@@ -204,319 +204,6 @@ __global__ void __launch_bounds__(kPrepThreads, 4) parts_kernel(const __grid_con
   }
 }
 
-// ---- products ----
-struct alignas(64) Prod32 {
-  CUtensorMap a, b;  // (64, rows, parts) boxes
-  int J, I, a_mn, b_mn, tiles_j, tiles_i, nk;
-  uint32_t idesc;
-  Epilogue epi;
-};
-
-struct Launch32 {
-  Prod32 p[2];
-  int units0, units, split;
-  int* fault;
-};
-
-// Sixteen epilogue warps: what they do at a tile's end (activation, stores)
-// runs beside two stages of the next tile's MMAs only, so it is spread as wide as
-// registers allow.
-constexpr int kEpi = 16, kF32Threads = (kEpi + 2) * 32;
-
-template <int BN, bool PAIR>
-struct Cfg {
-  static constexpr int kRowsB = PAIR ? BN / 2 : BN;
-  static constexpr int kBytesB = kParts * kRowsB * 128;
-  static constexpr int kStage = kParts * kBytesA + kBytesB;
-  static constexpr int kStages = 221184 / kStage;
-  static constexpr int kSmem = kStages * kStage + 1024;
-  static constexpr int kBufs = BN == 256 ? 2 : 4;
-  static constexpr int kColumns = kBufs * BN;  // of tensor memory
-  static constexpr int kCols = BN / (kEpi / 4);  // of an epilogue thread
-  static constexpr int kArrivals = kEpi * (PAIR ? 2 : 1);
-};
-
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                       int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
-      "bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
-      : "memory");
-}
-
-// The parts of an operand's rows.  K-major: all rows of b1, then of b2 and b3.
-// MN-major: per 64 rows, 8 KB of each.
-constexpr uint32_t kBoxMn = kParts * 8192;
-template <bool PAIR>
-__device__ __forceinline__ void load_parts(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int mn, int row, int rows, int t) {
-  if (!mn) {
-    if (PAIR) tma_3d_pair(dst, map, bar, t, row); else tma_3d(dst, map, bar, t, row);
-  } else {
-    for (int q = 0; q < rows; q += 64) {
-      if (PAIR) tma_3d_pair(dst + q / 64 * kBoxMn, map, bar, row + q, t);
-      else tma_3d(dst + q / 64 * kBoxMn, map, bar, row + q, t);
-    }
-  }
-}
-
-// One tile of `out` per unit of work.  PAIR: persistent CTA pairs, 256 x 256.
-// Otherwise a 128 x BN tile per cluster of L.split CTAs, each with a part of the
-// contraction (none, where it has fewer stages than CTAs); the parts are joined in the order of the ranks.
-template <int BN, bool PAIR>
-__global__ void __launch_bounds__(kF32Threads, 1) f32_kernel(const __grid_constant__ Launch32 L) {
-  using C = Cfg<BN, PAIR>;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
-  __shared__ __align__(8) uint64_t acc_full[C::kBufs], acc_free[C::kBufs], done;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int failed;
-  const volatile int* vfailed = &failed;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = ctarank();
-  const int size = PAIR ? 2 : L.split;
-  const int first = blockIdx.x / size, step = PAIR ? gridDim.x / 2 : L.units;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int q = 0; q < C::kBufs; ++q) {
-      mbar_init(&acc_full[q], 1);
-      mbar_init(&acc_free[q], C::kArrivals);
-    }
-    mbar_init(&done, 1);
-    failed = 0;
-    mbar_fence_init();
-  }
-  if (warp == 0) {
-    if (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                       smem_u32(&tmem_slot)),
-                   "r"(C::kColumns));
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                       smem_u32(&tmem_slot)),
-                   "r"(C::kColumns));
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-  }
-  fence_before_sync();
-  __syncthreads();
-  if (PAIR) cluster_sync();  // barriers of both CTAs are ready
-  fence_after_sync();
-  after_previous();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  // the part of a contraction of nk stages
-  const auto begin = [&](int nk) { return PAIR ? 0 : static_cast<int>((long long)nk * rank / size); };
-  const auto end = [&](int nk) {
-    return PAIR ? nk : static_cast<int>((long long)nk * (rank + 1) / size);
-  };
-
-  if (warp == kEpi) {  // TMA producer
-    const bool one = elect_one();
-    unsigned g = 0;
-    Ring ring;
-    bool ok = true;
-    const uint32_t full0 = PAIR ? map_rank(smem_u32(full), 0) : smem_u32(full);
-    for (int u = first; ok && u < L.units; u += step) {
-      const Prod32& p = L.p[u >= L.units0];
-      int ti, tj;
-      tile_at(p.tiles_i, p.tiles_j, u >= L.units0 ? u - L.units0 : u, ti, tj);
-      const int ja = PAIR ? (tj * 2 + rank) * kTileJ : tj * kTileJ;
-      const int ib = PAIR ? (ti * 2 + rank) * C::kRowsB : ti * BN;
-      const int a_mn = p.a_mn, b_mn = p.b_mn, k1 = end(p.nk);
-      for (int kb = begin(p.nk); kb < k1; ++kb, ++g, ring.next(C::kStages)) {
-        const int s = ring.s;
-        if (g >= C::kStages && !mbar_wait(&empty[s], ring.parity ^ 1, kSpinLimit, vfailed)) {
-          ok = false;
-          break;
-        }
-        if (one) {
-          if (!PAIR || rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * C::kStage);
-          const uint32_t bar = full0 + s * 8, st = smem + s * C::kStage;
-          load_parts<PAIR>(st, &p.a, bar, a_mn, ja, kTileJ, kb * kBK);
-          load_parts<PAIR>(st + kParts * kBytesA, &p.b, bar, b_mn, ib, C::kRowsB, kb * kBK);
-        }
-      }
-    }
-    if (!ok) failed = 1;
-    if (!PAIR || rank == 0)  // the copies in flight land before the CTAs leave
-      for (unsigned k = g > C::kStages ? g - C::kStages : 0; k < g; ++k)
-        if (!mbar_wait(&full[k % C::kStages], (k / C::kStages) & 1, kSpinLimit)) failed = 1;
-  } else if (warp == kEpi + 1) {  // MMA issuer
-    if (!PAIR || rank == 0) {
-      const bool one = elect_one();
-      Ring ring, buf;
-      unsigned chunks = 0;
-      bool ok = true;
-      for (int u = first; ok && u < L.units; u += step) {
-        const Prod32& p = L.p[u >= L.units0];
-        const int a_mn = p.a_mn, b_mn = p.b_mn, k1 = end(p.nk);
-        const Desc da = operand(smem, a_mn, C::kStage, kBoxMn);
-        const Desc db = operand(smem + kParts * kBytesA, b_mn, C::kStage, kBoxMn);
-        // from a part to the next
-        const uint32_t pa = (a_mn ? 8192 : kBytesA) >> 4;
-        const uint32_t pb = (b_mn ? 8192 : C::kBytesB / kParts) >> 4;
-        const uint32_t idesc = p.idesc;
-        for (int kb = begin(p.nk); kb < k1;
-             ++kb, ++chunks, ring.next(C::kStages), buf.next(C::kBufs)) {
-          if (!mbar_wait(&full[ring.s], ring.parity, kSpinLimit, vfailed) ||
-              (chunks >= C::kBufs &&
-               !mbar_wait(&acc_free[buf.s], buf.parity ^ 1, kDoneLimit, vfailed))) {
-            ok = false;
-            break;
-          }
-          fence_after_sync();
-          if (one) {
-            const uint32_t d = tmem + buf.s * BN;
-            const uint64_t a0 = da.base + ring.s * da.stage, b0 = db.base + ring.s * db.stage;
-            // the smallest products first: what their sums lose is of their size
-#pragma unroll
-            for (int sum = kParts - 1; sum >= 0; --sum) {
-#pragma unroll
-              for (int p = 0; p <= sum; ++p) {
-#pragma unroll
-                for (int k = 0; k < kBK / 16; ++k)
-                  mma_f16<PAIR>(d, a0 + p * pa + k * da.k, b0 + (sum - p) * pb + k * db.k, idesc,
-                                sum == kParts - 1 && p == 0 && k == 0 ? 0u : 1u);
-              }
-            }
-            if (PAIR) {
-              commit_pair(&empty[ring.s]);
-              commit_pair(&acc_full[buf.s]);
-            } else {
-              mma_commit(&empty[ring.s]);
-              mma_commit(&acc_full[buf.s]);
-            }
-          }
-        }
-      }
-      if (!ok) failed = 1;
-      if (one) {  // every MMA has finished before tensor memory is freed
-        if (PAIR) commit_pair(&done); else mma_commit(&done);
-      }
-    }
-    if (!mbar_wait(&done, 0, kDoneLimit)) failed = 1;
-  } else {
-    constexpr int kCols = C::kCols;
-    const int quad = warp & 3, col0 = (warp >> 2) * kCols;
-    const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + col0;
-    Ring buf;
-    bool ok = true;
-    for (int u = first; u < L.units; u += step) {
-      const Prod32& p = L.p[u >= L.units0];
-      int ti, tj;
-      tile_at(p.tiles_i, p.tiles_j, u >= L.units0 ? u - L.units0 : u, ti, tj);
-      const int j0 = (PAIR ? (tj * 2 + rank) * kTileJ : tj * kTileJ) + quad * 32;
-      const int i0 = ti * BN + col0;
-      const int chunks = end(p.nk) - begin(p.nk);
-      float acc[kCols];
-#pragma unroll
-      for (int k = 0; k < kCols; ++k) acc[k] = 0.f;
-      for (int kb = 0; ok && kb < chunks; ++kb, buf.next(C::kBufs)) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf.s], buf.parity, kDoneLimit, vfailed));
-        if (!ok) break;
-        fence_after_sync();
-#pragma unroll
-        for (int c = 0; c < kCols; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(base + buf.s * BN + c, r);
-          tmem_wait_ld(r);
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            acc[c + k] = __fadd_rn(acc[c + k], __uint_as_float(r[k]));
-        }
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR)
-            arrive_leader(&acc_free[buf.s]);
-          else
-            mbar_arrive(&acc_free[buf.s]);
-        }
-      }
-      if (!ok) {
-#pragma unroll
-        for (int k = 0; k < kCols; ++k) acc[k] = NAN;
-      }
-      if (!PAIR && size > 1) {  // partial sums where the stages were
-#pragma unroll
-        for (int k = 0; k < kCols; ++k)
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(
-                           smem + ((col0 + k) * kTileJ + quad * 32 + lane) * 4),
-                       "f"(acc[k])
-                       : "memory");
-        break;
-      }
-      const int I = p.I, J = p.J, j = j0 + (lane & ~3);
-      float bias[4];
-      bias_at<float>(p.epi, J, j, bias);
-#pragma unroll
-      for (int c = 0; c < kCols; c += 16) {
-        if (i0 + c < I) {  // warp-uniform
-          Residual<float, 4> res;
-          res.fetch(p.epi, I, J, i0 + c + (lane & 3), j);
-          float v[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = acc[c + k];
-          transpose4(v, lane);
-          emit<float, 4>(p.epi, I, J, i0 + c + (lane & 3), j, bias, v, res);
-        }
-      }
-    }
-    if (!ok) failed = 1;
-  }
-  fence_before_sync();
-  __syncthreads();
-  if (PAIR || size > 1) cluster_sync();
-  if (!PAIR && size > 1) {
-    if (warp < kEpi) {
-      const Prod32& p = L.p[first >= L.units0];
-      int ti, tj;
-      tile_at(p.tiles_i, p.tiles_j, first >= L.units0 ? first - L.units0 : first, ti, tj);
-      const Epilogue e = p.epi;
-      const int i0 = ti * BN, j = tj * kTileJ + lane * 4;
-      const int columns = min(BN, p.I - i0);
-      float bias[4];
-      bias_at<float>(e, p.J, j, bias);
-      for (int c = rank * kEpi + warp; c < columns; c += size * kEpi) {
-        const uint32_t at = smem + (c * kTileJ + lane * 4) * 4;
-        float v[4] = {};
-        for (int k = 0; k < size; ++k) {
-          const float4 t = peer_f32x4(map_rank(at, k));
-          v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
-        }
-        Residual<float, 1> res;
-        res.fetch(e, p.I, p.J, i0 + c, j);
-        emit<float, 1>(e, p.I, p.J, i0 + c, j, bias, v, res);
-      }
-    }
-    cluster_sync();  // no CTA leaves while its partial sums are read
-  }
-  if (warp == 0) {
-    if (PAIR)
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                   "r"(C::kColumns));
-    else
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                   "r"(C::kColumns));
-  }
-  if (threadIdx.x == 0 && failed) atomicOr(L.fault, kFaultLinear);
-}
-
 // ---- host ----
 // M N K from which the tensor cores are used.  Forward: 64 x 1024 x 1024 (2^26) 17 us
 // against 21 on the FP32 units, 512 x 512 x 256 (2^26) 15 against 22, but 64 x 512 x 512
@@ -547,19 +234,6 @@ Matrix matrix(Arena& ws, const void* p, long long ld, int rows, int cols) {
           ws.take<__nv_bfloat16>(parts_bytes(rows, cols)), pad8(cols), rows * pad8(cols)};
 }
 
-int make_map(CUtensorMap* map, const Matrix& h, int box_rows, const char* who) {
-  const auto fn = encode_fn();
-  if (!fn) return fail(VCB_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
-  const cuuint64_t dims[3] = {(cuuint64_t)h.cols, (cuuint64_t)h.rows, kParts};
-  const cuuint64_t strides[2] = {(cuuint64_t)h.ldp * 2, (cuuint64_t)h.plane * 2};
-  const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, kParts}, estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, h.parts, dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(VCB_ERR_CUDA, "%s: tensor map encode failed (%d)", who, (int)r);
-  return VCB_OK;
-}
-
 struct Plan32 {
   bool pair;
   int bn, split;
@@ -577,10 +251,10 @@ struct Shape {
 // CTAs at a time in clusters of 1, 2, 4 and 8.
 int slots_of(int size) {
   static const std::array<int, 4> slots = [] {
-    using C = Cfg<128, false>;
+    using C = Cfg<kParts, 128, false>;
     std::array<int, 4> n;
     for (int k = 0; k < 4; ++k)
-      n[k] = cluster_slots(f32_kernel<128, false>, kF32Threads, C::kSmem, 1 << k);
+      n[k] = cluster_slots(sum_kernel<float, kParts, 128, false>, kSumThreads, C::kSmem, 1 << k);
     return n;
   }();
   return slots[size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
@@ -609,40 +283,20 @@ Plan32 plan_of(std::initializer_list<Shape> products) {
   return best;
 }
 
-// mn: the operand is contiguous along its row index, not along the contraction.
-int set_prod(Prod32& r, int I, int J, int T, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn,
+int set_prod(SumProd& r, int I, int J, int T, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn,
              const Plan32& plan, const Epilogue& epi, const char* who) {
-  r.I = I, r.J = J;
-  r.a_mn = a_mn, r.b_mn = b_mn;
-  const int tj = plan.pair ? 256 : kTileJ;
-  r.tiles_j = (J + tj - 1) / tj;
-  r.tiles_i = (I + plan.bn - 1) / plan.bn;
-  r.nk = std::max(1, (T + kBK - 1) / kBK);
-  r.idesc = idesc_16(VCB_BF16, tj, plan.bn, a_mn, b_mn);
-  r.epi = epi;
-  r.epi.vec = vector_rows(epi, 4);
-  int rc = make_map(&r.a, a, a_mn ? kBK : kTileJ, who);
-  if (!rc) rc = make_map(&r.b, b, b_mn ? kBK : plan.pair ? kTileJ : plan.bn, who);
-  return rc;
+  const auto of = [](const Matrix& m, bool mn) {
+    return SumOperand{m.parts, static_cast<int>(m.rows), m.cols, m.ldp, m.plane, mn};
+  };
+  return set_sum<kParts>(r, VCB_BF16, I, J, T, of(a, a_mn), of(b, b_mn), plan.bn, plan.pair, epi, 4,
+                         who);
 }
 
-template <int BN, bool PAIR>
-int launch(Launch32& L, bool chained, cudaStream_t st, const char* who) {
-  using C = Cfg<BN, PAIR>;
-  const auto kernel = f32_kernel<BN, PAIR>;
-  int rc = fault_word(&L.fault);
-  if (!rc) rc = ensure_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
-  if (rc) return rc;
-  const int size = PAIR ? 2 : L.split;
-  return launch_clusters(kernel, L, size * (PAIR ? std::min(L.units, sm_count() / 2) : L.units),
-                         kF32Threads, C::kSmem, size, chained, st, who);
-}
-
-int launch_plan(Launch32& L, const Plan32& plan, bool chained, cudaStream_t st,
+int launch_plan(SumLaunch& L, const Plan32& plan, bool chained, cudaStream_t st,
                 const char* who) {
-  if (plan.pair) return launch<256, true>(L, chained, st, who);
-  return plan.bn == 64 ? launch<64, false>(L, chained, st, who)
-                       : launch<128, false>(L, chained, st, who);
+  if (plan.pair) return launch_sum<float, kParts, 256, true>(L, chained, st, who);
+  return plan.bn == 64 ? launch_sum<float, kParts, 64, false>(L, chained, st, who)
+                       : launch_sum<float, kParts, 128, false>(L, chained, st, who);
 }
 
 int launch_prep(Prep32& a, cudaStream_t st, const char* who) {
@@ -681,7 +335,7 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st) {
   int rc = launch_prep(prep, st, who);
   if (rc) return rc;
   const Plan32 plan = plan_of({{f.M, f.N, f.K}});
-  Launch32 L{};
+  SumLaunch L{};
   rc = set_prod(L.p[0], f.M, f.N, f.K, w, false, x, false, plan,
                 {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0}, who);
   if (rc) return rc;
@@ -723,7 +377,7 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   // a launch costs.
   const bool together = b.dx && b.dw && both.cycles < px.cycles + pw.cycles + 9000;
   if (together) px = pw = both;
-  Launch32 L{};
+  SumLaunch L{};
   if (b.dx) {
     rc = set_prod(L.p[0], b.M, b.K, b.N, w, true, dz, false, px, ex, who);
     if (rc) return rc;
@@ -735,7 +389,7 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
       L.units0 = L.units = 0;
     }
   }
-  Prod32& p = L.p[together ? 1 : 0];
+  SumProd& p = L.p[together ? 1 : 0];
   rc = set_prod(p, b.N, b.K, b.M, x, true, dz, true, pw, ew, who);
   if (rc) return rc;
   L.units += p.tiles_i * p.tiles_j;

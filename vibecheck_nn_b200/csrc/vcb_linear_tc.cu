@@ -25,6 +25,8 @@
 //    weight is what is read, and every SM takes part in reading it).  The
 //    partial sums are joined over distributed shared memory in the order of
 //    the ranks: no atomics, no second launch, the same bits every time.
+// A contraction that would give one accumulator more than kLongest stages goes to
+// sum_kernel (vcb_linear_sum.cuh), which empties accumulators on the way.
 // Measured: bf16 8192 x 8192 x 4096 with GELU, residual and pre-activation 350 us in
 // short bursts (1,570 TFLOP/s, 93 % of the library's measured rate), 465 us back to back
 // under the power cap (1,180); 4096^3 105 us; 2048 x 8192 x 1024 with the same epilogue
@@ -36,7 +38,7 @@
 #include <algorithm>
 #include <array>
 
-#include "vcb_linear_tc.cuh"
+#include "vcb_linear_sum.cuh"
 
 namespace vcb {
 namespace lin {
@@ -755,6 +757,46 @@ int launch_type(Launch& L, const Plan& plan, int type, bool chained, cudaStream_
 
 namespace {
 
+// One accumulator would take more than kLongest stages of a contraction of T entries.
+bool too_long(const Plan& plan, int T) {
+  const int nk = (T + kBK - 1) / kBK;
+  return (nk + plan.split - 1) / plan.split > kLongest;
+}
+
+// out(i, j) = sum_t b(i, t) a(j, t) for long T: cycles as in plan_of.
+template <typename E>
+int launch_long(int type, int I, int J, int T, const Operand& a, const Operand& b,
+                const Epilogue& epi, bool chained, cudaStream_t st, const char* who) {
+  const auto ceil = [](long long x, long long y) { return (x + y - 1) / y; };
+  const long long nk = ceil(T, kBK), tiles = ceil(I, 128) * ceil(J, kTileJ);
+  double least = static_cast<double>(ceil(ceil(I, 256) * ceil(J, 256), sm_count() / 2)) *
+                     (nk * 540 + 4000) + 4000;
+  SumLaunch L{};
+  for (int split : {1, 2, 4, 8}) {
+    const double t = static_cast<double>(ceil(tiles * split, slots_of(split))) *
+                         (ceil(nk, split) * 560 + 6500) + (split > 1 ? 2500 : 0);
+    if (t < least) least = t, L.split = split;
+  }
+  const bool pair = L.split == 0;
+  const auto of = [&](const Operand& o, int rows) {
+    const int r = o.mn ? T : rows;
+    return SumOperand{o.p, r, o.mn ? rows : T, o.ld, r * o.ld, o.mn};
+  };
+  const int rc = set_sum<1>(L.p[0], type, I, J, T, of(a, J), of(b, I), pair ? 256 : 128, pair, epi,
+                            2, who);
+  if (rc) return rc;
+  L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
+  return pair ? launch_sum<E, 1, 256, true>(L, chained, st, who)
+              : launch_sum<E, 1, 128, false>(L, chained, st, who);
+}
+
+int long_product(int type, int I, int J, int T, const Operand& a, const Operand& b,
+                 const Epilogue& epi, bool chained, cudaStream_t st, const char* who) {
+  return type == VCB_BF16
+             ? launch_long<__nv_bfloat16>(type, I, J, T, a, b, epi, chained, st, who)
+             : launch_long<__half>(type, I, J, T, a, b, epi, chained, st, who);
+}
+
 // M N K from which the tensor cores are used.  As the operands lie: bf16 64 x 256 x
 // 256 (2^22) 4.9 us against 5.4 on the FP32 units, 100 x 200 x 200 9.2 against 11.3,
 // 8 x 1024 x 1024 backward 10 against 45.  With a launch that prepares them: 128 x
@@ -835,11 +877,14 @@ int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
   int rc = launch_prep(prep, f.type, st, who);
   if (rc) return rc;
   const Plan plan = plan_of(f.M, f.N, f.K, true, false);
+  const Epilogue epi{f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
+  if (too_long(plan, f.K))
+    return long_product(f.type, f.M, f.N, f.K, a, b, epi, prep.copies > 0, st, who);
   Launch L{};
   Prod& p = L.p[0];
   rc = set_prod(p, f.type, f.M, f.N, f.K, a, b, plan.bn, plan.pair, who);
   if (rc) return rc;
-  p.epi = {f.y, f.z, f.bias, f.res, f.ldy, f.ldz, f.ldr, f.act, 0};
+  p.epi = epi;
   p.epi.vec = vector_rows(p.epi, 2);
   L.units0 = L.units = p.tiles_i * p.tiles_j;
   return launch_type(L, plan, f.type, prep.copies > 0, st, who);
@@ -880,30 +925,39 @@ int tc_backward(const Bwd& b, void* ws, cudaStream_t st) {
   int rc = launch_prep(prep, b.type, st, who);
   if (rc) return rc;
   const bool prepared = prep.strips || prep.copies;
-  // dX and dW share a launch when both are pairs or both are not; the contraction of
-  // dW, the rows, is then not cut
+  // dX and dW share a launch when both are pairs or both are not, and both are short
+  // enough for one accumulator; the contraction of dW, the rows, is then not cut
   const Plan px = plan_of(b.M, b.K, b.N, true, false), pw = plan_of(b.N, b.K, b.M, true, true);
   Launch L{};
   Operand dzt = dz;
   dzt.mn = true;
-  const bool together = b.dx && b.dw && px.pair == pw.pair;
-  if (b.dx) {
+  const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
+  const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+  const bool long_x = b.dx && too_long(px, b.N), long_w = b.dw && too_long(pw, b.M);
+  const bool together = b.dx && b.dw && px.pair == pw.pair && !long_x &&
+                        !too_long({pw.pair, pw.bn, 1}, b.M);
+  if (long_x) {
+    rc = long_product(b.type, b.M, b.K, b.N, w, dz, ex, prepared, st, who);
+    if (rc) return rc;
+  } else if (b.dx) {
     rc = set_prod(L.p[0], b.type, b.M, b.K, b.N, w, dz, px.bn, px.pair, who);
     if (rc) return rc;
-    L.p[0].epi = {b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
+    L.p[0].epi = ex;
     L.p[0].epi.vec = vector_rows(L.p[0].epi, 2);
     L.units0 = L.units = L.p[0].tiles_i * L.p[0].tiles_j;
   }
-  if (b.dx && !together) {
+  if (b.dx && !long_x && !together) {
     rc = launch_type(L, px, b.type, prepared, st, who);
     if (rc) return rc;
     L.units0 = L.units = 0;
   }
+  if (long_w)
+    return long_product(b.type, b.N, b.K, b.M, x, dzt, ew, prepared && !b.dx, st, who);
   if (b.dw) {
     Prod& p = L.p[1];
     rc = set_prod(p, b.type, b.N, b.K, b.M, x, dzt, pw.bn, pw.pair, who);
     if (rc) return rc;
-    p.epi = {b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
+    p.epi = ew;
     p.epi.vec = vector_rows(p.epi, 2);
     L.units += p.tiles_i * p.tiles_j;
     Plan plan = pw;
