@@ -3,12 +3,14 @@
     m = b1 m + (1 - b1) g            v = b2 v + (1 - b2) g^2
     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 
+with t counted per parameter: the steps in which it had a gradient.
+
 The moments of all tensors lie in one flat buffer; tensor i starts at
 ``offsets[i]``, a multiple of 256.  ``state_bits=8`` keeps codes with one
 float32 scale per 256 elements (``m = s sgn(c) (c/127)^2``, ``v = s
 (c/255)^4``): 2 bytes per weight instead of 8.  Codes are rounded up or down
 with the probability that keeps a moment's mean, from a hash of the element's
-place, the step and ``seed``, so a run is repeatable.  A gradient that is not
+place, the step t and ``seed``, so a run is repeatable.  A gradient that is not
 finite makes its block of 256 moments NaN.
 
 Weights are updated in place, in float32 arithmetic, rounded once to their own
@@ -46,6 +48,7 @@ class AdamW:
             raise ValueError(f'lr {lr}, betas {betas}, eps {eps}')
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
         self.state_bits, self.seed, self.t = state_bits, int(seed), 0
+        self._counts = [0] * len(self.params)  # of each parameter's own steps
         self.device = self.params[0].device
         self._types = [type_of(p, f'parameter {i}') for i, p in enumerate(self.params)]
         self._one_type = len(set(self._types)) == 1
@@ -69,16 +72,16 @@ class AdamW:
             self.m_scale = new(total // BLOCK, torch.float32)
             self.v_scale = new(total // BLOCK, torch.float32)
 
-    def _opts(self):
+    def _opts(self, t):
         b1, b2 = self.betas
-        t = self.t
         return _lib.VcbAdamwOpts(b1, 1 - b1, b2, 1 - b2, self.eps, self.lr / (1 - b1 ** t),
                                  (1 - b2 ** t) ** -0.5, 1 - self.lr * self.weight_decay,
                                  (self.seed * 0xBB67AE85 + t * 0x6A09E667) & _MASK32)
 
     def step(self, grads=None):
         """One step with ``grads`` (by default every parameter's ``.grad``); a
-        parameter whose gradient is None stays as it is."""
+        parameter whose gradient is None stays as it is, moments and step count
+        (the t of its bias corrections) included."""
         ps = self.params
         grads = [p.grad for p in ps] if grads is None else list(grads)
         if len(grads) != len(ps):
@@ -86,11 +89,14 @@ class AdamW:
         self._check_params()
         groups = self._groups(grads)
         self.t += 1
-        opts = self._opts()
         m, v = self.m.data_ptr(), self.v.data_ptr()
         ms, vs = _p(self.m_scale), _p(self.v_scale)
         step = _lib.lib().vcb_adamw
-        for pt, gt, idx, gp in groups:
+        counts = self._counts
+        for pt, gt, t, idx, gp in groups:
+            opts = self._opts(t)
+            for i in idx:
+                counts[i] = t
             if idx is self._all:
                 pp, (sizes, offsets) = array('Q', [p.data_ptr() for p in ps]), self._arrays
             else:
@@ -124,16 +130,17 @@ class AdamW:
                                  'was built')
 
     def _groups(self, grads):
-        """[(weights' type, gradients' type, indices, gradient pointers)], one
-        entry per launch."""
+        """[(weights' type, gradients' type, step count, indices, gradient
+        pointers)], one entry per launch."""
         here = self.device.index
+        counts = self._counts
         if not any([g is None for g in grads]):  # usually one type, and nothing to copy
             first = grads[0].dtype
-            if self._one_type and (first == torch.float32 or first == self._dtypes[0]) \
+            if self._one_type and counts.count(counts[0]) == len(counts) and (first == torch.float32 or first == self._dtypes[0]) \
                     and [g.shape for g in grads] == self._shapes \
                     and all([g.dtype is first and g.get_device() == here and g.is_contiguous()
                              for g in grads]):
-                return [(self._types[0], TYPES[first], self._all,
+                return [(self._types[0], TYPES[first], counts[0] + 1, self._all,
                          [g.data_ptr() for g in grads])]
         groups = {}
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
@@ -144,15 +151,15 @@ class AdamW:
                                  f'{tuple(shape)} on {self.device}')
             if not g.is_contiguous():
                 grads[i] = g = g.contiguous()  # grads keeps it until the launch
-            key = (self._types[i], g.dtype)
+            key = (self._types[i], g.dtype, counts[i] + 1)
             group = groups.get(key)
             if group is None:
                 if g.dtype != torch.float32 and g.dtype != self._dtypes[i]:
                     raise _lib.UnsupportedInput(f'vibecheck_nn_b200: gradient {i} of type '
                                                 f'{g.dtype}; the weight\'s or float32')
-                group = groups[key] = (key[0], TYPES[g.dtype], [], [])
-            group[2].append(i)
-            group[3].append(g.data_ptr())
+                group = groups[key] = (key[0], TYPES[g.dtype], key[2], [], [])
+            group[3].append(i)
+            group[4].append(g.data_ptr())
         return groups.values()
 
     def moments(self):
@@ -174,12 +181,17 @@ class AdamW:
         return {k: getattr(self, k) for k in names}
 
     def state_dict(self):
-        """The step count, the seed and copies of the state's buffers."""
-        return {'step': self.t, 'seed': self.seed,
+        """The step counts (of the optimiser and of each parameter), the seed and
+        copies of the state's buffers."""
+        return {'step': self.t, 'steps': list(self._counts), 'seed': self.seed,
                 **{k: t.clone() for k, t in self._buffers().items()}}
 
     def load_state_dict(self, state):
-        """Takes over a state of the same tensors and ``state_bits``."""
+        """Takes over a state of the same tensors and ``state_bits``; one without
+        ``steps`` counts ``step`` for every parameter."""
+        counts = [int(n) for n in state.get('steps', [state['step']] * len(self.params))]
+        if len(counts) != len(self.params):
+            raise ValueError(f'state of {len(counts)} parameters, expected {len(self.params)}')
         for k, t in self._buffers().items():
             s = state[k]
             if s.shape != t.shape or s.dtype != t.dtype:
@@ -187,7 +199,7 @@ class AdamW:
                                  f'{tuple(t.shape)}')
         for k, t in self._buffers().items():
             t.copy_(state[k])
-        self.t = int(state['step'])
+        self.t, self._counts = int(state['step']), counts
         self.seed = int(state.get('seed', self.seed))
 
 
