@@ -17,7 +17,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import linear, loss, ops, optim, workloads
+from . import _lib, linear, loss, ops, optim, workloads
 
 
 class MlpTrainer:
@@ -70,7 +70,9 @@ class MlpTrainer:
         return value
 
     def layers(self):
-        """The network as float32 (W, b) arrays."""
+        """The network as float32 (W, b) arrays; raises ``TimeoutError`` if a
+        bounded device wait ran out while it was trained."""
+        _lib.fault_check(self.weights[0].device)
         return [(W.float().cpu().numpy(), b.float().cpu().numpy())
                 for W, b in zip(self.weights, self.biases)]
 
