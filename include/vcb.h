@@ -704,6 +704,15 @@ int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type, const voi
 size_t vcb_linear_backward_workspace(int32_t M, int32_t N, int32_t K, int32_t type,
                                      int32_t act, int32_t rows16);
 
+/* Which kernel a product of these calls takes (for tests and measurements):
+ * product 0 forward, 1 dX, 2 dW of a backward pass that wants both.  0 the kernels
+ * for few rows, 1 the FP32 units, 2 tensor cores with the contraction cut over a
+ * cluster, 3 tensor cores in CTA pairs, 4 and 5 the same with accumulators emptied
+ * on the way (16-bit contractions beyond 8,192 entries per accumulator); -1 for
+ * arguments the calls refuse.  act and rows16 as above. */
+int vcb_linear_path(int32_t M, int32_t N, int32_t K, int32_t type, int32_t product, int32_t act,
+                    int32_t rows16);
+
 /* Softmax cross-entropy of logits (R x C) with int64 labels (R), and its
  * gradient (R x C): loss[0] = mean over the rows whose label is not
  * ignore_index of logsumexp(x_r) - x_r,label, 0 when there is none; ignored

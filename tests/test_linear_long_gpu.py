@@ -82,3 +82,18 @@ def test_input_gradients(M, N, K, dtype):
     dx, _, _ = linear.linear_backward(dy, x, w, z, 'relu')
     within(dx, want)
     _lib.fault_check()
+
+
+@pytest.mark.parametrize('dtype', list(HALF))
+def test_the_sizes_above_reach_what_they_mean(dtype):
+    t = linear.TYPES[dtype]
+    path = lambda M, N, K, product, aligned=1: \
+        _lib.lib().vcb_linear_path(M, N, K, t, product, 0, aligned)  # noqa: E731
+    cut, pairs = 4, 5
+    assert path(8192, 512, 512, 2) < cut  # the longest of one accumulator
+    assert path(131_072, 64, 64, 2) == cut and path(1_048_576, 200, 64, 2) == cut
+    assert path(12_000, 2048, 1500, 2) in (cut, pairs) and path(131_072, 2048, 2048, 2) == pairs
+    assert path(70_001, 131, 67, 2, 0) == cut
+    assert path(300, 260, 100_000, 0) == cut and path(2048, 1999, 20_000, 0) == pairs
+    assert path(200, 100_000, 180, 1) == cut and path(2048, 20_000, 2048, 1) == pairs
+    assert path(9_000, 9_500, 600, 1) >= cut and path(9_000, 9_500, 600, 2) >= cut

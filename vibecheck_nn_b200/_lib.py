@@ -139,6 +139,7 @@ SIGNATURES = {
     'vcb_linear_backward': [_I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _L,
                             _P, _P, ctypes.c_size_t, _P],
     'vcb_linear_backward_workspace': [_I, _I, _I, _I, _I, _I],
+    'vcb_linear_path': [_I] * 7,
     'vcb_cross_entropy': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _L, _P, ctypes.c_size_t, _P],
     'vcb_cross_entropy_scaled': [_I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _L, _P, ctypes.c_size_t,
                                  _P],

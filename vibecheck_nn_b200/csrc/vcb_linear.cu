@@ -444,6 +444,23 @@ extern "C" int vcb_linear_backward(int32_t M, int32_t N, int32_t K, int32_t type
                                                       static_cast<cudaStream_t>(stream));
 }
 
+extern "C" int vcb_linear_path(int32_t M, int32_t N, int32_t K, int32_t type, int32_t product,
+                               int32_t act, int32_t aligned) {
+  if (M < 0 || N < 0 || K < 0 || !valid_dtype(type) || product < 0 || product > 2) return -1;
+  if (product == 0 ? few_rows_forward(M, N, K, type) : few_rows_backward(M, N, K, type)) return 0;
+  // operands whose rows start on 16-byte boundaries, or all of them one element further
+  const auto* p = reinterpret_cast<const void*>(static_cast<uintptr_t>(aligned ? 4096 : 4100));
+  auto* q = const_cast<void*>(p);
+  const auto ld = [&](int n) { return aligned ? (n + 7LL) / 8 * 8 : n + 0LL; };
+  const lin::Fwd f{M, N, K, type, act, ld(K), ld(K), 0, ld(N), 0, p, p, nullptr, nullptr, q, nullptr};
+  const lin::Bwd b{M, N, K, type, act, ld(N), ld(K), ld(K), ld(N), ld(K), ld(K), p, p, p, p, q, q, q};
+  if (type == VCB_F32)
+    return (product == 0 ? lin::f32_forward_fits(f) : lin::f32_backward_fits(b))
+               ? lin::f32_path(M, N, K, product) : 1;
+  return (product == 0 ? lin::tc_forward_fits(f) : lin::tc_backward_fits(b))
+             ? lin::tc_path(M, N, K, product) : 1;
+}
+
 // Pointers of a packed argument list.
 template <typename T = void>
 static T* at(int64_t v) {

@@ -252,6 +252,7 @@ int tc_forward(const Fwd& f, void* ws, cudaStream_t st);
 bool tc_backward_fits(const Bwd& b);
 size_t tc_backward_bytes(int M, int N, int K, int act, bool rows16);
 int tc_backward(const Bwd& b, void* ws, cudaStream_t st);
+int tc_path(int M, int N, int K, int product);  // as vcb_linear_path, sizes that fit
 
 bool f32_forward_fits(const Fwd& f);
 size_t f32_forward_bytes(int M, int N, int K);
@@ -259,6 +260,7 @@ int f32_forward(const Fwd& f, void* ws, cudaStream_t st);
 bool f32_backward_fits(const Bwd& b);
 size_t f32_backward_bytes(int M, int N, int K);
 int f32_backward(const Bwd& b, void* ws, cudaStream_t st);
+int f32_path(int M, int N, int K, int product);
 
 }  // namespace lin
 

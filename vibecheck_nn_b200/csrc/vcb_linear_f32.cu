@@ -353,6 +353,30 @@ size_t f32_backward_bytes(int M, int N, int K) {
   return parts_bytes(M, N) + parts_bytes(N, K) + parts_bytes(M, K) + 256;
 }
 
+namespace {
+// One launch for both products unless their shapes want different cuts by more than
+// a launch costs.
+struct BackwardPlan {
+  Plan32 x, w;
+  bool together;
+};
+
+BackwardPlan backward_plan(int M, int N, int K, bool dx, bool dw) {
+  const Shape x{M, K, N}, w{N, K, M};
+  BackwardPlan p{plan_of({x}), plan_of({w}), false};
+  const Plan32 both = plan_of({x, w});
+  p.together = dx && dw && both.cycles < p.x.cycles + p.w.cycles + 9000;
+  if (p.together) p.x = p.w = both;
+  return p;
+}
+}  // namespace
+
+int f32_path(int M, int N, int K, int product) {
+  if (product == 0) return plan_of({{M, N, K}}).pair ? 3 : 2;
+  const BackwardPlan p = backward_plan(M, N, K, true, true);
+  return (product == 1 ? p.x : p.w).pair ? 3 : 2;
+}
+
 int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   const char* who = "vcb_linear_backward";
   Arena arena{reinterpret_cast<uint8_t*>(up256(reinterpret_cast<size_t>(ws)))};
@@ -370,13 +394,9 @@ int f32_backward(const Bwd& b, void* ws, cudaStream_t st) {
   if (rc) return rc;
   const Epilogue ex{b.dx, nullptr, nullptr, nullptr, b.lddx, 0, 0, VCB_ACT_NONE, 0};
   const Epilogue ew{b.dw, nullptr, nullptr, nullptr, b.lddw, 0, 0, VCB_ACT_NONE, 0};
-  const Shape shape_x{b.M, b.K, b.N}, shape_w{b.N, b.K, b.M};
-  Plan32 px = plan_of({shape_x}), pw = plan_of({shape_w});
-  const Plan32 both = plan_of({shape_x, shape_w});
-  // One launch for both products unless their shapes want different cuts by more than
-  // a launch costs.
-  const bool together = b.dx && b.dw && both.cycles < px.cycles + pw.cycles + 9000;
-  if (together) px = pw = both;
+  const BackwardPlan plan = backward_plan(b.M, b.N, b.K, b.dx, b.dw);
+  const Plan32 px = plan.x, pw = plan.w;
+  const bool together = plan.together;
   SumLaunch L{};
   if (b.dx) {
     rc = set_prod(L.p[0], b.M, b.K, b.N, w, true, dz, false, px, ex, who);

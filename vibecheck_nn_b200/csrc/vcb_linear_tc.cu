@@ -763,20 +763,27 @@ bool too_long(const Plan& plan, int T) {
   return (nk + plan.split - 1) / plan.split > kLongest;
 }
 
-// out(i, j) = sum_t b(i, t) a(j, t) for long T: cycles as in plan_of.
-template <typename E>
-int launch_long(int type, int I, int J, int T, const Operand& a, const Operand& b,
-                const Epilogue& epi, bool chained, cudaStream_t st, const char* who) {
+// CTAs of a cluster per tile of a long product, 0 for pairs: cycles as in plan_of.
+int long_plan(int I, int J, int T) {
   const auto ceil = [](long long x, long long y) { return (x + y - 1) / y; };
   const long long nk = ceil(T, kBK), tiles = ceil(I, 128) * ceil(J, kTileJ);
   double least = static_cast<double>(ceil(ceil(I, 256) * ceil(J, 256), sm_count() / 2)) *
                      (nk * 540 + 4000) + 4000;
-  SumLaunch L{};
+  int best = 0;
   for (int split : {1, 2, 4, 8}) {
     const double t = static_cast<double>(ceil(tiles * split, slots_of(split))) *
                          (ceil(nk, split) * 560 + 6500) + (split > 1 ? 2500 : 0);
-    if (t < least) least = t, L.split = split;
+    if (t < least) least = t, best = split;
   }
+  return best;
+}
+
+// out(i, j) = sum_t b(i, t) a(j, t) for long T.
+template <typename E>
+int launch_long(int type, int I, int J, int T, const Operand& a, const Operand& b,
+                const Epilogue& epi, bool chained, cudaStream_t st, const char* who) {
+  SumLaunch L{};
+  L.split = long_plan(I, J, T);
   const bool pair = L.split == 0;
   const auto of = [&](const Operand& o, int rows) {
     const int r = o.mn ? T : rows;
@@ -888,6 +895,14 @@ int tc_forward(const Fwd& f, void* ws, cudaStream_t st) {
   p.epi.vec = vector_rows(p.epi, 2);
   L.units0 = L.units = p.tiles_i * p.tiles_j;
   return launch_type(L, plan, f.type, prep.copies > 0, st, who);
+}
+
+int tc_path(int M, int N, int K, int product) {
+  const int I = product == 2 ? N : M, J = product == 0 ? N : K;
+  const int T = product == 0 ? K : product == 1 ? N : M;
+  const Plan plan = plan_of(I, J, T, true, product == 2);
+  if (!too_long(plan, T)) return plan.pair ? 3 : 2;
+  return long_plan(I, J, T) ? 4 : 5;
 }
 
 bool tc_backward_fits(const Bwd& b) {
