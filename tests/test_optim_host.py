@@ -14,6 +14,7 @@ def host_adamw(monkeypatch):
     """An optimiser of CPU tensors whose launches are recorded, not made."""
     made = []
     monkeypatch.setattr(optim, 'type_of', lambda t, name: linear.TYPES[t.dtype])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
     monkeypatch.setattr(_lib, 'launch', lambda *args: made.append(args) or 0)
 
     def build(*params, **kw):
@@ -142,3 +143,12 @@ def test_a_parameter_that_starts_late_steps_as_torch_would(bits):
         if bits == 32:
             for p, q in zip(ps, qs):
                 assert float((p - q.detach()).abs().max()) <= 1e-6 * (step + 1) * 4
+
+
+def test_adamw_refuses_to_be_captured(host_adamw, monkeypatch):
+    build, made = host_adamw
+    opt = build(torch.ones(4))
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='captured'):
+        opt.step([torch.ones(4)])
+    assert not made and opt.t == 0

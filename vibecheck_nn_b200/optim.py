@@ -18,7 +18,8 @@ type (float32, bfloat16, float16: in 16 bits a step below half a unit in the
 last place is lost); gradients have the weights' type or float32.  A parameter
 keeps the type, shape, device and contiguous layout that it had when the optimiser
 was built; a step refuses (``ValueError``) one that a conversion of its module
-has changed.
+has changed.  The step's constants are computed on the host, so a step refuses to be
+captured in a CUDA graph (``RuntimeError``).
 """
 from __future__ import annotations
 
@@ -82,6 +83,9 @@ class AdamW:
         """One step with ``grads`` (by default every parameter's ``.grad``); a
         parameter whose gradient is None stays as it is, moments and step count
         (the t of its bias corrections) included."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW.step cannot be captured in a CUDA graph: its constants go by '
+                               'the step count on the host')
         ps = self.params
         grads = [p.grad for p in ps] if grads is None else list(grads)
         if len(grads) != len(ps):
