@@ -341,8 +341,8 @@ namespace {
 bool misaligned(const void* p, int type) {
   return reinterpret_cast<uintptr_t>(p) % dtype_bytes(type) != 0;
 }
-// Which calls take the kernels for few rows (vcb_linear_rows.cu).  Times in us with
-// cold inputs, theirs first.  Forward: fp32 8 x 4096 x 4096 33 against 50, 16 x 1024 x
+// Which calls take the kernels for few rows (vcb_linear_rows.cu).  Times in us of single
+// calls between two events with cold inputs, theirs first.  Forward: fp32 8 x 4096 x 4096 33 against 50, 16 x 1024 x
 // 1024 11 against 14, 16 x 2048 x 2048 20 against 35, but 16 x 4096 x 4096 51 against
 // 48; bf16 1 x 4096 x 4096 16 against 18, x 4097 18 against 34, 2 x 4096 x 4097 23
 // against 35, 4 x 1024 x 1024 8 against 12, but 4 x 4096 x 4096 22 against 18.

@@ -24,8 +24,8 @@
 // of bfloat16), 680 us back to back under the power cap, both gradients 1,065 us;
 // largest error 1.7e-7 of the largest output, against 1.1e-6 of an fp32 sum.
 //
-// Preparation is bound by HBM: one launch reads each operand once and writes its
-// three parts (backward: dz = dy act'(z) and db in strips of columns, W and X flat
+// Preparation (two 2048^2 operands: 16 us, 27 % of DRAM, 56 % of issue slots): one
+// launch reads each operand once and writes its three parts (backward: dz = dy act'(z) and db in strips of columns, W and X flat
 // beside them).  The parts of dz serve both products, read along either index.
 // Then products as in vcb_linear_tc.cu: sum_kernel<float, 3, 256, true> in CTA pairs for
 // large ones, sum_kernel<float, 3, 64 / 128, false> with the contraction cut over a cluster

@@ -13,10 +13,11 @@
 // dz that are in shared memory anyway.  The ranges of a strip are a cluster, joined
 // over distributed shared memory in order.  All sums are in fp32.
 //
-// Measured with cold inputs, launch included (16 us of forward hold 5 of HBM): bf16 1
-// row 4096 x 4096 forward 16 us, backward 31 us (10 of HBM); fp32 8 rows 33 us (10)
-// and 49 us (20).  Loads of several rows are in flight past conversions and stores:
-// without that the backward took 47 and 66 us.
+// Measured with cold inputs, on the device (calls in a captured graph): bf16 1 row 4096
+// x 4096 forward 10.4 us (5 of HBM), backward 25 us (10 of HBM); fp32 8 rows 25 us (10)
+// and 42 us (20).  Single calls between two events, as in the rules of vcb_linear.cu:
+// 16, 31, 33 and 49 us.  Loads of several rows are in flight past conversions and
+// stores: without that the backward took 47 and 66 us.
 #include <algorithm>
 
 #include "vcb_linear_tc.cuh"

@@ -13,9 +13,10 @@
 // 8 KB stay in the registers of a warp, of up to 128 classes in those of 8 or 32
 // lanes without vectors.
 //
-// Measured: bf16 8192 x 131072 830 us with 3 rows of 10 ignored, 1,000 us with none
-// (4.3 TB/s; exponentials and conversions of both passes fill the issue slots), 2048 x
-// 50001 106 us (3.9 TB/s), fp32 100 x 10 one launch.
+// Measured: bf16 8192 x 131072 830 us with 3 rows of 10 ignored, 870 to 1,000 us with none
+// (4.3 TB/s; the two passes of a row, 64 % of issue slots together, wait for the
+// cluster in turn), 2048 x 50001 106 us (3.9 TB/s), fp32 100 x 10 one launch.  The loss
+// alone: 556 us with 1 row of 5 ignored (870 with the gradient), 75 and 12.
 //
 // A row without any class left (all logits -inf) has loss +inf and gradient
 // 0.  A label outside [0, C) that is not ignore_index makes its row and the
