@@ -62,3 +62,23 @@ def test_a_graph_that_is_not_used_does_no_harm(on_the_host, k):
     want, = torch.autograd.grad(values[k](), x)
     got, = torch.autograd.grad(values[k](), x, create_graph=True)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_on_the_gpu(dtype):
+    gen = torch.Generator('cuda').manual_seed(0)
+    x = torch.randn(40, 64, device='cuda', generator=gen).to(dtype).requires_grad_(True)
+    w = torch.randn(32, 64, device='cuda', generator=gen).to(dtype).requires_grad_(True)
+    y = torch.randint(0, 32, (40,), device='cuda', generator=gen)
+    for value in (lambda: linear.linear(x, w, None, 'silu').float().square().sum(),
+                  lambda: loss.cross_entropy(x @ w.t(), y)):
+        want, = torch.autograd.grad(value(), x)
+        got, = torch.autograd.grad(value(), x, create_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            got.float().square().sum().backward()
+    r = torch.randn(40, 32, device='cuda', generator=gen).to(dtype).requires_grad_(True)
+    g, = torch.autograd.grad(linear.linear(x, w, residual=r).float().square().sum(), r,
+                             create_graph=True)
+    assert g.requires_grad  # the residual's gradient is the upstream's, to any order
